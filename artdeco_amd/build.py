@@ -24,8 +24,10 @@ ARCH = "gfx950"
 # it replaces.  Whole step 2.44 -> 2.21 ms with it off: raster bwd 0.73 -> 0.62, raster fwd 0.35 -> 0.29, projection
 # bwd 0.345 -> 0.29, SSIM fwd 0.060 -> 0.052, LoD fwd 0.070 -> 0.060 ms; nothing got slower.  Results are unchanged
 # where they are compared bit-exactly (packed ops are the same IEEE operations per element).
+# -packed-fp32-ops (a feature of the device pass; the host pass warns that it does not know it): no v_pk_add/mul/fma_f32 from any other
+# pass either -- some of their forms have given wrong results on this hardware now and then.
 COMMON_FLAGS = ["--offload-arch=" + ARCH, "-O3", "-std=c++17", "-fPIC", "-Wall", "-Wno-unused-function",
-                "-fno-slp-vectorize", "-I" + CSRC, "-I" + os.path.join(os.path.dirname(HERE), "include")]
+                "-fno-slp-vectorize", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-I" + CSRC, "-I" + os.path.join(os.path.dirname(HERE), "include")]
 
 # Per-file extra flags.  IEEE-unfused arithmetic wherever the result feeds an
 # integer decision (radii, tile ids, sort keys) or is compared bit-exactly
