@@ -1,0 +1,137 @@
+"""An MLP's activation whose backward pass reads its input from 8 bits (csrc/activation8.hip), and the MLP that keeps nothing else.
+
+A float16 MLP layer keeps fc1's output for the activation's gradient and the activation's output for fc2's weight gradient: 4 bytes a
+hidden value.  Here the forward pass leaves one code a value, 32 consecutive values sharing a power of two (33/32 byte a value), and the
+backward pass takes both from it.  int8 holds a value to 1/254 .. 1/127 of its block's largest, e4m3 to 1/16 of itself; forward
+results are exact, gradients are those of the held values."""
+from __future__ import annotations
+
+from typing import NamedTuple
+
+import torch
+import torch.nn.functional as F
+
+from artdeco_amd import _lib
+
+_DTYPES = {torch.float16: 0, torch.float32: 1, torch.bfloat16: 2}
+_KINDS = {"gelu": 0, "gelu_tanh": 1, "silu": 2}
+_FORMATS = {"int8": 0, "e4m3": 1}
+
+
+class Packed8(NamedTuple):
+    """A tensor in 8 bits: `codes` (uint8, its values in order, then room up to a multiple of 32) and `units` (uint8, one for 32 values,
+    unit 2^(units - 127)); the tensor's shape and type, and the format."""
+    codes: torch.Tensor
+    units: torch.Tensor
+    shape: tuple
+    dtype: torch.dtype
+    format: str
+
+
+def _rows_width(what, shape, gated):
+    if not shape or (gated and shape[-1] % 2):
+        raise _lib.AdkError(f"{what}: x [..., width]{', width even (gate and up halves),' if gated else ''} is required; got {tuple(shape)}")
+    width = shape[-1] // 2 if gated else shape[-1]
+    rows = 1
+    for n in shape[:-1]:
+        rows *= n
+    return rows, width
+
+
+def _names(what, kind, format):
+    if kind not in _KINDS:
+        raise _lib.AdkError(f"{what}: kind is gelu, gelu_tanh or silu; got {kind!r}")
+    if format not in _FORMATS:
+        raise _lib.AdkError(f"{what}: format is int8 or e4m3; got {format!r}")
+
+
+def activation8_forward(x, *, kind="gelu", gated=False, format="int8"):
+    """-> (act(x), or act(gate) * up for x's halves, in x's type; x as Packed8), outside autograd.  x contiguous, float16, bfloat16 or
+    float32.  Infinities are held as the format's largest value in their block, NaN as NaN."""
+    _names("activation8", kind, format)
+    if x.dtype not in _DTYPES or not x.is_contiguous():
+        raise _lib.AdkError(f"activation8: a contiguous float16, bfloat16 or float32 tensor is required; got {x.dtype}, strides {x.stride()}")
+    rows, width = _rows_width("activation8", x.shape, gated)
+    _lib.require_cuda(x)
+    blocks = -(-x.numel() // 32)
+    y = torch.empty(*x.shape[:-1], width, dtype=x.dtype, device=x.device)
+    codes = torch.empty(32 * blocks, dtype=torch.uint8, device=x.device)
+    units = torch.empty(blocks, dtype=torch.uint8, device=x.device)
+    lib = _lib.load()
+    with _lib.on_device(x.device):
+        rc = lib.adk_activation8_fwd(x.data_ptr(), _DTYPES[x.dtype], rows, width, _KINDS[kind], int(bool(gated)), _FORMATS[format], y.data_ptr(), codes.data_ptr(),
+                                     units.data_ptr(), _lib.stream_of(x))
+    _lib.check(rc, "adk_activation8_fwd")
+    return y, Packed8(codes, units, tuple(x.shape), x.dtype, format)
+
+
+def activation8_backward(grad, packed, *, kind="gelu", gated=False, again=True):
+    """The gradient of activation8_forward's result from its Packed8 -> (dx, the activation of the held values or None without `again`).
+    grad of the result's shape and type."""
+    _names("activation8_backward", kind, packed.format)
+    rows, width = _rows_width("activation8_backward", packed.shape, gated)
+    shape = (*packed.shape[:-1], width)
+    if tuple(grad.shape) != shape or grad.dtype != packed.dtype:
+        raise _lib.AdkError(f"activation8_backward: grad {shape} {packed.dtype} is required; got {tuple(grad.shape)} {grad.dtype}")
+    n = rows * width * (2 if gated else 1)
+    c, u = packed.codes, packed.units
+    if (c.dtype != torch.uint8 or u.dtype != torch.uint8 or c.numel() < -(-n // 32) * 32 or u.numel() < -(-n // 32) or not c.is_contiguous() or not u.is_contiguous()
+            or c.device != grad.device or u.device != grad.device or c.data_ptr() % 8 or packed.dtype not in _DTYPES):
+        raise _lib.AdkError("activation8_backward: packed is not what activation8_forward returned, on grad's device")
+    _lib.require_cuda(grad, c, u)
+    grad = grad.contiguous()
+    dx = torch.empty(packed.shape, dtype=packed.dtype, device=grad.device)
+    y = torch.empty(shape, dtype=packed.dtype, device=grad.device) if again else None
+    lib = _lib.load()
+    with _lib.on_device(grad.device):
+        rc = lib.adk_activation8_bwd(grad.data_ptr(), c.data_ptr(), u.data_ptr(), _DTYPES[packed.dtype], rows, width, _KINDS[kind], int(bool(gated)),
+                                     _FORMATS[packed.format], dx.data_ptr(), _lib.ptr(y), _lib.stream_of(grad))
+    _lib.check(rc, "adk_activation8_bwd")
+    return dx, y
+
+
+class _Activation8(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, kind, gated, format):
+        y, packed = activation8_forward(x, kind=kind, gated=gated, format=format)
+        ctx.save_for_backward(packed.codes, packed.units)
+        ctx.how = (packed.shape, packed.dtype, format, kind, gated)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        shape, dtype, format, kind, gated = ctx.how
+        dx, _ = activation8_backward(grad, Packed8(*ctx.saved_tensors, shape, dtype, format), kind=kind, gated=gated, again=False)
+        return dx, None, None, None
+
+
+def activation8(x, *, kind="gelu", gated=False, format="int8") -> torch.Tensor:
+    """activation8_forward's result as part of autograd, which keeps x in 8 bits."""
+    return _Activation8.apply(x, kind, gated, format)
+
+
+class _Mlp8(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w1, b1, w2, b2, kind, gated, format):
+        y, packed = activation8_forward(F.linear(x, w1, b1), kind=kind, gated=gated, format=format)
+        ctx.save_for_backward(x, w1, w2, packed.codes, packed.units)
+        ctx.how = (packed.shape, packed.dtype, format, kind, gated, b1 is not None, b2 is not None)
+        return F.linear(y, w2, b2)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        x, w1, w2, codes, units = ctx.saved_tensors
+        shape, dtype, format, kind, gated, has1, has2 = ctx.how
+        g2 = grad.reshape(-1, grad.shape[-1])
+        dh, y = activation8_backward(torch.mm(g2, w2).view(*shape[:-1], w2.shape[1]), Packed8(codes, units, shape, dtype, format), kind=kind, gated=gated)
+        dh, y, x2 = dh.view(-1, dh.shape[-1]), y.view(-1, y.shape[-1]), x.reshape(-1, x.shape[-1])
+        return (torch.mm(dh, w1).view(x.shape), torch.mm(dh.t(), x2), dh.sum(0) if has1 else None, torch.mm(g2.t(), y), g2.sum(0) if has2 else None,
+                None, None, None)
+
+
+def mlp8(x, w1, b1, w2, b2, *, kind="gelu", gated=False, format="int8") -> torch.Tensor:
+    """act(x w1^T + b1) w2^T + b2 (gated: w1's outputs are gate and up halves), keeping x and 8 bits a hidden value for the backward pass.
+    x, weights and biases (or None) of one type.  The four products of the gradient are the library's."""
+    return _Mlp8.apply(x, w1, b1, w2, b2, kind, gated, format)

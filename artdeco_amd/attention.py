@@ -39,3 +39,186 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float | 
                                        float(scale if scale is not None else 1.0 / math.sqrt(D)), _lib.stream_of(q))
     _lib.check(rc, "adk_attention_fwd_f16")
     return out
+
+
+# ---------------------------------------------------------------------------------------------------------------------------
+# Attention with its gradient (csrc/attend.hip): what training the blocks, or answering token by token, needs beside the kernel
+# above.  fp16 or bf16, head sizes 8 .. 128 (multiples of 8), several query heads to a key head, causal order, a length for each
+# sequence, a free boolean mask.
+_DTYPES = {torch.float16: 0, torch.bfloat16: 2}
+
+
+def _strides(t: torch.Tensor):
+    """Element strides of the first three dimensions; a dimension of one element has none that matters."""
+    return [0 if n == 1 else s for n, s in zip(t.shape[:3], t.stride()[:3])]
+
+
+def _loadable(t: torch.Tensor) -> bool:
+    return (t.shape[-1] == 1 or t.stride(-1) == 1) and not any(s % 8 for s in _strides(t)) and t.data_ptr() % 16 == 0
+
+
+def _i64(values):
+    return (ctypes.c_int64 * len(values))(*values)
+
+
+def _check_attend(what, q, k, v, scale, mask, key_lengths):
+    """-> (scale, mask broadcast to [B, H, Nq, Nk] or None); raises AdkError for what the kernels do not take."""
+    if not (q.dim() == k.dim() == v.dim() == 4):
+        raise _lib.AdkError(f"{what}: q [B,H,Nq,D], k and v [B,Hk,Nk,D] are required")
+    B, H, Nq, D = q.shape
+    if k.shape != v.shape or k.shape[0] != B or k.shape[3] != D or k.shape[1] == 0 or H == 0 or H % k.shape[1]:
+        raise _lib.AdkError(f"{what}: k and v [B,Hk,Nk,D] of q's batch and head size, Hk dividing q's {H} heads, are required; got q {tuple(q.shape)}, "
+                            f"k {tuple(k.shape)}, v {tuple(v.shape)}")
+    if q.dtype not in _DTYPES or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise _lib.AdkError(f"{what}: q, k and v are float16 or bfloat16, all of one type; got {q.dtype}, {k.dtype}, {v.dtype}")
+    if D % 8 or not 8 <= D <= 128:
+        raise _lib.AdkError(f"{what}: head sizes 8 to 128, multiples of 8, are supported; got {D}")
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        if t.numel() and not _loadable(t):
+            raise _lib.AdkError(f"{what}: {name} needs a dense last dimension, strides that are multiples of 8 elements and 16-byte aligned storage")
+    for t in (k, v, mask, key_lengths):
+        if t is not None and t.device != q.device:
+            raise _lib.AdkError(f"{what}: all tensors are on one device; got {q.device} and {t.device}")
+    scale = float(scale) if scale is not None else 1.0 / math.sqrt(D)
+    if not 0.0 < scale < math.inf:
+        raise _lib.AdkError(f"{what}: scale is a positive number; got {scale}")
+    if key_lengths is not None and (key_lengths.dtype != torch.int32 or key_lengths.shape != (B,) or not key_lengths.is_contiguous()):
+        raise _lib.AdkError(f"{what}: key_lengths is a contiguous int32 tensor of the batch's size")
+    if mask is not None:
+        if mask.dtype != torch.bool:
+            raise _lib.AdkError(f"{what}: mask is a boolean tensor, True where a query sees a key (biases that are added to the scores are not supported)")
+        try:
+            mask = mask.broadcast_to(B, H, Nq, k.shape[2])
+        except RuntimeError:
+            raise _lib.AdkError(f"{what}: mask of shape {tuple(mask.shape)} does not broadcast to {(B, H, Nq, k.shape[2])}") from None
+    _lib.require_cuda(q, k, v, mask, key_lengths)
+    return scale, mask
+
+
+def _mask_args(mask):
+    if mask is None:
+        return None, None
+    return mask.data_ptr(), _i64([0 if n == 1 else s for n, s in zip(mask.shape, mask.stride())])
+
+
+def _workspace(nbytes, what, device):
+    if nbytes < 0:
+        _lib.check(nbytes, what)
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+
+
+def attend_forward(q, k, v, *, scale=None, causal=False, mask=None, key_lengths=None):
+    """softmax(scale q k^T) v over the keys that each query sees -> (out [B,Nq,H*D] in q's type, lse [B,H,Nq] float32), outside
+    autograd.  q [B,H,Nq,D], k / v [B,Hk,Nk,D], any views with a dense last dimension; query head h reads key head h * Hk // H.
+
+    scale        positive, 1/sqrt(D) if None.
+    causal       query i sees keys j <= i + Nk - Nq (the last query sees every key).
+    key_lengths  int32 [B]: sequence b has keys below key_lengths[b] (clamped to 0 .. Nk).  What lies behind is never read.
+    mask         bool, broadcastable to [B,H,Nq,Nk], True where a query sees a key; what it hides from a query has to hold finite
+                 numbers, unless the mask is the same for all queries and heads.
+    All three hold together.  A query that sees no key gives zeros and lse = -inf."""
+    scale, mask = _check_attend("attend_forward", q, k, v, scale, mask, key_lengths)
+    B, H, Nq, D = q.shape
+    Hk, Nk = k.shape[1], k.shape[2]
+    out = torch.empty(B, Nq, H * D, dtype=q.dtype, device=q.device)
+    lse = torch.empty(B, H, Nq, dtype=torch.float32, device=q.device)
+    lib = _lib.load()
+    with _lib.on_device(q.device):
+        ws = _workspace(lib.adk_attend_fwd_workspace_bytes(B, H, Hk, Nq, Nk, D), "adk_attend_fwd", q.device)
+        m, ms = _mask_args(mask)
+        rc = lib.adk_attend_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), _lib.ptr(key_lengths), m, _DTYPES[q.dtype],
+                                B, H, Hk, Nq, Nk, D, _i64(_strides(q)), _i64(_strides(k)), _i64(_strides(v)), ms, scale, int(bool(causal)),
+                                _lib.ptr(ws), 0 if ws is None else ws.numel(), _lib.stream_of(q))
+    _lib.check(rc, "adk_attend_fwd")
+    return out, lse
+
+
+def _backward_into(grad_out, q, k, v, out, lse, scale, causal, mask, key_lengths, dq, dk, dv):
+    B, H, Nq, D = q.shape
+    Hk, Nk = k.shape[1], k.shape[2]
+    grad = grad_out.reshape(B, Nq, H, D).transpose(1, 2)
+    if grad.numel() and not _loadable(grad):  # an expanded gradient, of a sum for instance
+        grad = grad_out.contiguous().view(B, Nq, H, D).transpose(1, 2)
+    lib = _lib.load()
+    with _lib.on_device(q.device):
+        ws = _workspace(lib.adk_attend_bwd_workspace_bytes(B, H, Hk, Nq, Nk, D), "adk_attend_bwd", q.device)
+        m, ms = _mask_args(mask)
+        rc = lib.adk_attend_bwd(grad.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), _lib.ptr(key_lengths), m,
+                                _DTYPES[q.dtype], B, H, Hk, Nq, Nk, D, _i64(_strides(grad)), _i64(_strides(q)), _i64(_strides(k)), _i64(_strides(v)), ms,
+                                scale, int(bool(causal)), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _i64(_strides(dq)), _i64(_strides(dk)),
+                                _i64(_strides(dv)), _lib.ptr(ws), 0 if ws is None else ws.numel(), _lib.stream_of(q))
+    _lib.check(rc, "adk_attend_bwd")
+
+
+def attend_backward(grad_out, q, k, v, out, lse, *, scale=None, causal=False, mask=None, key_lengths=None):
+    """The gradient of attend_forward's out, called with the same arguments and what it returned -> (dq, dk, dv) in the shapes and
+    the type of q, k and v ([B,N,heads,D] in memory).  grad_out [B,Nq,H*D].  The heads that share a key head are summed in 32 bits, in a
+    fixed order; keys behind a sequence's length get zeros."""
+    scale, mask = _check_attend("attend_backward", q, k, v, scale, mask, key_lengths)
+    B, H, Nq, D = q.shape
+    for name, t, shape, dtype in (("grad_out", grad_out, (B, Nq, H * D), q.dtype), ("out", out, (B, Nq, H * D), q.dtype), ("lse", lse, (B, H, Nq), torch.float32)):
+        if tuple(t.shape) != shape or t.dtype != dtype or t.device != q.device:
+            raise _lib.AdkError(f"attend_backward: {name} {shape} {dtype} on {q.device} is required; got {tuple(t.shape)} {t.dtype} on {t.device}")
+    out, lse = out.contiguous(), lse.contiguous()
+    if out.data_ptr() % 16:
+        out = out.clone()
+    dq, dk, dv = (torch.empty(t.shape[0], t.shape[2], t.shape[1], D, dtype=t.dtype, device=t.device).transpose(1, 2) for t in (q, k, v))
+    _backward_into(grad_out, q, k, v, out, lse, scale, causal, mask, key_lengths, dq, dk, dv)
+    return dq, dk, dv
+
+
+class _Attend(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, scale, causal, mask, key_lengths):
+        out, lse = attend_forward(q, k, v, scale=scale, causal=causal, mask=mask, key_lengths=key_lengths)
+        ctx.save_for_backward(q, k, v, out, lse, mask, key_lengths)
+        ctx.how = (scale, causal)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_out):
+        q, k, v, out, lse, mask, key_lengths = ctx.saved_tensors
+        scale, causal = ctx.how
+        dq, dk, dv = attend_backward(grad_out, q, k, v, out, lse, scale=scale, causal=causal, mask=mask, key_lengths=key_lengths)
+        return dq, dk, dv, None, None, None, None
+
+
+def attend(q, k, v, *, scale=None, causal=False, mask=None, key_lengths=None) -> torch.Tensor:
+    """attend_forward's out as part of autograd: differentiable once with respect to q, k and v.  -> [B,Nq,H*D]."""
+    return _Attend.apply(q, k, v, scale, causal, mask, key_lengths)
+
+
+def _packed_views(qkv, heads, kv_heads):
+    t = qkv.transpose(1, 2)
+    return t[:, :heads], t[:, heads:heads + kv_heads], t[:, heads + kv_heads:]
+
+
+class _AttendPacked(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, qkv, heads, kv_heads, scale, causal, mask, key_lengths):
+        q, k, v = _packed_views(qkv, heads, kv_heads)
+        out, lse = attend_forward(q, k, v, scale=scale, causal=causal, mask=mask, key_lengths=key_lengths)
+        ctx.save_for_backward(qkv, out, lse, mask, key_lengths)
+        ctx.how = (heads, kv_heads, scale, causal)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_out):
+        qkv, out, lse, mask, key_lengths = ctx.saved_tensors
+        heads, kv_heads, scale, causal = ctx.how
+        q, k, v = _packed_views(qkv, heads, kv_heads)
+        scale, mask = _check_attend("attend_packed", q, k, v, scale, mask, key_lengths)
+        grad = torch.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device)
+        _backward_into(grad_out, q, k, v, out, lse, scale, causal, mask, key_lengths, *_packed_views(grad, heads, kv_heads))
+        return grad, None, None, None, None, None, None
+
+
+def attend_packed(qkv, heads, kv_heads=None, *, scale=None, causal=False, mask=None, key_lengths=None) -> torch.Tensor:
+    """attend on the heads of one projection, qkv [B,N,heads + 2 kv_heads,D] (q's heads, then k's, then v's): the gradient arrives in
+    one tensor of that shape, where three views of qkv would each be padded to it and added up.  -> [B,N,heads*D]."""
+    kv_heads = heads if kv_heads is None else kv_heads
+    if qkv.dim() != 4 or heads < 1 or kv_heads < 1 or qkv.shape[2] != heads + 2 * kv_heads:
+        raise _lib.AdkError(f"attend_packed: qkv [B,N,heads + 2 kv_heads,D] is required; got {tuple(qkv.shape)} for {heads} and {kv_heads} heads")
+    return _AttendPacked.apply(qkv, heads, kv_heads, scale, causal, mask, key_lengths)
