@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+from array import array
 
 import torch
 
@@ -50,19 +51,19 @@ _DTYPES = {torch.float16: 0, torch.bfloat16: 2}
 
 def _strides(t: torch.Tensor):
     """Element strides of the first three dimensions; a dimension of one element has none that matters."""
-    return [0 if n == 1 else s for n, s in zip(t.shape[:3], t.stride()[:3])]
+    a, b, c = t.shape[:3]
+    x, y, z, _ = t.stride()
+    return [x if a > 1 else 0, y if b > 1 else 0, z if c > 1 else 0]
 
 
-def _loadable(t: torch.Tensor) -> bool:
-    return (t.shape[-1] == 1 or t.stride(-1) == 1) and not any(s % 8 for s in _strides(t)) and t.data_ptr() % 16 == 0
-
-
-def _i64(values):
-    return (ctypes.c_int64 * len(values))(*values)
+def _loadable(t: torch.Tensor, strides) -> bool:
+    a, b, c = strides
+    return t.stride(3) == 1 and not (a | b | c) & 7 and not t.data_ptr() & 15
 
 
 def _check_attend(what, q, k, v, scale, mask, key_lengths):
-    """-> (scale, mask broadcast to [B, H, Nq, Nk] or None); raises AdkError for what the kernels do not take."""
+    """-> (scale, mask broadcast to [B, H, Nq, Nk] or None, the strides of q, k, v and the mask); raises AdkError for what the kernels do
+    not take."""
     if not (q.dim() == k.dim() == v.dim() == 4):
         raise _lib.AdkError(f"{what}: q [B,H,Nq,D], k and v [B,Hk,Nk,D] are required")
     B, H, Nq, D = q.shape
@@ -73,11 +74,15 @@ def _check_attend(what, q, k, v, scale, mask, key_lengths):
         raise _lib.AdkError(f"{what}: q, k and v are float16 or bfloat16, all of one type; got {q.dtype}, {k.dtype}, {v.dtype}")
     if D % 8 or not 8 <= D <= 128:
         raise _lib.AdkError(f"{what}: head sizes 8 to 128, multiples of 8, are supported; got {D}")
+    strides = []
     for name, t in (("q", q), ("k", k), ("v", v)):
-        if t.numel() and not _loadable(t):
+        s = _strides(t)
+        strides += s
+        if not _loadable(t, s) and t.numel():
             raise _lib.AdkError(f"{what}: {name} needs a dense last dimension, strides that are multiples of 8 elements and 16-byte aligned storage")
+    device = q.device
     for t in (k, v, mask, key_lengths):
-        if t is not None and t.device != q.device:
+        if t is not None and t.device != device:
             raise _lib.AdkError(f"{what}: all tensors are on one device; got {q.device} and {t.device}")
     scale = float(scale) if scale is not None else 1.0 / math.sqrt(D)
     if not 0.0 < scale < math.inf:
@@ -91,14 +96,11 @@ def _check_attend(what, q, k, v, scale, mask, key_lengths):
             mask = mask.broadcast_to(B, H, Nq, k.shape[2])
         except RuntimeError:
             raise _lib.AdkError(f"{what}: mask of shape {tuple(mask.shape)} does not broadcast to {(B, H, Nq, k.shape[2])}") from None
-    _lib.require_cuda(q, k, v, mask, key_lengths)
-    return scale, mask
-
-
-def _mask_args(mask):
-    if mask is None:
-        return None, None
-    return mask.data_ptr(), _i64([0 if n == 1 else s for n, s in zip(mask.shape, mask.stride())])
+        strides += [0 if n == 1 else s for n, s in zip(mask.shape, mask.stride())]
+    else:
+        strides += (0, 0, 0, 0)
+    _lib.require_cuda(q)
+    return scale, mask, strides
 
 
 def _workspace(nbytes, what, device):
@@ -117,36 +119,38 @@ def attend_forward(q, k, v, *, scale=None, causal=False, mask=None, key_lengths=
     mask         bool, broadcastable to [B,H,Nq,Nk], True where a query sees a key; what it hides from a query has to hold finite
                  numbers, unless the mask is the same for all queries and heads.
     All three hold together.  A query that sees no key gives zeros and lse = -inf."""
-    scale, mask = _check_attend("attend_forward", q, k, v, scale, mask, key_lengths)
+    scale, mask, strides = _check_attend("attend_forward", q, k, v, scale, mask, key_lengths)
     B, H, Nq, D = q.shape
     Hk, Nk = k.shape[1], k.shape[2]
+    held = array("q", strides)  # alive until the call returns
     out = torch.empty(B, Nq, H * D, dtype=q.dtype, device=q.device)
     lse = torch.empty(B, H, Nq, dtype=torch.float32, device=q.device)
     lib = _lib.load()
     with _lib.on_device(q.device):
         ws = _workspace(lib.adk_attend_fwd_workspace_bytes(B, H, Hk, Nq, Nk, D), "adk_attend_fwd", q.device)
-        m, ms = _mask_args(mask)
-        rc = lib.adk_attend_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), _lib.ptr(key_lengths), m, _DTYPES[q.dtype],
-                                B, H, Hk, Nq, Nk, D, _i64(_strides(q)), _i64(_strides(k)), _i64(_strides(v)), ms, scale, int(bool(causal)),
-                                _lib.ptr(ws), 0 if ws is None else ws.numel(), _lib.stream_of(q))
+        rc = lib.adk_attend_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), _lib.ptr(key_lengths), _lib.ptr(mask), _DTYPES[q.dtype],
+                                B, H, Hk, Nq, Nk, D, held.buffer_info()[0], scale, bool(causal), _lib.ptr(ws), 0 if ws is None else ws.numel(),
+                                _lib.stream_of(q))
     _lib.check(rc, "adk_attend_fwd")
     return out, lse
 
 
-def _backward_into(grad_out, q, k, v, out, lse, scale, causal, mask, key_lengths, dq, dk, dv):
+def _backward_into(grad_out, q, k, v, out, lse, scale, causal, mask, key_lengths, strides, dq, dk, dv):
     B, H, Nq, D = q.shape
     Hk, Nk = k.shape[1], k.shape[2]
-    grad = grad_out.reshape(B, Nq, H, D).transpose(1, 2)
-    if grad.numel() and not _loadable(grad):  # an expanded gradient, of a sum for instance
-        grad = grad_out.contiguous().view(B, Nq, H, D).transpose(1, 2)
+    a, b, c = grad_out.stride()
+    g = [a if B > 1 else 0, D if H > 1 else 0, b if Nq > 1 else 0]
+    if grad_out.numel() and (c != 1 or (g[0] | g[2]) & 7 or grad_out.data_ptr() & 15):  # an expanded gradient, of a sum for instance
+        grad_out = grad_out.contiguous()
+        grad_out = grad_out.clone() if grad_out.data_ptr() & 15 else grad_out
+        g = [Nq * H * D, D, H * D]
     lib = _lib.load()
+    held = array("q", strides + g + _strides(dq) + _strides(dk) + _strides(dv))
     with _lib.on_device(q.device):
         ws = _workspace(lib.adk_attend_bwd_workspace_bytes(B, H, Hk, Nq, Nk, D), "adk_attend_bwd", q.device)
-        m, ms = _mask_args(mask)
-        rc = lib.adk_attend_bwd(grad.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), _lib.ptr(key_lengths), m,
-                                _DTYPES[q.dtype], B, H, Hk, Nq, Nk, D, _i64(_strides(grad)), _i64(_strides(q)), _i64(_strides(k)), _i64(_strides(v)), ms,
-                                scale, int(bool(causal)), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _i64(_strides(dq)), _i64(_strides(dk)),
-                                _i64(_strides(dv)), _lib.ptr(ws), 0 if ws is None else ws.numel(), _lib.stream_of(q))
+        rc = lib.adk_attend_bwd(grad_out.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), _lib.ptr(key_lengths), _lib.ptr(mask),
+                                _DTYPES[q.dtype], B, H, Hk, Nq, Nk, D, held.buffer_info()[0], scale, bool(causal), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+                                _lib.ptr(ws), 0 if ws is None else ws.numel(), _lib.stream_of(q))
     _lib.check(rc, "adk_attend_bwd")
 
 
@@ -154,16 +158,19 @@ def attend_backward(grad_out, q, k, v, out, lse, *, scale=None, causal=False, ma
     """The gradient of attend_forward's out, called with the same arguments and what it returned -> (dq, dk, dv) in the shapes and
     the type of q, k and v ([B,N,heads,D] in memory).  grad_out [B,Nq,H*D].  The heads that share a key head are summed in 32 bits, in a
     fixed order; keys behind a sequence's length get zeros."""
-    scale, mask = _check_attend("attend_backward", q, k, v, scale, mask, key_lengths)
+    scale, mask, strides = _check_attend("attend_backward", q, k, v, scale, mask, key_lengths)
     B, H, Nq, D = q.shape
     for name, t, shape, dtype in (("grad_out", grad_out, (B, Nq, H * D), q.dtype), ("out", out, (B, Nq, H * D), q.dtype), ("lse", lse, (B, H, Nq), torch.float32)):
         if tuple(t.shape) != shape or t.dtype != dtype or t.device != q.device:
             raise _lib.AdkError(f"attend_backward: {name} {shape} {dtype} on {q.device} is required; got {tuple(t.shape)} {t.dtype} on {t.device}")
     out, lse = out.contiguous(), lse.contiguous()
-    if out.data_ptr() % 16:
+    if out.data_ptr() & 15:
         out = out.clone()
-    dq, dk, dv = (torch.empty(t.shape[0], t.shape[2], t.shape[1], D, dtype=t.dtype, device=t.device).transpose(1, 2) for t in (q, k, v))
-    _backward_into(grad_out, q, k, v, out, lse, scale, causal, mask, key_lengths, dq, dk, dv)
+    Hk, Nk = k.shape[1], k.shape[2]
+    dq = torch.empty(B, Nq, H, D, dtype=q.dtype, device=q.device).transpose(1, 2)
+    dk = torch.empty(B, Nk, Hk, D, dtype=q.dtype, device=q.device).transpose(1, 2)
+    dv = torch.empty(B, Nk, Hk, D, dtype=q.dtype, device=q.device).transpose(1, 2)
+    _backward_into(grad_out, q, k, v, out, lse, scale, causal, mask, key_lengths, strides, dq, dk, dv)
     return dq, dk, dv
 
 
@@ -186,6 +193,8 @@ class _Attend(torch.autograd.Function):
 
 def attend(q, k, v, *, scale=None, causal=False, mask=None, key_lengths=None) -> torch.Tensor:
     """attend_forward's out as part of autograd: differentiable once with respect to q, k and v.  -> [B,Nq,H*D]."""
+    if not (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)):
+        return attend_forward(q, k, v, scale=scale, causal=causal, mask=mask, key_lengths=key_lengths)[0]
     return _Attend.apply(q, k, v, scale, causal, mask, key_lengths)
 
 
@@ -209,9 +218,9 @@ class _AttendPacked(torch.autograd.Function):
         qkv, out, lse, mask, key_lengths = ctx.saved_tensors
         heads, kv_heads, scale, causal = ctx.how
         q, k, v = _packed_views(qkv, heads, kv_heads)
-        scale, mask = _check_attend("attend_packed", q, k, v, scale, mask, key_lengths)
+        scale, mask, strides = _check_attend("attend_packed", q, k, v, scale, mask, key_lengths)
         grad = torch.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device)
-        _backward_into(grad_out, q, k, v, out, lse, scale, causal, mask, key_lengths, *_packed_views(grad, heads, kv_heads))
+        _backward_into(grad_out, q, k, v, out, lse, scale, causal, mask, key_lengths, strides, *_packed_views(grad, heads, kv_heads))
         return grad, None, None, None, None, None, None
 
 
@@ -221,4 +230,6 @@ def attend_packed(qkv, heads, kv_heads=None, *, scale=None, causal=False, mask=N
     kv_heads = heads if kv_heads is None else kv_heads
     if qkv.dim() != 4 or heads < 1 or kv_heads < 1 or qkv.shape[2] != heads + 2 * kv_heads:
         raise _lib.AdkError(f"attend_packed: qkv [B,N,heads + 2 kv_heads,D] is required; got {tuple(qkv.shape)} for {heads} and {kv_heads} heads")
+    if not (torch.is_grad_enabled() and qkv.requires_grad):
+        return attend_forward(*_packed_views(qkv, heads, kv_heads), scale=scale, causal=causal, mask=mask, key_lengths=key_lengths)[0]
     return _AttendPacked.apply(qkv, heads, kv_heads, scale, causal, mask, key_lengths)

@@ -649,10 +649,8 @@ static int at_check(int dtype, int B, int H, int Hk, int Nq, int Nk, int D, floa
     return 0;
 }
 
-static int at_tensor(const void* p, const int64_t* s) {
-    if (!p || !s) return ADK_EINVAL;
-    return (((uintptr_t)p & 15) || ((s[0] | s[1] | s[2]) & 7)) ? ADK_EINVAL : 0;
-}
+// s: strides (batch, head, token)
+static int at_tensor(const void* p, const int64_t* s) { return (!p || ((uintptr_t)p & 15) || ((s[0] | s[1] | s[2]) & 7)) ? ADK_EINVAL : 0; }
 
 #define AT_LAUNCH3(KERNEL, T, GRID)                                                                                             \
     do {                                                                                                                        \
@@ -682,16 +680,17 @@ template <typename T> static int at_bwd(const AttendArgs& a, hipStream_t stream)
     ADK_RETURN_LAST_ERROR();
 }
 
+// s: strides of q, k, v (batch, head, token each), then of the mask (batch, head, query, key)
 static void at_fill(AttendArgs& a, const void* q, const void* k, const void* v, const float* lse, const int* key_lengths, const uint8_t* mask, int B, int H, int Hk,
-                    int Nq, int Nk, int D, const int64_t* qs, const int64_t* ks, const int64_t* vs, const int64_t* ms, float scale, int causal) {
+                    int Nq, int Nk, int D, const int64_t* s, float scale, int causal) {
     a.q = q; a.k = k; a.v = v; a.lse = const_cast<float*>(lse);
-    a.key_lengths = key_lengths; a.mask = mask;
+    a.key_lengths = key_lengths; a.mask = Nq && Nk ? mask : nullptr;
     a.B = B; a.H = H; a.Hk = Hk; a.G = H / Hk; a.Nq = Nq; a.Nk = Nk; a.D = D; a.splits = 1; a.causal = causal;
-    a.q_sb = qs[0]; a.q_sh = qs[1]; a.q_sn = qs[2];
-    a.k_sb = ks[0]; a.k_sh = ks[1]; a.k_sn = ks[2];
-    a.v_sb = vs[0]; a.v_sh = vs[1]; a.v_sn = vs[2];
-    if (mask) { a.m_sb = ms[0]; a.m_sh = ms[1]; a.m_sq = ms[2]; a.m_sk = ms[3]; }
-    a.mask_by_key = mask && a.m_sq == 0 && (a.m_sh == 0 || a.G == 1);
+    a.q_sb = s[0]; a.q_sh = s[1]; a.q_sn = s[2];
+    a.k_sb = s[3]; a.k_sh = s[4]; a.k_sn = s[5];
+    a.v_sb = s[6]; a.v_sh = s[7]; a.v_sn = s[8];
+    if (mask) { a.m_sb = s[9]; a.m_sh = s[10]; a.m_sq = s[11]; a.m_sk = s[12]; }
+    a.mask_by_key = a.mask && a.m_sq == 0 && (a.m_sh == 0 || a.G == 1);
     a.scale = scale; a.scale_log2e = scale * 1.4426950408889634f;
 }
 
@@ -707,17 +706,15 @@ extern "C" int64_t adk_attend_fwd_workspace_bytes(int B, int H, int Hk, int Nq, 
 }
 
 extern "C" int adk_attend_fwd(const void* q, const void* k, const void* v, void* out, float* lse, const int32_t* key_lengths, const uint8_t* mask, int dtype, int B, int H,
-                              int Hk, int Nq, int Nk, int D, const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides, const int64_t* mask_strides,
-                              float scale, int causal, void* ws, int64_t ws_bytes, hipStream_t stream)
+                              int Hk, int Nq, int Nk, int D, const int64_t* strides, float scale, int causal, void* ws, int64_t ws_bytes, hipStream_t stream)
 {
-    int e = adk::at_check(dtype, B, H, Hk, Nq, Nk, D, scale);
+    const int e = adk::at_check(dtype, B, H, Hk, Nq, Nk, D, scale);
     if (e) return e;
     if ((int64_t)B * Nq == 0) return 0;
-    if ((e = adk::at_tensor(q, q_strides)) || !out || ((uintptr_t)out & 7) || !lse || (mask && !mask_strides)) return ADK_EINVAL;
-    if (Nk && (adk::at_tensor(k, k_strides) || adk::at_tensor(v, v_strides))) return ADK_EINVAL;
-    static const int64_t none[3] = {0, 0, 0};
+    if (!strides || adk::at_tensor(q, strides) || !out || ((uintptr_t)out & 7) || !lse) return ADK_EINVAL;
+    if (Nk && (adk::at_tensor(k, strides + 3) || adk::at_tensor(v, strides + 6))) return ADK_EINVAL;
     adk::AttendArgs a = {};
-    adk::at_fill(a, q, k, v, lse, key_lengths, Nk ? mask : nullptr, B, H, Hk, Nq, Nk, D, q_strides, Nk ? k_strides : none, Nk ? v_strides : none, mask_strides, scale, causal);
+    adk::at_fill(a, q, k, v, lse, key_lengths, mask, B, H, Hk, Nq, Nk, D, strides, scale, causal);
     a.out = out;
     const int64_t need = adk_attend_fwd_workspace_bytes(B, H, Hk, Nq, Nk, D);
     if (need > 0) {
@@ -738,30 +735,23 @@ extern "C" int64_t adk_attend_bwd_workspace_bytes(int B, int H, int Hk, int Nq, 
 }
 
 extern "C" int adk_attend_bwd(const void* dout, const void* q, const void* k, const void* v, const void* out, const float* lse, const int32_t* key_lengths,
-                              const uint8_t* mask, int dtype, int B, int H, int Hk, int Nq, int Nk, int D, const int64_t* dout_strides, const int64_t* q_strides,
-                              const int64_t* k_strides, const int64_t* v_strides, const int64_t* mask_strides, float scale, int causal, void* dq, void* dk, void* dv,
-                              const int64_t* dq_strides, const int64_t* dk_strides, const int64_t* dv_strides, void* ws, int64_t ws_bytes, hipStream_t stream)
+                              const uint8_t* mask, int dtype, int B, int H, int Hk, int Nq, int Nk, int D, const int64_t* strides, float scale, int causal, void* dq,
+                              void* dk, void* dv, void* ws, int64_t ws_bytes, hipStream_t stream)
 {
-    int e = adk::at_check(dtype, B, H, Hk, Nq, Nk, D, scale);
+    const int e = adk::at_check(dtype, B, H, Hk, Nq, Nk, D, scale);
     if (e) return e;
     if (B == 0 || (Nq == 0 && Nk == 0)) return 0;
-    if (Nq && (adk::at_tensor(q, q_strides) || adk::at_tensor(dout, dout_strides) || adk::at_tensor(dq, dq_strides) || !out || ((uintptr_t)out & 15) || !lse))
-        return ADK_EINVAL;
-    if (Nk && (adk::at_tensor(k, k_strides) || adk::at_tensor(v, v_strides) || adk::at_tensor(dk, dk_strides) || adk::at_tensor(dv, dv_strides))) return ADK_EINVAL;
-    if (mask && !mask_strides) return ADK_EINVAL;
-    static const int64_t none[3] = {0, 0, 0};
+    if (!strides) return ADK_EINVAL;
+    const int64_t* s = strides + 13; // of dout, dq, dk, dv
+    if (Nq && (adk::at_tensor(q, strides) || adk::at_tensor(dout, s) || adk::at_tensor(dq, s + 3) || !out || ((uintptr_t)out & 15) || !lse)) return ADK_EINVAL;
+    if (Nk && (adk::at_tensor(k, strides + 3) || adk::at_tensor(v, strides + 6) || adk::at_tensor(dk, s + 6) || adk::at_tensor(dv, s + 9))) return ADK_EINVAL;
     adk::AttendArgs a = {};
-    adk::at_fill(a, q, k, v, lse, key_lengths, Nq && Nk ? mask : nullptr, B, H, Hk, Nq, Nk, D, Nq ? q_strides : none, Nk ? k_strides : none, Nk ? v_strides : none,
-                 mask_strides, scale, causal);
+    adk::at_fill(a, q, k, v, lse, key_lengths, mask, B, H, Hk, Nq, Nk, D, strides, scale, causal);
     a.dout = dout; a.out_in = out; a.dq = dq; a.dk = dk; a.dv = dv;
-    if (Nq) {
-        a.g_sb = dout_strides[0]; a.g_sh = dout_strides[1]; a.g_sn = dout_strides[2];
-        a.dq_sb = dq_strides[0]; a.dq_sh = dq_strides[1]; a.dq_sn = dq_strides[2];
-    }
-    if (Nk) {
-        a.dk_sb = dk_strides[0]; a.dk_sh = dk_strides[1]; a.dk_sn = dk_strides[2];
-        a.dv_sb = dv_strides[0]; a.dv_sh = dv_strides[1]; a.dv_sn = dv_strides[2];
-    }
+    a.g_sb = s[0]; a.g_sh = s[1]; a.g_sn = s[2];
+    a.dq_sb = s[3]; a.dq_sh = s[4]; a.dq_sn = s[5];
+    a.dk_sb = s[6]; a.dk_sh = s[7]; a.dk_sn = s[8];
+    a.dv_sb = s[9]; a.dv_sh = s[10]; a.dv_sn = s[11];
     const int64_t rows = (int64_t)B * H * Nq;
     if (rows) {
         if (!ws || ws_bytes < adk_attend_bwd_workspace_bytes(B, H, Hk, Nq, Nk, D) || ((uintptr_t)ws & 15)) return ADK_EWORKSPACE;

@@ -140,17 +140,17 @@ template <typename T> static int rotary_of(RotaryArgs& a, int half, hipStream_t 
 } // namespace adk
 
 extern "C" int adk_rotary(const void* x, void* y, const int64_t* positions, const double* frequencies, int dtype, int B, int N, int H, int D, int turned, int pairs, int axes,
-                          int half, int transpose, float factor, const int64_t* x_strides, const int64_t* y_strides, const int64_t* position_strides, hipStream_t stream)
+                          int half, int transpose, float factor, const int64_t* strides, hipStream_t stream)
 {
     if (B < 0 || N < 0 || H < 0 || D < 0 || turned < 0 || turned > H || pairs < 1 || axes < 1 || (int64_t)2 * pairs * axes > D) return ADK_EINVAL;
     if (dtype < 0 || dtype > 2) return ADK_EUNSUPPORTED;
     if (B == 0 || N == 0 || H == 0) return 0;
-    if (!x || !y || !positions || !frequencies || !x_strides || !y_strides || !position_strides) return ADK_EINVAL;
+    if (!x || !y || !positions || !frequencies || !strides) return ADK_EINVAL;
     adk::RotaryArgs a = {};
     a.x = x; a.y = y; a.positions = positions; a.frequencies = frequencies;
-    a.x_sb = x_strides[0]; a.x_sn = x_strides[1]; a.x_sh = x_strides[2];
-    a.y_sb = y_strides[0]; a.y_sn = y_strides[1]; a.y_sh = y_strides[2];
-    a.p_sb = position_strides[0]; a.p_sn = position_strides[1]; a.p_sa = position_strides[2];
+    a.x_sb = strides[0]; a.x_sn = strides[1]; a.x_sh = strides[2];
+    a.y_sb = strides[3]; a.y_sn = strides[4]; a.y_sh = strides[5];
+    a.p_sb = strides[6]; a.p_sn = strides[7]; a.p_sa = strides[8];
     a.tokens = (int64_t)B * N;
     a.N = N; a.H = H; a.D = D; a.turned = turned; a.pairs = pairs; a.axes = axes; a.copy = x != y;
     a.factor = factor; a.sign = transpose ? -1.f : 1.f;

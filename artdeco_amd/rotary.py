@@ -7,8 +7,8 @@ rotary_ with two axes, layout "half" and frequencies base^(-m / P).  The angle i
 their turn."""
 from __future__ import annotations
 
-import ctypes
 import math
+from array import array
 
 import torch
 
@@ -75,26 +75,42 @@ def _turn(x, y, positions, frequencies, factor, layout, heads, transpose):
     axes = p.shape[-1]
     if tuple(p.shape[-3:-1]) not in ((B, N), (1, N), (N,)) or axes < 1:
         raise _lib.AdkError(f"rotary: positions of shape {tuple(positions.shape)} do not fit x {tuple(x.shape)}")
-    p = p.broadcast_to(B, N, axes)
     if 2 * axes * frequencies.numel() > D:
         raise _lib.AdkError(f"rotary: {axes} axes of {frequencies.numel()} pairs do not fit heads of {D}")
     heads = H if heads is None else heads
     if not 0 <= heads <= H:
         raise _lib.AdkError(f"rotary: {heads} of {H} heads to turn")
-    if x.device != positions.device or x.device != frequencies.device:
+    device = x.device
+    if device != positions.device or device != frequencies.device:
         raise _lib.AdkError("rotary: all tensors are on one device")
-    _lib.require_cuda(x, positions, frequencies)
-    i3 = ctypes.c_int64 * 3
+    _lib.require_cuda(x)
+    pb, pn, pa = p.stride()[-3:] if p.dim() == 3 else (0, *p.stride())
+    if p.dim() == 3 and p.shape[0] == 1:
+        pb = 0
+    held = array("q", (*_strides(x), *_strides(y), pb, pn, pa))  # alive until the call returns
     lib = _lib.load()
-    with _lib.on_device(x.device):
-        rc = lib.adk_rotary(x.data_ptr(), y.data_ptr(), p.data_ptr(), frequencies.data_ptr(), _DTYPES[x.dtype], B, N, H, D, heads, frequencies.numel(), axes,
-                            _LAYOUTS[layout], int(transpose), float(factor), i3(*_strides(x)), i3(*_strides(y)), i3(*p.stride()), _lib.stream_of(x))
+    with _lib.on_device(device):
+        rc = lib.adk_rotary(x.data_ptr(), y.data_ptr(), positions.data_ptr(), frequencies.data_ptr(), _DTYPES[x.dtype], B, N, H, D, heads, frequencies.numel(),
+                            axes, _LAYOUTS[layout], transpose, factor, held.buffer_info()[0], _lib.stream_of(x))
     _lib.check(rc, "adk_rotary")
     return y
 
 
 def _strides(t):
-    return [0 if n == 1 else s for n, s in zip(t.shape[:3], t.stride()[:3])]
+    """Element strides of (batch, token, head); a dimension of one element has none that matters."""
+    a, b, c = t.shape[:3]
+    x, y, z, _ = t.stride()
+    return (x if a > 1 else 0, y if b > 1 else 0, z if c > 1 else 0)
+
+
+def _recorded(x):
+    return torch.is_grad_enabled() and x.requires_grad
+
+
+def _new(x, positions, frequencies, factor, layout, heads, transpose):
+    if x.dim() != 4 or x.dtype not in _DTYPES:
+        raise _lib.AdkError(f"rotary: x [B,N,H,D] is required, float16, bfloat16 and float32 are supported; got {tuple(x.shape)} {x.dtype}")
+    return _turn(x, torch.empty(x.shape, dtype=x.dtype, device=x.device), positions, frequencies, factor, layout, heads, transpose)
 
 
 class _Rotary(torch.autograd.Function):
@@ -105,7 +121,7 @@ class _Rotary(torch.autograd.Function):
         if inplace:
             ctx.mark_dirty(x)
             return _turn(x, x, positions, frequencies, factor, layout, heads, transpose)
-        return _turn(x, torch.empty(x.shape, dtype=x.dtype, device=x.device), positions, frequencies, factor, layout, heads, transpose)
+        return _new(x, positions, frequencies, factor, layout, heads, transpose)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -114,13 +130,15 @@ class _Rotary(torch.autograd.Function):
         factor, layout, heads, transpose = ctx.how
         if grad.shape[-1] > 1 and grad.stride(-1) != 1:
             grad = grad.contiguous()
-        grad = _turn(grad, torch.empty(grad.shape, dtype=grad.dtype, device=grad.device), positions, frequencies, factor, layout, heads, not transpose)
+        grad = _new(grad, positions, frequencies, factor, layout, heads, not transpose)
         return (grad,) + (None,) * 7
 
 
 def rotary(x, positions, frequencies, *, factor=1.0, layout="half", heads=None) -> torch.Tensor:
     """x [B,N,H,D] (float16, bfloat16 or float32, dense last dimension) with the first `heads` heads (all if None) turned, as a new
     contiguous tensor; the other channels and heads are copied.  positions int64 [N], [B,N] or [B,N,axes].  Differentiable."""
+    if not _recorded(x):
+        return _new(x, positions, frequencies, factor, layout, heads, False)
     return _Rotary.apply(x, positions, frequencies, factor, layout, heads, False, False)
 
 
@@ -131,4 +149,6 @@ def rotary_(x, positions, frequencies, *, factor=1.0, layout="half", heads=None)
 
 def rotary_transpose(x, positions, frequencies, *, factor=1.0, layout="half", heads=None) -> torch.Tensor:
     """The transpose of rotary, which is the gradient's form: the same pairs turned back, times factor."""
+    if not _recorded(x):
+        return _new(x, positions, frequencies, factor, layout, heads, True)
     return _Rotary.apply(x, positions, frequencies, factor, layout, heads, True, False)

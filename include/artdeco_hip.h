@@ -309,36 +309,35 @@ int adk_attention_fwd_f16(const void* q, const void* k, const void* v, void* out
  * softmax's sum; the backward recomputes the probabilities from lse.  dtype 0 = float16, 2 = bfloat16; fp32 inside.
  *
  * q [B,H,Nq,D], k / v [B,Hk,Nk,D], H a multiple of Hk (query heads h Hk / H share key head h), D a multiple of 8, at most
- * 128.  Strides are element strides (batch, head, token), multiples of 8, the last dimension dense; pointers 16-byte aligned
- * (out 8-byte in the forward).  out [B,Nq,H,D] and lse [B,H,Nq] contiguous.  dout strides as q's; dq, dk, dv by strides.
+ * 128; out [B,Nq,H,D] and lse [B,H,Nq] contiguous, dout and dq as q, dk and dv as k.  strides: element strides on the host,
+ * (batch, head, token) of q, k, v, then (batch, head, query, key) of the mask, and in the backward (batch, head, token) of
+ * dout, dq, dk, dv: 13 and 25 numbers.  The tensors' strides are multiples of 8, their last dimension dense, their pointers
+ * 16-byte aligned (out 8-byte in the forward).
  * causal: query i sees keys j <= i + Nk - Nq.  key_lengths [B] int32 or NULL: sequence b has keys below key_lengths[b]; what
- * lies behind is never read, its dk and dv are 0.  mask or NULL: one byte a pair, 0 hides it, by 4 strides (batch, head,
- * query, key; 0 broadcasts).  A query without a visible key: out 0, lse -inf, no gradient.  scale > 0.  No atomics: the same
- * bits on every run.  ws: *_workspace_bytes() bytes (may be 0), 16-byte aligned, contents free after the call.
+ * lies behind is never read, its dk and dv are 0.  mask or NULL: one byte a pair, 0 hides it (a stride of 0 broadcasts).  A
+ * query without a visible key: out 0, lse -inf, no gradient.  scale > 0.  No atomics: the same bits on every run.
+ * ws: *_workspace_bytes() bytes (may be 0), 16-byte aligned, contents free after the call.
  */
 int64_t adk_attend_fwd_workspace_bytes(int B, int H, int Hk, int Nq, int Nk, int D);
 int adk_attend_fwd(const void* q, const void* k, const void* v, void* out, float* lse, const int32_t* key_lengths, const uint8_t* mask,
-                   int dtype, int B, int H, int Hk, int Nq, int Nk, int D, const int64_t* q_strides, const int64_t* k_strides,
-                   const int64_t* v_strides, const int64_t* mask_strides, float scale, int causal, void* ws, int64_t ws_bytes,
-                   adk_stream_t stream);
+                   int dtype, int B, int H, int Hk, int Nq, int Nk, int D, const int64_t* strides, float scale, int causal, void* ws,
+                   int64_t ws_bytes, adk_stream_t stream);
 int64_t adk_attend_bwd_workspace_bytes(int B, int H, int Hk, int Nq, int Nk, int D);
 int adk_attend_bwd(const void* dout, const void* q, const void* k, const void* v, const void* out, const float* lse,
                    const int32_t* key_lengths, const uint8_t* mask, int dtype, int B, int H, int Hk, int Nq, int Nk, int D,
-                   const int64_t* dout_strides, const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides,
-                   const int64_t* mask_strides, float scale, int causal, void* dq, void* dk, void* dv, const int64_t* dq_strides,
-                   const int64_t* dk_strides, const int64_t* dv_strides, void* ws, int64_t ws_bytes, adk_stream_t stream);
+                   const int64_t* strides, float scale, int causal, void* dq, void* dk, void* dv, void* ws, int64_t ws_bytes,
+                   adk_stream_t stream);
 
 /* ------------------------------------------------------------ rotary positions
  * adk_rope_2d's rotation for any number of axes, a part of the head, either layout, long contexts, out of place or in place, and
- * its transpose (the gradient).  x, y [B,N,H,D] by element strides (batch, token, head), last dimension dense, y == x in place;
- * positions int64 by strides (batch, token, axis); frequencies [pairs] float64, radians a position, the same for every axis.
- * Channels [2 pairs a, 2 pairs (a + 1)) of the first `turned` heads turn by positions[..., a]; half: pairs (m, m + pairs) of the
- * segment, otherwise (2m, 2m + 1).  factor multiplies cosine and sine.  The angle is reduced in 64 bits.  Other channels and
- * heads are copied.  dtype as adk_rope_2d.
+ * its transpose (the gradient).  x, y [B,N,H,D], last dimension dense, y == x in place; positions int64; frequencies [pairs]
+ * float64, radians a position, the same for every axis.  strides: 9 element strides on the host, (batch, token, head) of x, of y
+ * and (batch, token, axis) of positions.  Channels [2 pairs a, 2 pairs (a + 1)) of the first `turned` heads turn by
+ * positions[..., a]; half: pairs (m, m + pairs) of the segment, otherwise (2m, 2m + 1).  factor multiplies cosine and sine.  The
+ * angle is reduced in 64 bits.  Other channels and heads are copied.  dtype as adk_rope_2d.
  */
 int adk_rotary(const void* x, void* y, const int64_t* positions, const double* frequencies, int dtype, int B, int N, int H, int D,
-               int turned, int pairs, int axes, int half, int transpose, float factor, const int64_t* x_strides,
-               const int64_t* y_strides, const int64_t* position_strides, adk_stream_t stream);
+               int turned, int pairs, int axes, int half, int transpose, float factor, const int64_t* strides, adk_stream_t stream);
 
 /* ----------------------------------------------- activation with an 8-bit checkpoint
  * Forward: y = act(x), x [rows, width]; gated: act(x[:, :width]) * x[:, width:], x [rows, 2 width]; and x as codes, 32 consecutive

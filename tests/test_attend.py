@@ -344,11 +344,11 @@ def test_refusals():
 
 def test_c_entry_refuses_before_any_launch(lib):
     import ctypes
-    i3 = (ctypes.c_int64 * 3)(8, 8, 8)
-    odd = (ctypes.c_int64 * 3)(8, 4, 8)
+    fine = (ctypes.c_int64 * 25)(*[8] * 25)
+    odd = (ctypes.c_int64 * 25)(8, 4, *[8] * 23)
     P = ctypes.c_void_p(1 << 20)
-    fwd = lambda q=P, D=64, H=4, Hk=2, Nq=4, dtype=0, s=i3, scale=1.0, out=P, ws=None, n=0: lib.adk_attend_fwd(  # noqa: E731
-        q, P, P, out, P, None, None, dtype, 1, H, Hk, Nq, 4096, D, s, i3, i3, None, scale, 0, ws, n, None)
+    fwd = lambda q=P, D=64, H=4, Hk=2, Nq=4, dtype=0, s=fine, scale=1.0, out=P, ws=None, n=0: lib.adk_attend_fwd(  # noqa: E731
+        q, P, P, out, P, None, None, dtype, 1, H, Hk, Nq, 4096, D, s, scale, 0, ws, n, None)
     assert fwd(D=60) == -3 and fwd(D=256) == -3 and fwd(dtype=1) == -3
     assert fwd(H=3) == -1 and fwd(scale=0.0) == -1 and fwd(scale=float("nan")) == -1 and fwd(q=None) == -1 and fwd(s=odd) == -1 and fwd(out=None) == -1
     assert fwd(q=ctypes.c_void_p((1 << 20) + 8)) == -1
@@ -356,7 +356,7 @@ def test_c_entry_refuses_before_any_launch(lib):
     assert fwd(Nq=0) == 0
     assert lib.adk_attend_fwd_workspace_bytes(1, 4, 2, 4, 4096, 64) > 0 and lib.adk_attend_fwd_workspace_bytes(1, 4, 3, 4, 4, 64) == -1
     assert lib.adk_attend_bwd_workspace_bytes(2, 4, 2, 8, 8, 64) == 4 * (64 + 4)
-    assert lib.adk_attend_bwd(P, P, P, P, P, P, None, None, 0, 1, 4, 2, 4, 4, 64, i3, i3, i3, i3, None, 1.0, 0, P, P, P, i3, i3, i3, None, 0, None) == -2
+    assert lib.adk_attend_bwd(P, P, P, P, P, P, None, None, 0, 1, 4, 2, 4, 4, 64, fine, 1.0, 0, P, P, P, None, 0, None) == -2
 
 
 def test_the_formulas_are_torchs():

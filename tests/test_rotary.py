@@ -195,7 +195,7 @@ def test_refusals(lib):
     with pytest.raises(_lib.AdkError, match="share"):
         ro.rotary_(torch.zeros(1, 4, 3, 16).expand(2, 4, 3, 16), pos, f)
     N = None
-    assert lib.adk_rotary(N, N, N, N, 0, 1, 1, 1, 16, 1, 9, 1, 1, 0, 1.0, N, N, N, N) == -1      # 18 channels of 16
-    assert lib.adk_rotary(N, N, N, N, 3, 1, 1, 1, 16, 1, 8, 1, 1, 0, 1.0, N, N, N, N) == -3
-    assert lib.adk_rotary(N, N, N, N, 0, 1, 1, 1, 16, 1, 8, 1, 1, 0, 1.0, N, N, N, N) == -1
-    assert lib.adk_rotary(N, N, N, N, 0, 0, 1, 1, 16, 1, 8, 1, 1, 0, 1.0, N, N, N, N) == 0
+    assert lib.adk_rotary(N, N, N, N, 0, 1, 1, 1, 16, 1, 9, 1, 1, 0, 1.0, N, N) == -1      # 18 channels of 16
+    assert lib.adk_rotary(N, N, N, N, 3, 1, 1, 1, 16, 1, 8, 1, 1, 0, 1.0, N, N) == -3
+    assert lib.adk_rotary(N, N, N, N, 0, 1, 1, 1, 16, 1, 8, 1, 1, 0, 1.0, N, N) == -1
+    assert lib.adk_rotary(N, N, N, N, 0, 0, 1, 1, 16, 1, 8, 1, 1, 0, 1.0, N, N) == 0
