@@ -102,38 +102,43 @@ template <typename T, int DP> __device__ __forceinline__ typename AtEl<T>::x8 at
     return __builtin_shufflevector(__builtin_bit_cast(typename AtEl<T>::x4, lo), __builtin_bit_cast(typename AtEl<T>::x4, hi), 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
-// A tile of AT_TILE rows on its way from memory to LDS: this thread's 16-byte chunks.
-template <typename T, int DP> struct AtStage {
-    static constexpr int CH = DP / 8, STEP = 256 / CH, IT = AT_TILE / STEP;
-    at_u32x4 r[IT];
-    __device__ __forceinline__ void put(T* tile) const {
-        const int ch = threadIdx.x % CH, r0 = threadIdx.x / CH;
-#pragma unroll
-        for (int i = 0; i < IT; ++i) *reinterpret_cast<at_u32x4*>(tile + at_off<DP>(r0 + i * STEP, ch)) = r[i];
-    }
-    // keys: rows past `end` repeat the last one before it (they are hidden in the scores, and what lies there is never read)
-    __device__ __forceinline__ void get_keys(const T* base, int64_t sn, int first, int end, int D) {
-        const int ch = threadIdx.x % CH, r0 = threadIdx.x / CH;
-#pragma unroll
-        for (int i = 0; i < IT; ++i) {
-            const int row = min(first + r0 + i * STEP, end - 1);
-            r[i] = ch * 8 < D ? *reinterpret_cast<const at_u32x4*>(base + (int64_t)row * sn + ch * 8) : at_u32x4{0, 0, 0, 0};
-        }
-    }
-    // a mask that is the same for every query hides a key altogether: zeros, whatever stands there
-    __device__ __forceinline__ void hide_keys(const uint8_t* mask, int64_t sk, int first, int end) {
-        const int r0 = threadIdx.x / CH;
-#pragma unroll
-        for (int i = 0; i < IT; ++i)
-            if (!mask[(int64_t)min(first + r0 + i * STEP, end - 1) * sk]) r[i] = at_u32x4{0, 0, 0, 0};
-    }
-    __device__ __forceinline__ void get_rows(const T* base, int64_t sh, int64_t sn, int first, int R, int Nq, int D) {
-        const int ch = threadIdx.x % CH, r0 = threadIdx.x / CH;
+// A tile of AT_TILE rows goes from memory to LDS without passing through registers: each wave instruction moves 64 chunks of 16 bytes
+// to consecutive LDS addresses, so the swizzle is in which chunk a lane asks for.  In asm because the compiler waits for the
+// builtin's loads before any LDS read; the waits are at_landed() before the barrier that hands a tile over.  The address is a
+// uniform base and a 32-bit byte offset (token strides are below 2^24 elements).
+__device__ __forceinline__ void at_lds16(uint32_t lds, const void* base, uint32_t offset) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(offset), "s"(base) : "memory");
+}
+__device__ __forceinline__ void at_landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+template <typename T, int DP> struct AtTile {
+    static constexpr int CH = DP / 8, IT = AT_TILE * CH / 256;
+    // rows from base on; those past the `rows` (>= 1) that there are repeat the last (they are hidden in the scores, and what lies
+    // there is never read); chunks past D are left as they are
+    static __device__ __forceinline__ void load(T* tile, const T* base, int sn, int rows, int D) {
+        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+        const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)tile;
 #pragma unroll
         for (int i = 0; i < IT; ++i) {
-            const int row = min(first + r0 + i * STEP, R - 1), g = row / Nq;
-            r[i] = ch * 8 < D ? *reinterpret_cast<const at_u32x4*>(base + (int64_t)g * sh + (int64_t)(row - g * Nq) * sn + ch * 8) : at_u32x4{0, 0, 0, 0};
+            const int row = (4 * i + wave) * (64 / CH) + lane / CH, chunk = (lane % CH) ^ at_swz<DP>(row);
+            const uint32_t off = (uint32_t)min(row, rows - 1) * (uint32_t)sn * 2u + chunk * 16;
+            if (DP == D || chunk * 8 < D) at_lds16(lds + (4 * i + wave) * 1024, base, off);
         }
+    }
+    // a mask that is the same for every query hides a key altogether: zeros, whatever stands there (by the lanes that loaded it)
+    static __device__ __forceinline__ void hide(T* tile, const uint8_t* mask, int64_t sk, int rows) {
+        const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+#pragma unroll
+        for (int i = 0; i < IT; ++i) {
+            const int row = (4 * i + wave) * (64 / CH) + lane / CH;
+            if (!mask[(int64_t)min(row, rows - 1) * sk]) *reinterpret_cast<at_u32x4*>(tile + (4 * i + wave) * 512 + lane * 8) = at_u32x4{0, 0, 0, 0};
+        }
+    }
+    // zeros in the chunks past D of `tiles` tiles, which no load touches
+    static __device__ __forceinline__ void pad(T* first, int tiles, int D) {
+        if (D == DP) return;
+        for (int n = threadIdx.x; n < tiles * AT_TILE * CH; n += 256)
+            if (((n % CH) ^ at_swz<DP>(n / CH % AT_TILE)) * 8 >= D) *reinterpret_cast<at_u32x4*>(first + n * 8) = at_u32x4{0, 0, 0, 0};
     }
 };
 
@@ -170,13 +175,28 @@ __device__ __forceinline__ uint32_t at_below_bits(int k0, int lim) {
     return bits;
 }
 
+// A workgroup's LDS.  The tiles come first: the loads' 16-bit LDS base has to reach them.
+template <typename T, int DP> struct AtShared {
+    T tiles[2][2][AT_TILE * DP];
+    int tops[4];
+    float unit4[4];
+};
+template <typename T, int DP, bool MASKED> struct AtSharedKeys {
+    T tiles[2][2][AT_TILE * DP];
+    float lse[2][AT_TILE], delta[2][AT_TILE];
+    int lim[2][AT_TILE];
+    int64_t mask[MASKED ? 2 : 1][MASKED ? AT_TILE : 1];
+    float unit4[4];
+};
+
 // ------------------------------------------------------------------------------------------------------------------- forward
 template <typename T, int DP, bool MASKED>
 __global__ __launch_bounds__(256, 2) void at_fwd_kernel(AttendArgs a)
 {
     typedef typename AtEl<T>::x8 x8;
     typedef typename AtEl<T>::x4 x4;
-    __shared__ __attribute__((aligned(16))) T smem[2][2][AT_TILE * DP];
+    __shared__ __attribute__((aligned(16))) AtShared<T, DP> sh;
+    auto& smem = sh.tiles;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, c = lane & 31;
     const int R = a.G * a.Nq, tiles = (R + AT_ROWS - 1) / AT_ROWS;
     int id = xcd_remap(blockIdx.x, gridDim.x);
@@ -191,10 +211,10 @@ __global__ __launch_bounds__(256, 2) void at_fwd_kernel(AttendArgs a)
     const int head = kh * a.G + g;
     const int lim = row >= R ? 0 : a.causal ? min(len, max(0, i + a.Nk - a.Nq + 1)) : len; // this row sees keys below lim
     const int wave_top = at_wave_max(lim), wave_low = at_wave_min(row < R ? lim : 0x7fffffff);
-    __shared__ int tops[4];
+    int* const tops = sh.tops;
     if (lane == 0) tops[wave] = wave_top;
     __syncthreads();
-    const int top = max(max(tops[0], tops[1]), max(tops[2], tops[3]));
+    const int top = __builtin_amdgcn_readfirstlane(max(max(tops[0], tops[1]), max(tops[2], tops[3])));
     const int all = (top + AT_TILE - 1) / AT_TILE, per = (all + a.splits - 1) / a.splits;
     const int t0 = split * per, t1 = min(all, t0 + per);
 
@@ -212,17 +232,22 @@ __global__ __launch_bounds__(256, 2) void at_fwd_kernel(AttendArgs a)
     at_f32x16 ot[DP / 32] = {};
     float m_run = -INFINITY, l_run = 0.f; // running maximum (raw scores), this lane's share of the sum
 
-    AtStage<T, DP> sk, sv;
-    auto fetch = [&](int t) {
-        sk.get_keys(kb, a.k_sn, t * AT_TILE, len, a.D);
-        sv.get_keys(vb, a.v_sn, t * AT_TILE, len, a.D);
-        if (MASKED && a.mask_by_key) { sk.hide_keys(mkey, a.m_sk, t * AT_TILE, len); sv.hide_keys(mkey, a.m_sk, t * AT_TILE, len); }
+    auto load = [&](int t, int buf) {
+        AtTile<T, DP>::load(smem[buf][0], kb + (int64_t)t * AT_TILE * a.k_sn, (int)a.k_sn, len - t * AT_TILE, a.D);
+        AtTile<T, DP>::load(smem[buf][1], vb + (int64_t)t * AT_TILE * a.v_sn, (int)a.v_sn, len - t * AT_TILE, a.D);
     };
-    if (t0 < t1) { fetch(t0); sk.put(smem[0][0]); sv.put(smem[0][1]); }
+    AtTile<T, DP>::pad(smem[0][0], 4, a.D);
+    if (t0 < t1) load(t0, 0);
     for (int t = t0; t < t1; ++t) {
+        const int buf = (t - t0) & 1;
+        at_landed();
+        if (MASKED && a.mask_by_key) {
+            AtTile<T, DP>::hide(smem[buf][0], mkey + (int64_t)t * AT_TILE * a.m_sk, a.m_sk, len - t * AT_TILE);
+            AtTile<T, DP>::hide(smem[buf][1], mkey + (int64_t)t * AT_TILE * a.m_sk, a.m_sk, len - t * AT_TILE);
+        }
         __syncthreads(); // tile t is in place, and nobody reads the other buffer any more
-        const T *tk = smem[(t - t0) & 1][0], *tv = smem[(t - t0) & 1][1];
-        if (t + 1 < t1) fetch(t + 1);
+        const T *tk = smem[buf][0], *tv = smem[buf][1];
+        if (t + 1 < t1) load(t + 1, buf ^ 1);
         if (t * AT_TILE < wave_top) {
             at_f32x16 st[2] = {};
 #pragma unroll
@@ -273,7 +298,6 @@ __global__ __launch_bounds__(256, 2) void at_fwd_kernel(AttendArgs a)
 #pragma unroll
                     for (int db = 0; db < DP / 32; ++db) ot[db] = AtEl<T>::mfma(at_colfrag<T, DP>(tv, 32 * n + 16 * s, db, lane), pf[n][s], ot[db]);
         }
-        if (t + 1 < t1) { sk.put(smem[(t + 1 - t0) & 1][0]); sv.put(smem[(t + 1 - t0) & 1][1]); }
     }
 
     const float l = l_run + at_other_half(l_run);
@@ -386,16 +410,16 @@ __global__ __launch_bounds__(256, 2) void at_bwd_rows_kernel(AttendArgs a)
 {
     typedef typename AtEl<T>::x8 x8;
     typedef typename AtEl<T>::x4 x4;
-    __shared__ __attribute__((aligned(16))) T smem[2][2][AT_TILE * DP];
-    __shared__ float unit4[4];
-    __shared__ int tops[4];
+    __shared__ __attribute__((aligned(16))) AtShared<T, DP> sh;
+    auto& smem = sh.tiles;
+    int* const tops = sh.tops;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, c = lane & 31;
     const int R = a.G * a.Nq, tiles = (R + AT_ROWS - 1) / AT_ROWS;
     int id = xcd_remap(blockIdx.x, gridDim.x);
     const int tile = a.causal ? tiles - 1 - id % tiles : id % tiles;
     id /= tiles;
     const int kh = id % a.Hk, b = id / a.Hk;
-    const float unit = at_grad_unit<T>(a, b, kh, unit4);
+    const float unit = at_grad_unit<T>(a, b, kh, sh.unit4);
 
     const int len = a.key_lengths ? min(max(a.key_lengths[b], 0), a.Nk) : a.Nk;
     const int row = tile * AT_ROWS + wave * 32 + c, rowc = min(row, R - 1), g = rowc / a.Nq, i = rowc - g * a.Nq;
@@ -404,7 +428,7 @@ __global__ __launch_bounds__(256, 2) void at_bwd_rows_kernel(AttendArgs a)
     const int wave_top = at_wave_max(lim), wave_low = at_wave_min(row < R ? lim : 0x7fffffff);
     if (lane == 0) tops[wave] = wave_top;
     __syncthreads();
-    const int t1 = (max(max(tops[0], tops[1]), max(tops[2], tops[3])) + AT_TILE - 1) / AT_TILE;
+    const int t1 = (__builtin_amdgcn_readfirstlane(max(max(tops[0], tops[1]), max(tops[2], tops[3]))) + AT_TILE - 1) / AT_TILE;
 
     const T* kb = static_cast<const T*>(a.k) + (int64_t)b * a.k_sb + (int64_t)kh * a.k_sh;
     const T* vb = static_cast<const T*>(a.v) + (int64_t)b * a.v_sb + (int64_t)kh * a.v_sh;
@@ -421,17 +445,22 @@ __global__ __launch_bounds__(256, 2) void at_bwd_rows_kernel(AttendArgs a)
     const float lse = a.lse[at], neg_lse = lse == -INFINITY ? -INFINITY : -lse * 1.4426950408889634f, neg_delta = -a.delta[at] * unit;
     at_f32x16 acc[DP / 32] = {};
 
-    AtStage<T, DP> sk, sv;
-    auto fetch = [&](int t) {
-        sk.get_keys(kb, a.k_sn, t * AT_TILE, len, a.D);
-        sv.get_keys(vb, a.v_sn, t * AT_TILE, len, a.D);
-        if (MASKED && a.mask_by_key) { sk.hide_keys(mkey, a.m_sk, t * AT_TILE, len); sv.hide_keys(mkey, a.m_sk, t * AT_TILE, len); }
+    auto load = [&](int t, int buf) {
+        AtTile<T, DP>::load(smem[buf][0], kb + (int64_t)t * AT_TILE * a.k_sn, (int)a.k_sn, len - t * AT_TILE, a.D);
+        AtTile<T, DP>::load(smem[buf][1], vb + (int64_t)t * AT_TILE * a.v_sn, (int)a.v_sn, len - t * AT_TILE, a.D);
     };
-    if (0 < t1) { fetch(0); sk.put(smem[0][0]); sv.put(smem[0][1]); }
+    AtTile<T, DP>::pad(smem[0][0], 4, a.D);
+    if (t1 > 0) load(0, 0);
     for (int t = 0; t < t1; ++t) {
-        __syncthreads();
-        const T *tk = smem[t & 1][0], *tv = smem[t & 1][1];
-        if (t + 1 < t1) fetch(t + 1);
+        const int buf = t & 1;
+        at_landed();
+        if (MASKED && a.mask_by_key) {
+            AtTile<T, DP>::hide(smem[buf][0], mkey + (int64_t)t * AT_TILE * a.m_sk, a.m_sk, len - t * AT_TILE);
+            AtTile<T, DP>::hide(smem[buf][1], mkey + (int64_t)t * AT_TILE * a.m_sk, a.m_sk, len - t * AT_TILE);
+        }
+        __syncthreads(); // tile t is in place, and nobody reads the other buffer any more
+        const T *tk = smem[buf][0], *tv = smem[buf][1];
+        if (t + 1 < t1) load(t + 1, buf ^ 1);
         if (t * AT_TILE < wave_top) {
             at_f32x16 st[2] = {}, dp[2] = {};
 #pragma unroll
@@ -441,23 +470,24 @@ __global__ __launch_bounds__(256, 2) void at_bwd_rows_kernel(AttendArgs a)
                     st[n] = AtEl<T>::mfma(at_rowfrag<T, DP>(tk, 32 * n, ks, lane), qf[ks], st[n]);
                     dp[n] = AtEl<T>::mfma(at_rowfrag<T, DP>(tv, 32 * n, ks, lane), gf[ks], dp[n]);
                 }
-            const bool edge = MASKED || (t + 1) * AT_TILE > wave_low;
+            if (MASKED || (t + 1) * AT_TILE > wave_low) {
+#pragma unroll
+                for (int n = 0; n < 2; ++n) {
+                    const int k0 = t * AT_TILE + 32 * n + 4 * h;
+                    uint32_t see = at_below_bits(k0, lim);
+                    if (MASKED) see &= at_mask_bits(mrow, a.m_sk, k0, a.Nk - 1, a.m_sk == 1 && (t + 1) * AT_TILE <= a.Nk);
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) st[n][r] = (see >> r) & 1u ? st[n][r] : -INFINITY;
+                }
+            }
             x8 ds[2][2];
 #pragma unroll
-            for (int n = 0; n < 2; ++n) {
-                uint32_t see = 0xffffu;
-                if (edge) {
-                    const int k0 = t * AT_TILE + 32 * n + 4 * h;
-                    see = at_below_bits(k0, lim);
-                    if (MASKED) see &= at_mask_bits(mrow, a.m_sk, k0, a.Nk - 1, a.m_sk == 1 && (t + 1) * AT_TILE <= a.Nk);
-                }
+            for (int n = 0; n < 2; ++n)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
                     const float p = __builtin_amdgcn_exp2f(fmaf(st[n][r], a.scale_log2e, neg_lse));
-                    const float x = p * fmaf(dp[n][r], unit, neg_delta);
-                    ds[n][r >> 3][r & 7] = (T)((see >> r) & 1u ? x : 0.f);
+                    ds[n][r >> 3][r & 7] = (T)(p * fmaf(dp[n][r], unit, neg_delta));
                 }
-            }
 #pragma unroll
             for (int n = 0; n < 2; ++n)
 #pragma unroll
@@ -465,7 +495,6 @@ __global__ __launch_bounds__(256, 2) void at_bwd_rows_kernel(AttendArgs a)
 #pragma unroll
                     for (int db = 0; db < DP / 32; ++db) acc[db] = AtEl<T>::mfma(at_colfrag<T, DP>(tk, 32 * n + 16 * s, db, lane), ds[n][s], acc[db]);
         }
-        if (t + 1 < t1) { sk.put(smem[(t + 1) & 1][0]); sv.put(smem[(t + 1) & 1][1]); }
     }
     if (row >= R) return;
     const float f = a.scale / unit;
@@ -485,24 +514,21 @@ __global__ __launch_bounds__(256, 2) void at_bwd_rows_kernel(AttendArgs a)
 
 // dK, dV: a wave owns 32 keys and walks the rows that may see them.
 template <typename T, int DP, bool MASKED>
-__global__ __launch_bounds__(256, 1) void at_bwd_keys_kernel(AttendArgs a)
+__global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void at_bwd_keys_kernel(AttendArgs a)
 {
     typedef typename AtEl<T>::x8 x8;
     typedef typename AtEl<T>::x4 x4;
-    __shared__ __attribute__((aligned(16))) T smem[2][2][AT_TILE * DP];
-    __shared__ __attribute__((aligned(16))) float s_lse[2][AT_TILE], s_delta[2][AT_TILE];
-    __shared__ __attribute__((aligned(16))) int s_lim[2][AT_TILE];
-    __shared__ int64_t s_mask[MASKED ? 2 : 1][AT_TILE];
-    __shared__ float unit4[4];
+    __shared__ __attribute__((aligned(16))) AtSharedKeys<T, DP, MASKED> sh;
+    auto& smem = sh.tiles;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, c = lane & 31;
     const int R = a.G * a.Nq, tiles = (a.Nk + AT_ROWS - 1) / AT_ROWS, off = a.Nk - a.Nq;
     int id = xcd_remap(blockIdx.x, gridDim.x);
     const int tile = id % tiles; // causal: the first keys are seen by most rows, the long ones come first as they are
     id /= tiles;
     const int kh = id % a.Hk, b = id / a.Hk;
-    const float unit = at_grad_unit<T>(a, b, kh, unit4);
+    const float unit = at_grad_unit<T>(a, b, kh, sh.unit4);
     const int len = a.key_lengths ? min(max(a.key_lengths[b], 0), a.Nk) : a.Nk;
-    const int k0 = tile * AT_ROWS, key = k0 + wave * 32 + c;
+    const int k0 = tile * AT_ROWS, wave_k0 = k0 + __builtin_amdgcn_readfirstlane(wave) * 32, key = wave_k0 + c;
 
     at_f32x16 dk[DP / 32] = {}, dv[DP / 32] = {};
     if (k0 < len) {
@@ -518,54 +544,47 @@ __global__ __launch_bounds__(256, 1) void at_bwd_keys_kernel(AttendArgs a)
         const T* gb = static_cast<const T*>(a.dout) + (int64_t)b * a.g_sb + (int64_t)kh * a.G * a.g_sh;
         const int64_t at0 = ((int64_t)b * a.Hk + kh) * R;
         const uint8_t* mkey = MASKED ? a.mask + (int64_t)b * a.m_sb + (int64_t)kh * a.G * a.m_sh + (int64_t)keyc * a.m_sk : nullptr;
-        const int t1 = (R + AT_TILE - 1) / AT_TILE;
-        // the next tile from t on with a row that sees a key of this workgroup
-        auto seek = [&](int t) {
-            if (!a.causal) return t;
-            for (; t < t1; ++t) {
-                const int r0 = t * AT_TILE, r1 = min(r0 + AT_TILE, R) - 1, g0 = r0 / a.Nq, g1 = r1 / a.Nq;
-                const int last = g1 > g0 ? a.Nq - 1 : r1 - g1 * a.Nq;
-                if (last + off >= k0) break;
-            }
-            return t;
-        };
-        AtStage<T, DP> sq, sg;
+        if (MASKED && a.mask_by_key && !mkey[0]) {
+#pragma unroll
+            for (int ks = 0; ks < DP / 16; ++ks) { kf[ks] = x8{}; vf[ks] = x8{}; }
+        }
+        // the tiles: head by head, from the first query that sees a key of this workgroup
+        const int i_first = a.causal ? max(0, k0 - off) : 0, per_head = a.Nq > i_first ? (a.Nq - i_first + AT_TILE - 1) / AT_TILE : 0, t1 = a.G * per_head;
+        int g_next = 0, i_next = i_first;
         float n_lse = 0.f, n_delta = 0.f;
         int n_lim = -1;
         int64_t n_mask = 0;
-        auto fetch = [&](int t) {
-            sq.get_rows(qb, a.q_sh, a.q_sn, t * AT_TILE, R, a.Nq, a.D);
-            sg.get_rows(gb, a.g_sh, a.g_sn, t * AT_TILE, R, a.Nq, a.D);
+        auto load = [&](int buf) { // tile (g_next, i_next)
+            AtTile<T, DP>::load(smem[buf][0], qb + (int64_t)g_next * a.q_sh + (int64_t)i_next * a.q_sn, (int)a.q_sn, a.Nq - i_next, a.D);
+            AtTile<T, DP>::load(smem[buf][1], gb + (int64_t)g_next * a.g_sh + (int64_t)i_next * a.g_sn, (int)a.g_sn, a.Nq - i_next, a.D);
             if (threadIdx.x < AT_TILE) {
-                const int row = t * AT_TILE + threadIdx.x, rowc = min(row, R - 1), g = rowc / a.Nq, i = rowc - g * a.Nq;
-                const float lse = a.lse[at0 + rowc];
+                const int i = i_next + threadIdx.x, ic = min(i, a.Nq - 1);
+                const int64_t at = at0 + (int64_t)g_next * a.Nq + ic;
+                const float lse = a.lse[at];
                 n_lse = lse == -INFINITY ? -INFINITY : -lse * 1.4426950408889634f;
-                n_delta = -a.delta[at0 + rowc] * unit;
-                n_lim = row >= R ? -1 : a.causal ? min(len - 1, i + off) : len - 1; // the last key that the row sees
-                if (MASKED) n_mask = (int64_t)g * a.m_sh + (int64_t)i * a.m_sq;
+                n_delta = -a.delta[at] * unit;
+                n_lim = i >= a.Nq ? -1 : a.causal ? min(len - 1, i + off) : len - 1; // the last key that the row sees
+                if (MASKED) n_mask = (int64_t)g_next * a.m_sh + (int64_t)ic * a.m_sq;
             }
         };
-        auto put = [&](int buf) {
-            sq.put(smem[buf][0]);
-            sg.put(smem[buf][1]);
+        auto note = [&](int buf) {
             if (threadIdx.x < AT_TILE) {
-                s_lse[buf][threadIdx.x] = n_lse; s_delta[buf][threadIdx.x] = n_delta; s_lim[buf][threadIdx.x] = n_lim;
-                if (MASKED) s_mask[buf][threadIdx.x] = n_mask;
+                sh.lse[buf][threadIdx.x] = n_lse; sh.delta[buf][threadIdx.x] = n_delta; sh.lim[buf][threadIdx.x] = n_lim;
+                if (MASKED) sh.mask[buf][threadIdx.x] = n_mask;
             }
         };
-        int t = seek(0), buf = 0;
-        if (t < t1) { fetch(t); put(0); }
-        while (t < t1) {
+        AtTile<T, DP>::pad(smem[0][0], 4, a.D);
+        if (t1 > 0) { load(0); note(0); }
+        for (int t = 0; t < t1; ++t) {
+            const int buf = t & 1, i0 = i_next;
+            i_next += AT_TILE;
+            if (i_next >= a.Nq) { i_next = i_first; ++g_next; }
+            at_landed();
             __syncthreads();
             const T *tq = smem[buf][0], *tg = smem[buf][1];
-            const int next = seek(t + 1);
-            if (next < t1) fetch(next);
-            // every row of the tile sees every key of the wave: nothing to hide
-            bool edge = MASKED || (t + 1) * AT_TILE > R || k0 + wave * 32 + 32 > len;
-            if (a.causal && !edge) {
-                const int g0 = (t * AT_TILE) / a.Nq, g1 = (t * AT_TILE + AT_TILE - 1) / a.Nq;
-                edge = (g1 > g0 ? 0 : t * AT_TILE - g0 * a.Nq) + off < k0 + wave * 32 + 31;
-            }
+            if (t + 1 < t1) load(buf ^ 1);
+            // unless every row of the tile sees every key of the wave
+            const bool edge = MASKED || i0 + AT_TILE > a.Nq || wave_k0 + 32 > len || (a.causal && i0 + off < wave_k0 + 31);
 #pragma unroll
             for (int n = 0; n < 2; ++n) {
                 at_f32x16 st = {}, dp = {};
@@ -574,29 +593,26 @@ __global__ __launch_bounds__(256, 1) void at_bwd_keys_kernel(AttendArgs a)
                     st = AtEl<T>::mfma(at_rowfrag<T, DP>(tq, 32 * n, ks, lane), kf[ks], st);
                     dp = AtEl<T>::mfma(at_rowfrag<T, DP>(tg, 32 * n, ks, lane), vf[ks], dp);
                 }
-                uint32_t see = 0xffffu;
                 if (edge) {
-                    see = 0;
 #pragma unroll
                     for (int r = 0; r < 16; ++r) {
                         const int q = 32 * n + 8 * (r >> 2) + 4 * h + (r & 3);
-                        bool on = key <= s_lim[buf][q];
-                        if (MASKED) on = on & (mkey[s_mask[buf][q]] != 0);
-                        see |= (on ? 1u : 0u) << r;
+                        bool on = key <= sh.lim[buf][q];
+                        if (MASKED) on = on & (mkey[sh.mask[buf][q]] != 0);
+                        st[r] = on ? st[r] : -INFINITY;
                     }
                 }
                 x8 pf[2], df[2];
 #pragma unroll
                 for (int r4 = 0; r4 < 4; ++r4) {
                     const int q0 = 32 * n + 8 * r4 + 4 * h;
-                    const at_f32x4 nl = *reinterpret_cast<const at_f32x4*>(&s_lse[buf][q0]), nd = *reinterpret_cast<const at_f32x4*>(&s_delta[buf][q0]);
+                    const at_f32x4 nl = *reinterpret_cast<const at_f32x4*>(&sh.lse[buf][q0]), nd = *reinterpret_cast<const at_f32x4*>(&sh.delta[buf][q0]);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const int r = 4 * r4 + e;
                         const float p = __builtin_amdgcn_exp2f(fmaf(st[r], a.scale_log2e, nl[e]));
-                        const float x = p * fmaf(dp[r], unit, nd[e]);
-                        pf[r >> 3][r & 7] = (T)((see >> r) & 1u ? p : 0.f);
-                        df[r >> 3][r & 7] = (T)((see >> r) & 1u ? x : 0.f);
+                        pf[r >> 3][r & 7] = (T)p;
+                        df[r >> 3][r & 7] = (T)(p * fmaf(dp[r], unit, nd[e]));
                     }
                 }
 #pragma unroll
@@ -607,9 +623,7 @@ __global__ __launch_bounds__(256, 1) void at_bwd_keys_kernel(AttendArgs a)
                         dk[db] = AtEl<T>::mfma(at_colfrag<T, DP>(tq, 32 * n + 16 * s, db, lane), df[s], dk[db]);
                     }
             }
-            if (next < t1) put(buf ^ 1);
-            t = next;
-            buf ^= 1;
+            if (t + 1 < t1) note(buf ^ 1);
         }
     }
     if (key >= a.Nk) return;
@@ -650,7 +664,10 @@ static int at_check(int dtype, int B, int H, int Hk, int Nq, int Nk, int D, floa
 }
 
 // s: strides (batch, head, token)
-static int at_tensor(const void* p, const int64_t* s) { return (!p || ((uintptr_t)p & 15) || ((s[0] | s[1] | s[2]) & 7)) ? ADK_EINVAL : 0; }
+static int at_tensor(const void* p, const int64_t* s) {
+    if (!p || ((uintptr_t)p & 15) || ((s[0] | s[1] | s[2]) & 7)) return ADK_EINVAL;
+    return s[2] < 0 || s[2] >= (1 << 24) ? ADK_EUNSUPPORTED : 0; // 64 rows of a tile in 32-bit byte offsets
+}
 
 #define AT_LAUNCH3(KERNEL, T, GRID)                                                                                             \
     do {                                                                                                                        \
@@ -708,11 +725,11 @@ extern "C" int64_t adk_attend_fwd_workspace_bytes(int B, int H, int Hk, int Nq, 
 extern "C" int adk_attend_fwd(const void* q, const void* k, const void* v, void* out, float* lse, const int32_t* key_lengths, const uint8_t* mask, int dtype, int B, int H,
                               int Hk, int Nq, int Nk, int D, const int64_t* strides, float scale, int causal, void* ws, int64_t ws_bytes, hipStream_t stream)
 {
-    const int e = adk::at_check(dtype, B, H, Hk, Nq, Nk, D, scale);
+    int e = adk::at_check(dtype, B, H, Hk, Nq, Nk, D, scale);
     if (e) return e;
     if ((int64_t)B * Nq == 0) return 0;
-    if (!strides || adk::at_tensor(q, strides) || !out || ((uintptr_t)out & 7) || !lse) return ADK_EINVAL;
-    if (Nk && (adk::at_tensor(k, strides + 3) || adk::at_tensor(v, strides + 6))) return ADK_EINVAL;
+    if (!strides || !out || ((uintptr_t)out & 7) || !lse) return ADK_EINVAL;
+    if ((e = adk::at_tensor(q, strides)) || (Nk && ((e = adk::at_tensor(k, strides + 3)) || (e = adk::at_tensor(v, strides + 6))))) return e;
     adk::AttendArgs a = {};
     adk::at_fill(a, q, k, v, lse, key_lengths, mask, B, H, Hk, Nq, Nk, D, strides, scale, causal);
     a.out = out;
@@ -738,13 +755,14 @@ extern "C" int adk_attend_bwd(const void* dout, const void* q, const void* k, co
                               const uint8_t* mask, int dtype, int B, int H, int Hk, int Nq, int Nk, int D, const int64_t* strides, float scale, int causal, void* dq,
                               void* dk, void* dv, void* ws, int64_t ws_bytes, hipStream_t stream)
 {
-    const int e = adk::at_check(dtype, B, H, Hk, Nq, Nk, D, scale);
+    int e = adk::at_check(dtype, B, H, Hk, Nq, Nk, D, scale);
     if (e) return e;
     if (B == 0 || (Nq == 0 && Nk == 0)) return 0;
     if (!strides) return ADK_EINVAL;
     const int64_t* s = strides + 13; // of dout, dq, dk, dv
-    if (Nq && (adk::at_tensor(q, strides) || adk::at_tensor(dout, s) || adk::at_tensor(dq, s + 3) || !out || ((uintptr_t)out & 15) || !lse)) return ADK_EINVAL;
-    if (Nk && (adk::at_tensor(k, strides + 3) || adk::at_tensor(v, strides + 6) || adk::at_tensor(dk, s + 6) || adk::at_tensor(dv, s + 9))) return ADK_EINVAL;
+    if (Nq && (!out || ((uintptr_t)out & 15) || !lse)) return ADK_EINVAL;
+    if (Nq && ((e = adk::at_tensor(q, strides)) || (e = adk::at_tensor(dout, s)) || (e = adk::at_tensor(dq, s + 3)))) return e;
+    if (Nk && ((e = adk::at_tensor(k, strides + 3)) || (e = adk::at_tensor(v, strides + 6)) || (e = adk::at_tensor(dk, s + 6)) || (e = adk::at_tensor(dv, s + 9)))) return e;
     adk::AttendArgs a = {};
     adk::at_fill(a, q, k, v, lse, key_lengths, mask, B, H, Hk, Nq, Nk, D, strides, scale, causal);
     a.dout = dout; a.out_in = out; a.dq = dq; a.dk = dk; a.dv = dv;
