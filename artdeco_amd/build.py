@@ -33,6 +33,9 @@ COMMON_FLAGS = ["--offload-arch=" + ARCH, "-O3", "-std=c++17", "-fPIC", "-Wall",
 # integer decision (radii, tile ids, sort keys) or is compared bit-exactly
 # against the oracle; fast contraction only in the compositing kernels.
 EXTRA_FLAGS = {
+    # matrix products in the form whose accumulators are ordinary registers: in the other form the compiler moves dK, dV (head size 128)
+    # between the two halves of the register file on every tile, 320 moves for 64 products
+    "attend.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "adam.hip": ["-ffp-contract=off"],
     "raster_project.hip": ["-ffp-contract=off"],
     "matching.hip": ["-ffp-contract=off"],
