@@ -19,6 +19,10 @@
 // e % 4, the order the accumulator has), and likewise S = Q K^T gives P, dS as B operands of dV^T = dO^T P, dK^T = Q^T dS.  The
 // transposed A operands come from row-major tiles through ds_read_b64_tr_b16.
 //
+// Two shapes.  Wide: a workgroup owns 128 rows (or keys), 32 a wave, and its four waves share tiles of 64 keys (or rows).  Narrow, for
+// calls too small to fill the chip so: a workgroup owns 32, and each wave walks every fourth tile of 32 with LDS tiles of its own and
+// no barrier; the four partial results are joined through LDS at the end, in a fixed order.
+//
 // LDS tiles hold 16-byte chunks at chunk ^ f(row): with f below, the 16 rows of a 128-bit fragment read and the 4 rows of a
 // transposing read fall on different banks without padding.
 #include "adk_common.hpp"
@@ -63,8 +67,13 @@ struct AttendArgs {
     float scale, scale_log2e;
 };
 
-#define AT_ROWS 128 // rows (or keys) that a workgroup owns: 4 waves of 32
-#define AT_TILE 64  // keys (or rows) of a staged tile
+// A shape's numbers.
+template <bool NARROW> struct AtShape {
+    static constexpr int OWN = NARROW ? 32 : 128;   // rows (or keys) that a workgroup owns
+    static constexpr int TILE = NARROW ? 32 : 64;   // keys (or rows) of a staged tile
+    static constexpr int WAVES = NARROW ? 1 : 4;    // waves that share a tile
+    static constexpr int STREAMS = NARROW ? 4 : 1;  // tiles in work at once
+};
 
 template <int DP> __device__ __forceinline__ int at_swz(int row) {
     return DP == 64 ? ((((row >> 1) & 1) << 2) | ((row >> 2) & 3)) : (((row & 3) << 2) | ((row >> 2) & 3));
@@ -102,43 +111,46 @@ template <typename T, int DP> __device__ __forceinline__ typename AtEl<T>::x8 at
     return __builtin_shufflevector(__builtin_bit_cast(typename AtEl<T>::x4, lo), __builtin_bit_cast(typename AtEl<T>::x4, hi), 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
-// A tile of AT_TILE rows goes from memory to LDS without passing through registers: each wave instruction moves 64 chunks of 16 bytes
+// A tile goes from memory to LDS without passing through registers: each wave instruction moves 64 chunks of 16 bytes
 // to consecutive LDS addresses, so the swizzle is in which chunk a lane asks for.  In asm because the compiler waits for the
-// builtin's loads before any LDS read; the waits are at_landed() before the barrier that hands a tile over.  The address is a
+// builtin's loads before any LDS read; the waits are at_landed() before a tile is read.  The address is a
 // uniform base and a 32-bit byte offset (token strides are below 2^24 elements).
 __device__ __forceinline__ void at_lds16(uint32_t lds, const void* base, uint32_t offset) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(offset), "s"(base) : "memory");
 }
-__device__ __forceinline__ void at_landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+// the wave's tiles are in LDS (all but its last `later` loads), and its reads of earlier ones are done, so that what it loads next
+// may take their place
+template <int later = 0> __device__ __forceinline__ void at_landed() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"i"(later) : "memory"); }
 
-template <typename T, int DP> struct AtTile {
-    static constexpr int CH = DP / 8, IT = AT_TILE * CH / 256;
+template <typename T, int DP, bool NARROW> struct AtTile {
+    static constexpr int TILE = AtShape<NARROW>::TILE, WAVES = AtShape<NARROW>::WAVES, CH = DP / 8, IT = TILE * CH / (64 * WAVES);
     // rows from base on; those past the `rows` (>= 1) that there are repeat the last (they are hidden in the scores, and what lies
     // there is never read); chunks past D are left as they are
     static __device__ __forceinline__ void load(T* tile, const T* base, int sn, int rows, int D) {
-        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+        const int wave = NARROW ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
         const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)tile;
 #pragma unroll
         for (int i = 0; i < IT; ++i) {
-            const int row = (4 * i + wave) * (64 / CH) + lane / CH, chunk = (lane % CH) ^ at_swz<DP>(row);
+            const int row = (WAVES * i + wave) * (64 / CH) + lane / CH, chunk = (lane % CH) ^ at_swz<DP>(row);
             const uint32_t off = (uint32_t)min(row, rows - 1) * (uint32_t)sn * 2u + chunk * 16;
-            if (DP == D || chunk * 8 < D) at_lds16(lds + (4 * i + wave) * 1024, base, off);
+            if (DP == D || chunk * 8 < D) at_lds16(lds + (WAVES * i + wave) * 1024, base, off);
         }
     }
     // a mask that is the same for every query hides a key altogether: zeros, whatever stands there (by the lanes that loaded it)
     static __device__ __forceinline__ void hide(T* tile, const uint8_t* mask, int64_t sk, int rows) {
-        const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+        const int wave = NARROW ? 0 : threadIdx.x >> 6, lane = threadIdx.x & 63;
 #pragma unroll
         for (int i = 0; i < IT; ++i) {
-            const int row = (4 * i + wave) * (64 / CH) + lane / CH;
-            if (!mask[(int64_t)min(row, rows - 1) * sk]) *reinterpret_cast<at_u32x4*>(tile + (4 * i + wave) * 512 + lane * 8) = at_u32x4{0, 0, 0, 0};
+            const int row = (WAVES * i + wave) * (64 / CH) + lane / CH;
+            if (!mask[(int64_t)min(row, rows - 1) * sk]) *reinterpret_cast<at_u32x4*>(tile + (WAVES * i + wave) * 512 + lane * 8) = at_u32x4{0, 0, 0, 0};
         }
     }
-    // zeros in the chunks past D of `tiles` tiles, which no load touches
-    static __device__ __forceinline__ void pad(T* first, int tiles, int D) {
+    // zeros in the chunks past D of the workgroup's tiles, which no load touches
+    static __device__ __forceinline__ void pad(T* first, int bufs, int D) {
         if (D == DP) return;
-        for (int n = threadIdx.x; n < tiles * AT_TILE * CH; n += 256)
-            if (((n % CH) ^ at_swz<DP>(n / CH % AT_TILE)) * 8 >= D) *reinterpret_cast<at_u32x4*>(first + n * 8) = at_u32x4{0, 0, 0, 0};
+        for (int n = threadIdx.x; n < AtShape<NARROW>::STREAMS * 2 * bufs * TILE * CH; n += 256)
+            if (((n % CH) ^ at_swz<DP>(n / CH % TILE)) * 8 >= D) *reinterpret_cast<at_u32x4*>(first + n * 8) = at_u32x4{0, 0, 0, 0};
+        __syncthreads(); // narrow: a wave's tiles are its own from here on
     }
 };
 
@@ -175,30 +187,48 @@ __device__ __forceinline__ uint32_t at_below_bits(int k0, int lim) {
     return bits;
 }
 
-// A workgroup's LDS.  The tiles come first: the loads' 16-bit LDS base has to reach them.
-template <typename T, int DP> struct AtShared {
-    T tiles[2][2][AT_TILE * DP];
+// A workgroup's LDS.  Narrow: when the tiles are done with, their place takes the waves' partial results, 64 lanes a register.
+template <typename T, int DP, bool NARROW, int BUFS = 2> struct AtShared {
+    T tiles[AtShape<NARROW>::STREAMS][BUFS][2][AtShape<NARROW>::TILE * DP]; // stream, buffer, tensor
     int tops[4];
     float unit4[4];
+    float m[4][32], l[4][32];
 };
-template <typename T, int DP, bool MASKED> struct AtSharedKeys {
-    T tiles[2][2][AT_TILE * DP];
-    float lse[2][AT_TILE], delta[2][AT_TILE];
-    int lim[2][AT_TILE];
-    int64_t mask[MASKED ? 2 : 1][MASKED ? AT_TILE : 1];
+template <typename T, int DP, bool MASKED, bool NARROW> struct AtSharedKeys {
+    static constexpr int S = AtShape<NARROW>::STREAMS, TILE = AtShape<NARROW>::TILE;
+    T tiles[S][2][2][TILE * DP];
+    float lse[S][2][TILE], delta[S][2][TILE];
+    int lim[S][2][TILE];
+    int64_t mask[S][MASKED ? 2 : 1][MASKED ? TILE : 1];
     float unit4[4];
 };
 
+// Narrow: the sum of the four waves' `regs` values a lane; wave w gets the values w regs / 4 + 0 .. regs / 4 - 1.
+template <int REGS> __device__ __forceinline__ void at_sum_waves(const float* mine, float* room, float* sum) {
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+#pragma unroll
+    for (int r = 0; r < REGS; ++r) room[(wave * REGS + r) * 64 + lane] = mine[r];
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < REGS / 4; ++r) {
+        const float* p = room + (wave * (REGS / 4) + r) * 64 + lane;
+        sum[r] = (p[0] + p[REGS * 64]) + (p[2 * REGS * 64] + p[3 * REGS * 64]);
+    }
+}
+// The first channel of the four that accumulator values 4 n .. 4 n + 3 hold.
+__device__ __forceinline__ int at_channel(int n, int h) { return 32 * (n >> 2) + 8 * (n & 3) + 4 * h; }
+
 // ------------------------------------------------------------------------------------------------------------------- forward
-template <typename T, int DP, bool MASKED>
+template <typename T, int DP, bool MASKED, bool NARROW>
 __global__ __launch_bounds__(256, 2) void at_fwd_kernel(AttendArgs a)
 {
     typedef typename AtEl<T>::x8 x8;
     typedef typename AtEl<T>::x4 x4;
-    __shared__ __attribute__((aligned(16))) AtShared<T, DP> sh;
-    auto& smem = sh.tiles;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, c = lane & 31;
-    const int R = a.G * a.Nq, tiles = (R + AT_ROWS - 1) / AT_ROWS;
+    typedef AtTile<T, DP, NARROW> Tile;
+    constexpr int OWN = AtShape<NARROW>::OWN, TILE = AtShape<NARROW>::TILE, STREAMS = AtShape<NARROW>::STREAMS, SUBS = TILE / 32, BUFS = NARROW ? 1 : 2;
+    __shared__ __attribute__((aligned(16))) AtShared<T, DP, NARROW, BUFS> sh;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, c = lane & 31, stream = NARROW ? wave : 0;
+    const int R = a.G * a.Nq, tiles = (R + OWN - 1) / OWN;
     int id = xcd_remap(blockIdx.x, gridDim.x);
     const int tile = a.causal ? tiles - 1 - id % tiles : id % tiles; // the long rows of a causal call first
     id /= tiles;
@@ -207,15 +237,17 @@ __global__ __launch_bounds__(256, 2) void at_fwd_kernel(AttendArgs a)
     const int kh = id % a.Hk, b = id / a.Hk;
 
     const int len = a.key_lengths ? min(max(a.key_lengths[b], 0), a.Nk) : a.Nk;
-    const int row = tile * AT_ROWS + wave * 32 + c, rowc = min(row, R - 1), g = rowc / a.Nq, i = rowc - g * a.Nq;
+    const int row = tile * OWN + (NARROW ? 0 : wave * 32) + c, rowc = min(row, R - 1), g = rowc / a.Nq, i = rowc - g * a.Nq;
     const int head = kh * a.G + g;
     const int lim = row >= R ? 0 : a.causal ? min(len, max(0, i + a.Nk - a.Nq + 1)) : len; // this row sees keys below lim
     const int wave_top = at_wave_max(lim), wave_low = at_wave_min(row < R ? lim : 0x7fffffff);
-    int* const tops = sh.tops;
-    if (lane == 0) tops[wave] = wave_top;
-    __syncthreads();
-    const int top = __builtin_amdgcn_readfirstlane(max(max(tops[0], tops[1]), max(tops[2], tops[3])));
-    const int all = (top + AT_TILE - 1) / AT_TILE, per = (all + a.splits - 1) / a.splits;
+    int top = wave_top;
+    if (!NARROW) {
+        if (lane == 0) sh.tops[wave] = wave_top;
+        __syncthreads();
+        top = __builtin_amdgcn_readfirstlane(max(max(sh.tops[0], sh.tops[1]), max(sh.tops[2], sh.tops[3])));
+    }
+    const int all = (top + TILE - 1) / TILE, per = (all + a.splits - 1) / a.splits;
     const int t0 = split * per, t1 = min(all, t0 + per);
 
     const T* kb = static_cast<const T*>(a.k) + (int64_t)b * a.k_sb + (int64_t)kh * a.k_sh;
@@ -223,6 +255,13 @@ __global__ __launch_bounds__(256, 2) void at_fwd_kernel(AttendArgs a)
     const uint8_t* mrow = MASKED ? a.mask + (int64_t)b * a.m_sb + (int64_t)head * a.m_sh + (int64_t)i * a.m_sq : nullptr;
     const uint8_t* mkey = MASKED ? a.mask + (int64_t)b * a.m_sb + (int64_t)kh * a.G * a.m_sh : nullptr;
 
+    auto load_k = [&](int t, int buf) { Tile::load(sh.tiles[stream][buf][0], kb + (int64_t)t * TILE * a.k_sn, (int)a.k_sn, len - t * TILE, a.D); };
+    auto load_v = [&](int t, int buf) { Tile::load(sh.tiles[stream][buf][1], vb + (int64_t)t * TILE * a.v_sn, (int)a.v_sn, len - t * TILE, a.D); };
+    auto hide = [&](int t, T* tile) {
+        if (MASKED && a.mask_by_key) Tile::hide(tile, mkey + (int64_t)t * TILE * a.m_sk, a.m_sk, len - t * TILE);
+    };
+    Tile::pad(sh.tiles[0][0][0], BUFS, a.D);
+    if (t0 + stream < t1) { load_k(t0 + stream, 0); load_v(t0 + stream, 0); }
     x8 qf[DP / 16];
     {
         const T* qp = static_cast<const T*>(a.q) + (int64_t)b * a.q_sb + (int64_t)head * a.q_sh + (int64_t)i * a.q_sn;
@@ -232,122 +271,160 @@ __global__ __launch_bounds__(256, 2) void at_fwd_kernel(AttendArgs a)
     at_f32x16 ot[DP / 32] = {};
     float m_run = -INFINITY, l_run = 0.f; // running maximum (raw scores), this lane's share of the sum
 
-    auto load = [&](int t, int buf) {
-        AtTile<T, DP>::load(smem[buf][0], kb + (int64_t)t * AT_TILE * a.k_sn, (int)a.k_sn, len - t * AT_TILE, a.D);
-        AtTile<T, DP>::load(smem[buf][1], vb + (int64_t)t * AT_TILE * a.v_sn, (int)a.v_sn, len - t * AT_TILE, a.D);
-    };
-    AtTile<T, DP>::pad(smem[0][0], 4, a.D);
-    if (t0 < t1) load(t0, 0);
-    for (int t = t0; t < t1; ++t) {
-        const int buf = (t - t0) & 1;
-        at_landed();
-        if (MASKED && a.mask_by_key) {
-            AtTile<T, DP>::hide(smem[buf][0], mkey + (int64_t)t * AT_TILE * a.m_sk, a.m_sk, len - t * AT_TILE);
-            AtTile<T, DP>::hide(smem[buf][1], mkey + (int64_t)t * AT_TILE * a.m_sk, a.m_sk, len - t * AT_TILE);
+    int buf = 0;
+    for (int t = t0 + stream; t < t1; t += STREAMS, buf ^= BUFS - 1) {
+        T *tk = sh.tiles[stream][buf][0], *tv = sh.tiles[stream][buf][1];
+        if (NARROW) { // K is there; V's loads, the last, may still be under way
+            at_landed<Tile::IT>();
+            hide(t, tk);
+        } else {
+            at_landed();
+            hide(t, tk);
+            hide(t, tv);
+            __syncthreads(); // tile t is in place, and nobody reads the other buffer any more
+            if (t + 1 < t1) { load_k(t + 1, buf ^ 1); load_v(t + 1, buf ^ 1); }
+            if (t * TILE >= wave_top) continue;
         }
-        __syncthreads(); // tile t is in place, and nobody reads the other buffer any more
-        const T *tk = smem[buf][0], *tv = smem[buf][1];
-        if (t + 1 < t1) load(t + 1, buf ^ 1);
-        if (t * AT_TILE < wave_top) {
-            at_f32x16 st[2] = {};
+        at_f32x16 st[SUBS] = {};
 #pragma unroll
-            for (int ks = 0; ks < DP / 16; ++ks)
+        for (int ks = 0; ks < DP / 16; ++ks)
 #pragma unroll
-                for (int n = 0; n < 2; ++n) st[n] = AtEl<T>::mfma(at_rowfrag<T, DP>(tk, 32 * n, ks, lane), qf[ks], st[n]);
-            if (MASKED || (t + 1) * AT_TILE > wave_low) {
+            for (int n = 0; n < SUBS; ++n) st[n] = AtEl<T>::mfma(at_rowfrag<T, DP>(tk, 32 * n, ks, lane), qf[ks], st[n]);
+        if (MASKED || (t + 1) * TILE > wave_low) {
 #pragma unroll
-                for (int n = 0; n < 2; ++n) {
-                    const int k0 = t * AT_TILE + 32 * n + 4 * h;
-                    uint32_t see = at_below_bits(k0, lim);
-                    if (MASKED) see &= at_mask_bits(mrow, a.m_sk, k0, a.Nk - 1, a.m_sk == 1 && (t + 1) * AT_TILE <= a.Nk);
+            for (int n = 0; n < SUBS; ++n) {
+                const int k0 = t * TILE + 32 * n + 4 * h;
+                uint32_t see = at_below_bits(k0, lim);
+                if (MASKED) see &= at_mask_bits(mrow, a.m_sk, k0, a.Nk - 1, a.m_sk == 1 && (t + 1) * TILE <= a.Nk);
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) st[n][r] = (see >> r) & 1u ? st[n][r] : -INFINITY;
-                }
+                for (int r = 0; r < 16; ++r) st[n][r] = (see >> r) & 1u ? st[n][r] : -INFINITY;
             }
-            float top0 = m_run, top1 = -INFINITY;
+        }
+        if (NARROW) { // one buffer: K's next tile as soon as this one is read, V's at the end; half the LDS, so twice the waves
+            at_landed();
+            if (t + STREAMS < t1) load_k(t + STREAMS, 0);
+            hide(t, tv);
+        }
+        float tops[SUBS];
 #pragma unroll
-            for (int r = 0; r < 16; r += 2) {
-                top0 = at_max3(top0, st[0][r], st[0][r + 1]);
-                top1 = at_max3(top1, st[1][r], st[1][r + 1]);
+        for (int n = 0; n < SUBS; ++n) {
+            tops[n] = n ? -INFINITY : m_run;
+#pragma unroll
+            for (int r = 0; r < 16; r += 2) tops[n] = at_max3(tops[n], st[n][r], st[n][r + 1]);
+        }
+        const float most = SUBS > 1 ? fmaxf(tops[0], tops[SUBS - 1]) : tops[0];
+        const float m_new = fmaxf(most, at_other_half(most));
+        const float m_use = m_new == -INFINITY ? 0.f : m_new, neg_m = -m_use * a.scale_log2e;
+        if (__builtin_amdgcn_ballot_w64(m_new > m_run) != 0ull) { // no row's maximum rose: the factor is 1
+            const float alpha = __builtin_amdgcn_exp2f((m_run - m_use) * a.scale_log2e);
+            l_run *= alpha;
+#pragma unroll
+            for (int db = 0; db < DP / 32; ++db) ot[db] *= alpha;
+        }
+        m_run = m_new;
+        float ps[4] = {0.f, 0.f, 0.f, 0.f};
+        x8 pf[SUBS][2];
+#pragma unroll
+        for (int n = 0; n < SUBS; ++n)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const float p = __builtin_amdgcn_exp2f(fmaf(st[n][r], a.scale_log2e, neg_m));
+                ps[r & 3] += p;
+                pf[n][r >> 3][r & 7] = (T)p; // rounded to the operands' type for the second product; the sum keeps 32 bits
             }
-            top0 = fmaxf(top0, top1);
-            const float m_new = fmaxf(top0, at_other_half(top0));
-            const float m_use = m_new == -INFINITY ? 0.f : m_new, neg_m = -m_use * a.scale_log2e;
-            if (__builtin_amdgcn_ballot_w64(m_new > m_run) != 0ull) { // no row's maximum rose: the factor is 1
-                const float alpha = __builtin_amdgcn_exp2f((m_run - m_use) * a.scale_log2e);
-                l_run *= alpha;
+        l_run += (ps[0] + ps[1]) + (ps[2] + ps[3]);
 #pragma unroll
-                for (int db = 0; db < DP / 32; ++db) ot[db] *= alpha;
-            }
-            m_run = m_new;
-            float ps[4] = {0.f, 0.f, 0.f, 0.f};
-            x8 pf[2][2];
+        for (int n = 0; n < SUBS; ++n)
 #pragma unroll
-            for (int n = 0; n < 2; ++n)
+            for (int s = 0; s < 2; ++s)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const float p = __builtin_amdgcn_exp2f(fmaf(st[n][r], a.scale_log2e, neg_m));
-                    ps[r & 3] += p;
-                    pf[n][r >> 3][r & 7] = (T)p; // rounded to the operands' type for the second product; the sum keeps 32 bits
-                }
-            l_run += (ps[0] + ps[1]) + (ps[2] + ps[3]);
-#pragma unroll
-            for (int n = 0; n < 2; ++n)
-#pragma unroll
-                for (int s = 0; s < 2; ++s)
-#pragma unroll
-                    for (int db = 0; db < DP / 32; ++db) ot[db] = AtEl<T>::mfma(at_colfrag<T, DP>(tv, 32 * n + 16 * s, db, lane), pf[n][s], ot[db]);
+                for (int db = 0; db < DP / 32; ++db) ot[db] = AtEl<T>::mfma(at_colfrag<T, DP>(tv, 32 * n + 16 * s, db, lane), pf[n][s], ot[db]);
+        if (NARROW && t + STREAMS < t1) {
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            load_v(t + STREAMS, 0);
         }
     }
 
-    const float l = l_run + at_other_half(l_run);
-    if (row >= R) return;
+    float l = l_run + at_other_half(l_run), m = m_run;
     const int64_t at = ((int64_t)b * a.Hk + kh) * R + row; // = (b H + head) Nq + i
-    if (a.splits > 1) {
-        const int64_t slot = (int64_t)split * a.B * a.Hk * R + at;
-        if (h == 0) { a.part_ml[2 * slot] = m_run; a.part_ml[2 * slot + 1] = l; }
+    const int64_t slot = (int64_t)split * a.B * a.Hk * R + at;
+    auto statistics = [&]() {
+        if (a.splits > 1) { a.part_ml[2 * slot] = m; a.part_ml[2 * slot + 1] = l; }
+        else a.lse[at] = l == 0.f ? -INFINITY : m * a.scale + logf(l);
+    };
+    auto store = [&](int n, const float* o, float inv) { // four values, n as at_channel's
+        const int d = at_channel(n, h);
+        if (d >= a.D) return;
+        if (a.splits > 1) { *reinterpret_cast<at_f32x4*>(a.part_o + slot * a.D + d) = at_f32x4{o[0], o[1], o[2], o[3]}; return; }
+        x4 y;
 #pragma unroll
-        for (int db = 0; db < DP / 32; ++db)
+        for (int e = 0; e < 4; ++e) y[e] = (T)(o[e] * inv);
+        *reinterpret_cast<x4*>(static_cast<T*>(a.out) + (((int64_t)b * a.Nq + i) * a.H + head) * a.D + d) = y;
+    };
+    float flat[DP / 2];
 #pragma unroll
-            for (int r = 0; r < 16; r += 4) {
-                const int d = 32 * db + 2 * r + 4 * h;
-                if (d < a.D) *reinterpret_cast<at_f32x4*>(a.part_o + slot * a.D + d) = at_f32x4{ot[db][r], ot[db][r + 1], ot[db][r + 2], ot[db][r + 3]};
-            }
+    for (int r = 0; r < DP / 2; ++r) flat[r] = ot[r >> 4][r & 15];
+    if (NARROW) {
+        if (h == 0) { sh.m[wave][c] = m; sh.l[wave][c] = l; }
+        __syncthreads(); // and every wave is done with its tiles
+        const float m_own = m;
+        m = fmaxf(fmaxf(sh.m[0][c], sh.m[1][c]), fmaxf(sh.m[2][c], sh.m[3][c]));
+        const float m_use = m == -INFINITY ? 0.f : m;
+        l = 0.f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) l += sh.l[w][c] * __builtin_amdgcn_exp2f((sh.m[w][c] - m_use) * a.scale_log2e);
+        const float weight = __builtin_amdgcn_exp2f((m_own - m_use) * a.scale_log2e);
+#pragma unroll
+        for (int r = 0; r < DP / 2; ++r) flat[r] *= weight;
+        float sum[DP / 8];
+        at_sum_waves<DP / 2>(flat, reinterpret_cast<float*>(sh.tiles), sum);
+        if (row >= R) return;
+        if (wave == 0 && h == 0) statistics();
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+        for (int n = 0; n < DP / 32; ++n) store(wave * (DP / 32) + n, sum + 4 * n, inv);
         return;
     }
+    if (row >= R) return;
+    if (h == 0) statistics();
     const float inv = l == 0.f ? 0.f : 1.f / l;
-    if (h == 0) a.lse[at] = l == 0.f ? -INFINITY : m_run * a.scale + logf(l);
-    T* op = static_cast<T*>(a.out) + (((int64_t)b * a.Nq + i) * a.H + head) * a.D;
 #pragma unroll
-    for (int db = 0; db < DP / 32; ++db)
-#pragma unroll
-        for (int r = 0; r < 16; r += 4) {
-            const int d = 32 * db + 2 * r + 4 * h;
-            x4 o;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[e] = (T)(ot[db][r + e] * inv);
-            if (d < a.D) *reinterpret_cast<x4*>(op + d) = o;
-        }
+    for (int n = 0; n < DP / 8; ++n) store(n, flat + 4 * n, inv);
 }
 
-// Joins the parts of a row that several workgroups computed: 32 lanes a row, 4 elements a lane.
+// Joins the parts of a row that several workgroups computed: 32 lanes a row, 4 elements a lane; lane s brings the statistics of parts s and s + 32.
 template <typename T>
 __global__ __launch_bounds__(256) void at_join_kernel(AttendArgs a)
 {
     typedef typename AtEl<T>::x4 x4;
-    const int64_t rows = (int64_t)a.B * a.H * a.Nq, at = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-    if (at >= rows) return;
-    const int d = (threadIdx.x & 31) * 4;
-    float m = -INFINITY;
-    for (int s = 0; s < a.splits; ++s) m = fmaxf(m, a.part_ml[2 * (s * rows + at)]);
-    const float m_use = m == -INFINITY ? 0.f : m;
-    float l = 0.f;
-    at_f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < a.splits; ++s) {
-        const float w = __builtin_amdgcn_exp2f((a.part_ml[2 * (s * rows + at)] - m_use) * a.scale_log2e);
-        l += w * a.part_ml[2 * (s * rows + at) + 1];
-        if (d < a.D) o += w * *reinterpret_cast<const at_f32x4*>(a.part_o + (s * rows + at) * a.D + d);
+    const int64_t rows = (int64_t)a.B * a.H * a.Nq, at = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5), atc = at < rows ? at : rows - 1;
+    const int s32 = threadIdx.x & 31, d = s32 * 4;
+    float ms[2], ls[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const int s = s32 + 32 * k;
+        ms[k] = s < a.splits ? a.part_ml[2 * (s * rows + atc)] : -INFINITY;
+        ls[k] = s < a.splits ? a.part_ml[2 * (s * rows + atc) + 1] : 0.f;
     }
+    float m = fmaxf(ms[0], ms[1]);
+    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+    const float m_use = m == -INFINITY ? 0.f : m;
+    const float w0 = __builtin_amdgcn_exp2f((ms[0] - m_use) * a.scale_log2e), w1 = __builtin_amdgcn_exp2f((ms[1] - m_use) * a.scale_log2e);
+    float l = ls[0] * w0 + ls[1] * w1;
+    for (int o = 16; o; o >>= 1) l += __shfl_xor(l, o);
+    at_f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    const float* p = a.part_o + atc * a.D + (d < a.D ? d : 0);
+    for (int s0 = 0; s0 < a.splits; s0 += 4) { // four parts' loads under way at a time; a part past the last weighs 0
+        at_f32x4 x[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x[k] = *reinterpret_cast<const at_f32x4*>(p + min(s0 + k, a.splits - 1) * rows * a.D);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const float w = __shfl(s0 < 32 ? w0 : w1, (s0 + k) & 31, 32);
+            if (s0 + k < a.splits) o += w * x[k];
+        }
+    }
+    if (at >= rows) return;
     const float inv = l == 0.f ? 0.f : 1.f / l;
     if (d == 0) a.lse[at] = l == 0.f ? -INFINITY : m * a.scale + logf(l);
     if (d >= a.D) return;
@@ -405,35 +482,42 @@ template <typename T> __device__ __forceinline__ float at_grad_unit(const Attend
 }
 
 // dQ: a wave owns 32 rows and walks the keys that they see.
-template <typename T, int DP, bool MASKED>
-__global__ __launch_bounds__(256, 2) void at_bwd_rows_kernel(AttendArgs a)
+template <typename T, int DP, bool MASKED, bool NARROW> __device__ __forceinline__ void at_bwd_rows(const AttendArgs& a, AtShared<T, DP, NARROW>& sh, int id)
 {
     typedef typename AtEl<T>::x8 x8;
     typedef typename AtEl<T>::x4 x4;
-    __shared__ __attribute__((aligned(16))) AtShared<T, DP> sh;
-    auto& smem = sh.tiles;
-    int* const tops = sh.tops;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, c = lane & 31;
-    const int R = a.G * a.Nq, tiles = (R + AT_ROWS - 1) / AT_ROWS;
-    int id = xcd_remap(blockIdx.x, gridDim.x);
+    typedef AtTile<T, DP, NARROW> Tile;
+    constexpr int OWN = AtShape<NARROW>::OWN, TILE = AtShape<NARROW>::TILE, STREAMS = AtShape<NARROW>::STREAMS, SUBS = TILE / 32;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, c = lane & 31, stream = NARROW ? wave : 0;
+    const int R = a.G * a.Nq, tiles = (R + OWN - 1) / OWN;
     const int tile = a.causal ? tiles - 1 - id % tiles : id % tiles;
     id /= tiles;
     const int kh = id % a.Hk, b = id / a.Hk;
     const float unit = at_grad_unit<T>(a, b, kh, sh.unit4);
 
     const int len = a.key_lengths ? min(max(a.key_lengths[b], 0), a.Nk) : a.Nk;
-    const int row = tile * AT_ROWS + wave * 32 + c, rowc = min(row, R - 1), g = rowc / a.Nq, i = rowc - g * a.Nq;
+    const int row = tile * OWN + (NARROW ? 0 : wave * 32) + c, rowc = min(row, R - 1), g = rowc / a.Nq, i = rowc - g * a.Nq;
     const int head = kh * a.G + g;
     const int lim = row >= R ? 0 : a.causal ? min(len, max(0, i + a.Nk - a.Nq + 1)) : len;
     const int wave_top = at_wave_max(lim), wave_low = at_wave_min(row < R ? lim : 0x7fffffff);
-    if (lane == 0) tops[wave] = wave_top;
-    __syncthreads();
-    const int t1 = (__builtin_amdgcn_readfirstlane(max(max(tops[0], tops[1]), max(tops[2], tops[3]))) + AT_TILE - 1) / AT_TILE;
+    int top = wave_top;
+    if (!NARROW) {
+        if (lane == 0) sh.tops[wave] = wave_top;
+        __syncthreads();
+        top = __builtin_amdgcn_readfirstlane(max(max(sh.tops[0], sh.tops[1]), max(sh.tops[2], sh.tops[3])));
+    }
+    const int t1 = (top + TILE - 1) / TILE;
 
     const T* kb = static_cast<const T*>(a.k) + (int64_t)b * a.k_sb + (int64_t)kh * a.k_sh;
     const T* vb = static_cast<const T*>(a.v) + (int64_t)b * a.v_sb + (int64_t)kh * a.v_sh;
     const uint8_t* mrow = MASKED ? a.mask + (int64_t)b * a.m_sb + (int64_t)head * a.m_sh + (int64_t)i * a.m_sq : nullptr;
     const uint8_t* mkey = MASKED ? a.mask + (int64_t)b * a.m_sb + (int64_t)kh * a.G * a.m_sh : nullptr;
+    auto load = [&](int t, int buf) {
+        Tile::load(sh.tiles[stream][buf][0], kb + (int64_t)t * TILE * a.k_sn, (int)a.k_sn, len - t * TILE, a.D);
+        Tile::load(sh.tiles[stream][buf][1], vb + (int64_t)t * TILE * a.v_sn, (int)a.v_sn, len - t * TILE, a.D);
+    };
+    Tile::pad(sh.tiles[0][0][0], 2, a.D);
+    if (stream < t1) load(stream, 0);
     x8 qf[DP / 16], gf[DP / 16];
     {
         const T* qp = static_cast<const T*>(a.q) + (int64_t)b * a.q_sb + (int64_t)head * a.q_sh + (int64_t)i * a.q_sn;
@@ -445,149 +529,157 @@ __global__ __launch_bounds__(256, 2) void at_bwd_rows_kernel(AttendArgs a)
     const float lse = a.lse[at], neg_lse = lse == -INFINITY ? -INFINITY : -lse * 1.4426950408889634f, neg_delta = -a.delta[at] * unit;
     at_f32x16 acc[DP / 32] = {};
 
-    auto load = [&](int t, int buf) {
-        AtTile<T, DP>::load(smem[buf][0], kb + (int64_t)t * AT_TILE * a.k_sn, (int)a.k_sn, len - t * AT_TILE, a.D);
-        AtTile<T, DP>::load(smem[buf][1], vb + (int64_t)t * AT_TILE * a.v_sn, (int)a.v_sn, len - t * AT_TILE, a.D);
-    };
-    AtTile<T, DP>::pad(smem[0][0], 4, a.D);
-    if (t1 > 0) load(0, 0);
-    for (int t = 0; t < t1; ++t) {
-        const int buf = t & 1;
+    int buf = 0;
+    for (int t = stream; t < t1; t += STREAMS, buf ^= 1) {
+        T *tk = sh.tiles[stream][buf][0], *tv = sh.tiles[stream][buf][1];
         at_landed();
         if (MASKED && a.mask_by_key) {
-            AtTile<T, DP>::hide(smem[buf][0], mkey + (int64_t)t * AT_TILE * a.m_sk, a.m_sk, len - t * AT_TILE);
-            AtTile<T, DP>::hide(smem[buf][1], mkey + (int64_t)t * AT_TILE * a.m_sk, a.m_sk, len - t * AT_TILE);
+            Tile::hide(tk, mkey + (int64_t)t * TILE * a.m_sk, a.m_sk, len - t * TILE);
+            Tile::hide(tv, mkey + (int64_t)t * TILE * a.m_sk, a.m_sk, len - t * TILE);
         }
-        __syncthreads(); // tile t is in place, and nobody reads the other buffer any more
-        const T *tk = smem[buf][0], *tv = smem[buf][1];
-        if (t + 1 < t1) load(t + 1, buf ^ 1);
-        if (t * AT_TILE < wave_top) {
-            at_f32x16 st[2] = {}, dp[2] = {};
+        if (!NARROW) __syncthreads();
+        if (t + STREAMS < t1) load(t + STREAMS, buf ^ 1);
+        if (t * TILE >= wave_top) continue;
+        at_f32x16 st[SUBS] = {}, dp[SUBS] = {};
 #pragma unroll
-            for (int ks = 0; ks < DP / 16; ++ks)
+        for (int ks = 0; ks < DP / 16; ++ks)
 #pragma unroll
-                for (int n = 0; n < 2; ++n) {
-                    st[n] = AtEl<T>::mfma(at_rowfrag<T, DP>(tk, 32 * n, ks, lane), qf[ks], st[n]);
-                    dp[n] = AtEl<T>::mfma(at_rowfrag<T, DP>(tv, 32 * n, ks, lane), gf[ks], dp[n]);
-                }
-            if (MASKED || (t + 1) * AT_TILE > wave_low) {
-#pragma unroll
-                for (int n = 0; n < 2; ++n) {
-                    const int k0 = t * AT_TILE + 32 * n + 4 * h;
-                    uint32_t see = at_below_bits(k0, lim);
-                    if (MASKED) see &= at_mask_bits(mrow, a.m_sk, k0, a.Nk - 1, a.m_sk == 1 && (t + 1) * AT_TILE <= a.Nk);
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) st[n][r] = (see >> r) & 1u ? st[n][r] : -INFINITY;
-                }
+            for (int n = 0; n < SUBS; ++n) {
+                st[n] = AtEl<T>::mfma(at_rowfrag<T, DP>(tk, 32 * n, ks, lane), qf[ks], st[n]);
+                dp[n] = AtEl<T>::mfma(at_rowfrag<T, DP>(tv, 32 * n, ks, lane), gf[ks], dp[n]);
             }
-            x8 ds[2][2];
+        if (MASKED || (t + 1) * TILE > wave_low) {
 #pragma unroll
-            for (int n = 0; n < 2; ++n)
+            for (int n = 0; n < SUBS; ++n) {
+                const int k0 = t * TILE + 32 * n + 4 * h;
+                uint32_t see = at_below_bits(k0, lim);
+                if (MASKED) see &= at_mask_bits(mrow, a.m_sk, k0, a.Nk - 1, a.m_sk == 1 && (t + 1) * TILE <= a.Nk);
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const float p = __builtin_amdgcn_exp2f(fmaf(st[n][r], a.scale_log2e, neg_lse));
-                    ds[n][r >> 3][r & 7] = (T)(p * fmaf(dp[n][r], unit, neg_delta));
-                }
-#pragma unroll
-            for (int n = 0; n < 2; ++n)
-#pragma unroll
-                for (int s = 0; s < 2; ++s)
-#pragma unroll
-                    for (int db = 0; db < DP / 32; ++db) acc[db] = AtEl<T>::mfma(at_colfrag<T, DP>(tk, 32 * n + 16 * s, db, lane), ds[n][s], acc[db]);
+                for (int r = 0; r < 16; ++r) st[n][r] = (see >> r) & 1u ? st[n][r] : -INFINITY;
+            }
         }
+        x8 ds[SUBS][2];
+#pragma unroll
+        for (int n = 0; n < SUBS; ++n)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const float p = __builtin_amdgcn_exp2f(fmaf(st[n][r], a.scale_log2e, neg_lse));
+                ds[n][r >> 3][r & 7] = (T)(p * fmaf(dp[n][r], unit, neg_delta));
+            }
+#pragma unroll
+        for (int n = 0; n < SUBS; ++n)
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int db = 0; db < DP / 32; ++db) acc[db] = AtEl<T>::mfma(at_colfrag<T, DP>(tk, 32 * n + 16 * s, db, lane), ds[n][s], acc[db]);
+    }
+    const float f = a.scale / unit;
+    const bool blind = lse == -INFINITY; // sees nothing: a gradient of zero whatever the (unread) products gave
+    auto store = [&](int n, const float* o) {
+        const int d = at_channel(n, h);
+        x4 y;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = blind ? (T)0.f : (T)(o[e] * f);
+        if (d < a.D) *reinterpret_cast<x4*>(static_cast<T*>(a.dq) + (int64_t)b * a.dq_sb + (int64_t)head * a.dq_sh + (int64_t)i * a.dq_sn + d) = y;
+    };
+    float flat[DP / 2];
+#pragma unroll
+    for (int r = 0; r < DP / 2; ++r) flat[r] = acc[r >> 4][r & 15];
+    if (NARROW) {
+        float sum[DP / 8];
+        __syncthreads(); // every wave is done with its tiles
+        at_sum_waves<DP / 2>(flat, reinterpret_cast<float*>(sh.tiles), sum);
+        if (row >= R) return;
+#pragma unroll
+        for (int n = 0; n < DP / 32; ++n) store(wave * (DP / 32) + n, sum + 4 * n);
+        return;
     }
     if (row >= R) return;
-    const float f = a.scale / unit;
-    T* op = static_cast<T*>(a.dq) + (int64_t)b * a.dq_sb + (int64_t)head * a.dq_sh + (int64_t)i * a.dq_sn;
-    const bool blind = lse == -INFINITY; // sees nothing: a gradient of zero whatever the (unread) products gave
 #pragma unroll
-    for (int db = 0; db < DP / 32; ++db)
-#pragma unroll
-        for (int r = 0; r < 16; r += 4) {
-            const int d = 32 * db + 2 * r + 4 * h;
-            x4 o;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[e] = blind ? (T)0.f : (T)(acc[db][r + e] * f);
-            if (d < a.D) *reinterpret_cast<x4*>(op + d) = o;
-        }
+    for (int n = 0; n < DP / 8; ++n) store(n, flat + 4 * n);
 }
 
 // dK, dV: a wave owns 32 keys and walks the rows that may see them.
-template <typename T, int DP, bool MASKED>
-__global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void at_bwd_keys_kernel(AttendArgs a)
+template <typename T, int DP, bool MASKED, bool NARROW> __device__ __forceinline__ void at_bwd_keys(const AttendArgs& a, AtSharedKeys<T, DP, MASKED, NARROW>& sh, int id)
 {
     typedef typename AtEl<T>::x8 x8;
     typedef typename AtEl<T>::x4 x4;
-    __shared__ __attribute__((aligned(16))) AtSharedKeys<T, DP, MASKED> sh;
-    auto& smem = sh.tiles;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, c = lane & 31;
-    const int R = a.G * a.Nq, tiles = (a.Nk + AT_ROWS - 1) / AT_ROWS, off = a.Nk - a.Nq;
-    int id = xcd_remap(blockIdx.x, gridDim.x);
+    typedef AtTile<T, DP, NARROW> Tile;
+    constexpr int OWN = AtShape<NARROW>::OWN, TILE = AtShape<NARROW>::TILE, STREAMS = AtShape<NARROW>::STREAMS, SUBS = TILE / 32;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, c = lane & 31, stream = NARROW ? wave : 0;
+    const int R = a.G * a.Nq, tiles = (a.Nk + OWN - 1) / OWN, off = a.Nk - a.Nq;
     const int tile = id % tiles; // causal: the first keys are seen by most rows, the long ones come first as they are
     id /= tiles;
     const int kh = id % a.Hk, b = id / a.Hk;
     const float unit = at_grad_unit<T>(a, b, kh, sh.unit4);
     const int len = a.key_lengths ? min(max(a.key_lengths[b], 0), a.Nk) : a.Nk;
-    const int k0 = tile * AT_ROWS, wave_k0 = k0 + __builtin_amdgcn_readfirstlane(wave) * 32, key = wave_k0 + c;
+    const int k0 = tile * OWN, wave_k0 = k0 + (NARROW ? 0 : wave * 32), key = wave_k0 + c;
 
     at_f32x16 dk[DP / 32] = {}, dv[DP / 32] = {};
     if (k0 < len) {
-        x8 kf[DP / 16], vf[DP / 16];
         const int keyc = min(key, len - 1);
+        const T* qb = static_cast<const T*>(a.q) + (int64_t)b * a.q_sb + (int64_t)kh * a.G * a.q_sh;
+        const T* gb = static_cast<const T*>(a.dout) + (int64_t)b * a.g_sb + (int64_t)kh * a.G * a.g_sh;
+        const int64_t at0 = ((int64_t)b * a.Hk + kh) * R;
+        const uint8_t* mkey = MASKED ? a.mask + (int64_t)b * a.m_sb + (int64_t)kh * a.G * a.m_sh + (int64_t)keyc * a.m_sk : nullptr;
+        // the tiles: head by head, from the first query that sees a key of this workgroup
+        const int i_first = a.causal ? max(0, k0 - off) : 0, per_head = a.Nq > i_first ? (a.Nq - i_first + TILE - 1) / TILE : 0, t1 = a.G * per_head;
+        const int slot = threadIdx.x & (TILE - 1);                       // the row whose numbers this thread brings
+        const bool brings = NARROW ? lane < TILE : threadIdx.x < TILE;
+        float n_lse = 0.f, n_delta = 0.f;
+        int n_lim = -1;
+        int64_t n_mask = 0;
+        int g_next = 0, j_next = stream; // the next tile: head and number in it
+        while (j_next >= per_head && g_next < a.G) { j_next -= per_head; ++g_next; }
+        auto load = [&](int buf) { // returns the first row of the tile
+            const int g = g_next, i0 = i_first + j_next * TILE;
+            j_next += STREAMS;
+            while (j_next >= per_head) { j_next -= per_head; ++g_next; }
+            Tile::load(sh.tiles[stream][buf][0], qb + (int64_t)g * a.q_sh + (int64_t)i0 * a.q_sn, (int)a.q_sn, a.Nq - i0, a.D);
+            Tile::load(sh.tiles[stream][buf][1], gb + (int64_t)g * a.g_sh + (int64_t)i0 * a.g_sn, (int)a.g_sn, a.Nq - i0, a.D);
+            if (brings) {
+                const int i = i0 + slot, ic = min(i, a.Nq - 1);
+                const int64_t at = at0 + (int64_t)g * a.Nq + ic;
+                n_lse = a.lse[at]; // as they are: worked on in note(), when they have long arrived
+                n_delta = a.delta[at];
+                n_lim = i >= a.Nq ? -1 : a.causal ? min(len - 1, i + off) : len - 1; // the last key that the row sees
+                if (MASKED) n_mask = (int64_t)g * a.m_sh + (int64_t)ic * a.m_sq;
+            }
+            return i0;
+        };
+        auto note = [&](int buf) {
+            if (brings) {
+                sh.lse[stream][buf][slot] = n_lse == -INFINITY ? -INFINITY : -n_lse * 1.4426950408889634f;
+                sh.delta[stream][buf][slot] = -n_delta * unit;
+                sh.lim[stream][buf][slot] = n_lim;
+                if (MASKED) sh.mask[stream][buf][slot] = n_mask;
+            }
+        };
+        Tile::pad(sh.tiles[0][0][0], 2, a.D);
+        int i0 = 0, i0_next = 0;
+        if (stream < t1) { i0_next = load(0); note(0); }
+        x8 kf[DP / 16], vf[DP / 16];
         {
             const T* kp = static_cast<const T*>(a.k) + (int64_t)b * a.k_sb + (int64_t)kh * a.k_sh + (int64_t)keyc * a.k_sn;
             const T* vp = static_cast<const T*>(a.v) + (int64_t)b * a.v_sb + (int64_t)kh * a.v_sh + (int64_t)keyc * a.v_sn;
 #pragma unroll
             for (int ks = 0; ks < DP / 16; ++ks) { kf[ks] = at_global_frag<T>(kp, ks, lane, a.D); vf[ks] = at_global_frag<T>(vp, ks, lane, a.D); }
         }
-        const T* qb = static_cast<const T*>(a.q) + (int64_t)b * a.q_sb + (int64_t)kh * a.G * a.q_sh;
-        const T* gb = static_cast<const T*>(a.dout) + (int64_t)b * a.g_sb + (int64_t)kh * a.G * a.g_sh;
-        const int64_t at0 = ((int64_t)b * a.Hk + kh) * R;
-        const uint8_t* mkey = MASKED ? a.mask + (int64_t)b * a.m_sb + (int64_t)kh * a.G * a.m_sh + (int64_t)keyc * a.m_sk : nullptr;
         if (MASKED && a.mask_by_key && !mkey[0]) {
 #pragma unroll
             for (int ks = 0; ks < DP / 16; ++ks) { kf[ks] = x8{}; vf[ks] = x8{}; }
         }
-        // the tiles: head by head, from the first query that sees a key of this workgroup
-        const int i_first = a.causal ? max(0, k0 - off) : 0, per_head = a.Nq > i_first ? (a.Nq - i_first + AT_TILE - 1) / AT_TILE : 0, t1 = a.G * per_head;
-        int g_next = 0, i_next = i_first;
-        float n_lse = 0.f, n_delta = 0.f;
-        int n_lim = -1;
-        int64_t n_mask = 0;
-        auto load = [&](int buf) { // tile (g_next, i_next)
-            AtTile<T, DP>::load(smem[buf][0], qb + (int64_t)g_next * a.q_sh + (int64_t)i_next * a.q_sn, (int)a.q_sn, a.Nq - i_next, a.D);
-            AtTile<T, DP>::load(smem[buf][1], gb + (int64_t)g_next * a.g_sh + (int64_t)i_next * a.g_sn, (int)a.g_sn, a.Nq - i_next, a.D);
-            if (threadIdx.x < AT_TILE) {
-                const int i = i_next + threadIdx.x, ic = min(i, a.Nq - 1);
-                const int64_t at = at0 + (int64_t)g_next * a.Nq + ic;
-                n_lse = a.lse[at]; // as they are: worked on in note(), when they have long arrived
-                n_delta = a.delta[at];
-                n_lim = i >= a.Nq ? -1 : a.causal ? min(len - 1, i + off) : len - 1; // the last key that the row sees
-                if (MASKED) n_mask = (int64_t)g_next * a.m_sh + (int64_t)ic * a.m_sq;
-            }
-        };
-        auto note = [&](int buf) {
-            if (threadIdx.x < AT_TILE) {
-                sh.lse[buf][threadIdx.x] = n_lse == -INFINITY ? -INFINITY : -n_lse * 1.4426950408889634f;
-                sh.delta[buf][threadIdx.x] = -n_delta * unit;
-                sh.lim[buf][threadIdx.x] = n_lim;
-                if (MASKED) sh.mask[buf][threadIdx.x] = n_mask;
-            }
-        };
-        AtTile<T, DP>::pad(smem[0][0], 4, a.D);
-        if (t1 > 0) { load(0); note(0); }
-        for (int t = 0; t < t1; ++t) {
-            const int buf = t & 1, i0 = i_next;
-            i_next += AT_TILE;
-            if (i_next >= a.Nq) { i_next = i_first; ++g_next; }
+        int buf = 0;
+        for (int t = stream; t < t1; t += STREAMS, buf ^= 1) {
+            const T *tq = sh.tiles[stream][buf][0], *tg = sh.tiles[stream][buf][1];
             at_landed();
-            __syncthreads();
-            const T *tq = smem[buf][0], *tg = smem[buf][1];
-            if (t + 1 < t1) load(buf ^ 1);
+            if (!NARROW) __syncthreads();
+            i0 = i0_next;
+            if (t + STREAMS < t1) i0_next = load(buf ^ 1);
             // unless every row of the tile sees every key of the wave
-            const bool edge = MASKED || i0 + AT_TILE > a.Nq || wave_k0 + 32 > len || (a.causal && i0 + off < wave_k0 + 31);
-            at_f32x16 st[2] = {}, dp[2] = {};
-            x8 pf[2][2], df[2][2], gt[2][DP / 32], qt[2][DP / 32];
+            const bool edge = MASKED || i0 + TILE > a.Nq || wave_k0 + 32 > len || (a.causal && i0 + off < wave_k0 + 31);
+            at_f32x16 st[SUBS] = {}, dp[SUBS] = {};
+            x8 pf[SUBS][2], df[SUBS][2], gt[2][DP / 32], qt[2][DP / 32];
             auto scores = [&](int n) {
                 x8 qa[DP / 16], ga[DP / 16];
 #pragma unroll
@@ -603,8 +695,8 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void at_bwd_keys_kernel(Atte
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
                     const int q = 32 * n + 8 * (r >> 2) + 4 * h + (r & 3);
-                    bool on = key <= sh.lim[buf][q];
-                    if (MASKED) on = on & (mkey[sh.mask[buf][q]] != 0);
+                    bool on = key <= sh.lim[stream][buf][q];
+                    if (MASKED) on = on & (mkey[sh.mask[stream][buf][q]] != 0);
                     st[n][r] = on ? st[n][r] : -INFINITY;
                 }
             };
@@ -612,7 +704,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void at_bwd_keys_kernel(Atte
 #pragma unroll
                 for (int r4 = 0; r4 < 4; ++r4) {
                     const int q0 = 32 * n + 8 * r4 + 4 * h;
-                    const at_f32x4 nl = *reinterpret_cast<const at_f32x4*>(&sh.lse[buf][q0]), nd = *reinterpret_cast<const at_f32x4*>(&sh.delta[buf][q0]);
+                    const at_f32x4 nl = *reinterpret_cast<const at_f32x4*>(&sh.lse[stream][buf][q0]), nd = *reinterpret_cast<const at_f32x4*>(&sh.delta[stream][buf][q0]);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const int r = 4 * r4 + e;
@@ -640,7 +732,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void at_bwd_keys_kernel(Atte
                         dk[db] = AtEl<T>::mfma(qt[s][db], df[n][s], dk[db]);
                     }
             };
-            if (DP == 128) {
+            if constexpr (DP == 128 && SUBS == 2) {
                 // 128 accumulators and 64 registers of K and V leave one wave a SIMD, whose own products have to cover its arithmetic:
                 // the scores of the second 32 rows run while the probabilities of the first are worked out, and so on.  4096 tokens x
                 // 16 heads: 594 -> 520 us for the whole backward pass against one step after the other.
@@ -659,7 +751,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void at_bwd_keys_kernel(Atte
                 gradients(1);
             } else { // three waves a SIMD cover each other; the order above costs registers and one of them (1070 -> 1258 us at 8192 x 16)
 #pragma unroll
-                for (int n = 0; n < 2; ++n) {
+                for (int n = 0; n < SUBS; ++n) {
                     scores(n);
                     if (edge) hide(n);
                     probs(n);
@@ -667,32 +759,70 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void at_bwd_keys_kernel(Atte
                     gradients(n);
                 }
             }
-            if (t + 1 < t1) note(buf ^ 1);
+            if (t + STREAMS < t1) note(buf ^ 1);
         }
     }
-    if (key >= a.Nk) return;
     const float f = a.scale / unit;
-    T* kp = static_cast<T*>(a.dk) + (int64_t)b * a.dk_sb + (int64_t)kh * a.dk_sh + (int64_t)key * a.dk_sn;
-    T* vp = static_cast<T*>(a.dv) + (int64_t)b * a.dv_sb + (int64_t)kh * a.dv_sh + (int64_t)key * a.dv_sn;
+    auto store = [&](int n, const float* x, const float* y) {
+        const int d = at_channel(n, h);
+        x4 k4, v4;
 #pragma unroll
-    for (int db = 0; db < DP / 32; ++db)
-#pragma unroll
-        for (int r = 0; r < 16; r += 4) {
-            const int d = 32 * db + 2 * r + 4 * h;
-            x4 x, y;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) { x[e] = (T)(dk[db][r + e] * f); y[e] = (T)dv[db][r + e]; }
-            if (d < a.D) { *reinterpret_cast<x4*>(kp + d) = x; *reinterpret_cast<x4*>(vp + d) = y; }
+        for (int e = 0; e < 4; ++e) { k4[e] = (T)(x[e] * f); v4[e] = (T)y[e]; }
+        if (d < a.D) {
+            *reinterpret_cast<x4*>(static_cast<T*>(a.dk) + (int64_t)b * a.dk_sb + (int64_t)kh * a.dk_sh + (int64_t)key * a.dk_sn + d) = k4;
+            *reinterpret_cast<x4*>(static_cast<T*>(a.dv) + (int64_t)b * a.dv_sb + (int64_t)kh * a.dv_sh + (int64_t)key * a.dv_sn + d) = v4;
         }
+    };
+    float fk[DP / 2], fv[DP / 2];
+#pragma unroll
+    for (int r = 0; r < DP / 2; ++r) { fk[r] = dk[r >> 4][r & 15]; fv[r] = dv[r >> 4][r & 15]; }
+    if (NARROW) {
+        float sk[DP / 8], sv[DP / 8];
+        __syncthreads(); // every wave is done with its tiles
+        at_sum_waves<DP / 2>(fk, reinterpret_cast<float*>(sh.tiles), sk);
+        __syncthreads();
+        at_sum_waves<DP / 2>(fv, reinterpret_cast<float*>(sh.tiles), sv);
+        if (key >= a.Nk) return;
+#pragma unroll
+        for (int n = 0; n < DP / 32; ++n) store(wave * (DP / 32) + n, sk + 4 * n, sv + 4 * n);
+        return;
+    }
+    if (key >= a.Nk) return;
+#pragma unroll
+    for (int n = 0; n < DP / 8; ++n) store(n, fk + 4 * n, fv + 4 * n);
+}
+
+// PART 1: the rows' workgroups, 2: the keys', 3: both in one launch, the keys' first (they are the longer ones).
+template <typename T, int DP, bool MASKED, bool NARROW, int PART>
+__global__ __launch_bounds__(256, PART > 1 && (DP == 128 || NARROW) ? 1 : 2) void at_bwd_kernel(AttendArgs a)
+{
+    union Shared {
+        AtShared<T, DP, NARROW> rows;
+        AtSharedKeys<T, DP, MASKED, NARROW> keys;
+    };
+    if constexpr (PART == 1) {
+        __shared__ __attribute__((aligned(16))) AtShared<T, DP, NARROW> sh;
+        at_bwd_rows<T, DP, MASKED, NARROW>(a, sh, xcd_remap(blockIdx.x, gridDim.x));
+    } else if constexpr (PART == 2) {
+        __shared__ __attribute__((aligned(16))) AtSharedKeys<T, DP, MASKED, NARROW> sh;
+        at_bwd_keys<T, DP, MASKED, NARROW>(a, sh, xcd_remap(blockIdx.x, gridDim.x));
+    } else {
+        __shared__ __attribute__((aligned(16))) char raw[sizeof(Shared)];
+        Shared& sh = *reinterpret_cast<Shared*>(raw);
+        const int first = (a.Nk + AtShape<NARROW>::OWN - 1) / AtShape<NARROW>::OWN * a.B * a.Hk, id = blockIdx.x;
+        if (id < first) at_bwd_keys<T, DP, MASKED, NARROW>(a, sh.keys, xcd_remap(id, first));
+        else at_bwd_rows<T, DP, MASKED, NARROW>(a, sh.rows, xcd_remap(id - first, gridDim.x - first));
+    }
 }
 
 // -------------------------------------------------------------------------------------------------------------------- launches
-// Parts that a row's keys are cut into: enough workgroups for two on each of the 256 CUs, at least two tiles of keys a part.
+// The wide shape fills the chip from two workgroups a CU on.
+static bool at_narrow(int64_t B, int Hk, int64_t owned) { return B * Hk * ceil_div(owned, 128) < 512; }
+// Parts that a row's keys are cut into where even the narrow shape's workgroups are few: two on each of the 256 CUs, at least 256 keys a part.
 static int at_splits(int64_t B, int Hk, int64_t R, int Nk) {
-    const int64_t groups = B * Hk * ceil_div(R, AT_ROWS);
-    const int64_t tiles = ceil_div(Nk, AT_TILE);
-    int64_t s = ceil_div(512, groups);
-    if (s > tiles / 2) s = tiles / 2;
+    if (!at_narrow(B, Hk, R)) return 1;
+    int64_t s = 512 / (B * Hk * ceil_div(R, 32));
+    if (s > Nk / 256) s = Nk / 256;
     return (int)(s < 1 ? 1 : s > 64 ? 64 : s);
 }
 
@@ -702,7 +832,7 @@ static int at_check(int dtype, int B, int H, int Hk, int Nq, int Nk, int D, floa
     if (D < 8 || D > 128 || (D & 7)) return ADK_EUNSUPPORTED;
     if (!(scale > 0.f) || !(scale < INFINITY)) return ADK_EINVAL;
     const int64_t R = (int64_t)(H / Hk) * Nq; // row and key numbers, and a grid, in 31 bits
-    if (R > 0x7fffff00ll || Nk > 0x7fffff00 || (int64_t)B * Hk * ceil_div(R > Nk ? R : Nk, AT_ROWS) > 0x1ffffff) return ADK_EUNSUPPORTED;
+    if (R > 0x7fffff00ll || Nk > 0x7fffff00 || (int64_t)B * Hk * ceil_div(R + Nk, 32) > 0xffffff) return ADK_EUNSUPPORTED;
     if ((int64_t)B * H * Nq > 0x7fffff00ll * 8) return ADK_EUNSUPPORTED;
     return 0;
 }
@@ -713,31 +843,39 @@ static int at_tensor(const void* p, const int64_t* s) {
     return s[2] < 0 || s[2] >= (1 << 24) ? ADK_EUNSUPPORTED : 0; // 64 rows of a tile in 32-bit byte offsets
 }
 
-#define AT_LAUNCH3(KERNEL, T, GRID)                                                                                             \
-    do {                                                                                                                        \
-        if (a.D <= 64) {                                                                                                        \
-            if (a.mask) hipLaunchKernelGGL((KERNEL<T, 64, true>), dim3(GRID), dim3(256), 0, stream, a);                         \
-            else hipLaunchKernelGGL((KERNEL<T, 64, false>), dim3(GRID), dim3(256), 0, stream, a);                               \
-        } else {                                                                                                                \
-            if (a.mask) hipLaunchKernelGGL((KERNEL<T, 128, true>), dim3(GRID), dim3(256), 0, stream, a);                        \
-            else hipLaunchKernelGGL((KERNEL<T, 128, false>), dim3(GRID), dim3(256), 0, stream, a);                              \
-        }                                                                                                                       \
-    } while (0)
+template <typename T, int DP, bool MASKED> static void at_launch_fwd(const AttendArgs& a, hipStream_t stream) {
+    const int64_t R = (int64_t)a.G * a.Nq;
+    if (at_narrow(a.B, a.Hk, R)) hipLaunchKernelGGL((at_fwd_kernel<T, DP, MASKED, true>), dim3((unsigned)(ceil_div(R, 32) * a.B * a.Hk * a.splits)), dim3(256), 0, stream, a);
+    else hipLaunchKernelGGL((at_fwd_kernel<T, DP, MASKED, false>), dim3((unsigned)(ceil_div(R, 128) * a.B * a.Hk)), dim3(256), 0, stream, a);
+}
+template <typename T, int DP, bool MASKED> static void at_launch_bwd(const AttendArgs& a, hipStream_t stream) {
+    const int64_t R = (int64_t)a.G * a.Nq, bh = (int64_t)a.B * a.Hk;
+    if (at_narrow(a.B, a.Hk, R + a.Nk)) {
+        const int64_t groups = (ceil_div(a.Nk, 32) + ceil_div(R, 32)) * bh;
+        hipLaunchKernelGGL((at_bwd_kernel<T, DP, MASKED, true, 3>), dim3((unsigned)groups), dim3(256), 0, stream, a);
+    } else {
+        const int64_t groups = (ceil_div(a.Nk, 128) + ceil_div(R, 128)) * bh;
+        if (DP == 64 && groups < 2048) { // 8 a CU: below, the tails of two launches cost more than the rows' third wave a SIMD brings
+            hipLaunchKernelGGL((at_bwd_kernel<T, 64, MASKED, false, 3>), dim3((unsigned)groups), dim3(256), 0, stream, a);
+            return;
+        }
+        if (a.Nk) hipLaunchKernelGGL((at_bwd_kernel<T, DP, MASKED, false, 2>), dim3((unsigned)(ceil_div(a.Nk, 128) * bh)), dim3(256), 0, stream, a);
+        if (R) hipLaunchKernelGGL((at_bwd_kernel<T, DP, MASKED, false, 1>), dim3((unsigned)(ceil_div(R, 128) * bh)), dim3(256), 0, stream, a);
+    }
+}
 
 template <typename T> static int at_fwd(const AttendArgs& a, hipStream_t stream) {
-    const int64_t R = (int64_t)a.G * a.Nq;
-    AT_LAUNCH3(at_fwd_kernel, T, (unsigned)(ceil_div(R, AT_ROWS) * a.B * a.Hk * a.splits));
+    if (a.D <= 64) { if (a.mask) at_launch_fwd<T, 64, true>(a, stream); else at_launch_fwd<T, 64, false>(a, stream); }
+    else { if (a.mask) at_launch_fwd<T, 128, true>(a, stream); else at_launch_fwd<T, 128, false>(a, stream); }
     if (a.splits > 1) hipLaunchKernelGGL((at_join_kernel<T>), dim3((unsigned)ceil_div((int64_t)a.B * a.H * a.Nq, 8)), dim3(256), 0, stream, a);
     ADK_RETURN_LAST_ERROR();
 }
 
 template <typename T> static int at_bwd(const AttendArgs& a, hipStream_t stream) {
-    const int64_t R = (int64_t)a.G * a.Nq, rows = (int64_t)a.B * a.H * a.Nq;
-    if (rows) {
-        hipLaunchKernelGGL((at_delta_kernel<T>), dim3((unsigned)ceil_div(rows, AT_DELTA_ROWS)), dim3(256), 0, stream, a);
-        AT_LAUNCH3(at_bwd_rows_kernel, T, (unsigned)(ceil_div(R, AT_ROWS) * a.B * a.Hk));
-    }
-    if (a.Nk) AT_LAUNCH3(at_bwd_keys_kernel, T, (unsigned)(ceil_div(a.Nk, AT_ROWS) * a.B * a.Hk));
+    const int64_t rows = (int64_t)a.B * a.H * a.Nq;
+    if (rows) hipLaunchKernelGGL((at_delta_kernel<T>), dim3((unsigned)ceil_div(rows, AT_DELTA_ROWS)), dim3(256), 0, stream, a);
+    if (a.D <= 64) { if (a.mask) at_launch_bwd<T, 64, true>(a, stream); else at_launch_bwd<T, 64, false>(a, stream); }
+    else { if (a.mask) at_launch_bwd<T, 128, true>(a, stream); else at_launch_bwd<T, 128, false>(a, stream); }
     ADK_RETURN_LAST_ERROR();
 }
 
