@@ -160,24 +160,32 @@ template <typename T> __device__ __forceinline__ typename AtEl<T>::x8 at_global_
     return col < D ? *reinterpret_cast<const typename AtEl<T>::x8*>(row + col) : z;
 }
 
-// Which of a row's keys k0 + 8 (r / 4) + r % 4 a mask shows, as bit r.  Bytes are read at keys of the tensor (`last` repeats); where 4
-// keys lie side by side in memory and the whole range is inside, four at a time.
+// Which of a row's keys k0 + 8 (r / 4) + r % 4 a mask shows.  Asked for a tile ahead: 16 bytes stay on their way until bits() wants them
+// (bit r for key r).  Where 4 keys lie side by side in memory and the whole range is inside the tensor, four at a time; otherwise bytes,
+// at keys of the tensor (`last` repeats).
 struct __attribute__((packed, aligned(1))) AtFour { uint32_t x; };
-__device__ __forceinline__ uint32_t at_mask_bits(const uint8_t* row, int64_t sk, int k0, int last, bool four) {
-    uint32_t bits = 0;
-    if (four) {
+struct AtMask16 {
+    uint32_t x[4];
+    __device__ __forceinline__ void ask(const uint8_t* row, int64_t sk, int k0, int last, bool four) {
+        if (four) {
 #pragma unroll
-        for (int r4 = 0; r4 < 4; ++r4) {
-            const uint32_t x = reinterpret_cast<const AtFour*>(row + k0 + 8 * r4)->x;
+            for (int r4 = 0; r4 < 4; ++r4) x[r4] = reinterpret_cast<const AtFour*>(row + k0 + 8 * r4)->x;
+        } else {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) bits |= ((x >> (8 * e)) & 255u ? 1u : 0u) << (4 * r4 + e);
+            for (int r4 = 0; r4 < 4; ++r4) {
+                x[r4] = 0;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[r4] |= (uint32_t)row[(int64_t)min(k0 + 8 * r4 + e, last) * sk] << (8 * e);
+            }
         }
-    } else {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) bits |= (row[(int64_t)min(k0 + 8 * (r >> 2) + (r & 3), last) * sk] ? 1u : 0u) << r;
     }
-    return bits;
-}
+    __device__ __forceinline__ uint32_t bits() const {
+        uint32_t b = 0;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) b |= ((x[r >> 2] >> (8 * (r & 3))) & 255u ? 1u : 0u) << r;
+        return b;
+    }
+};
 // Hiding is by selects on such bits: with a branch around the byte's load hipcc 7.2 lost the hiding of an accumulator's element 0.
 // Bits r of the keys k0 + 8 (r / 4) + r % 4 that lie below lim.
 __device__ __forceinline__ uint32_t at_below_bits(int k0, int lim) {
@@ -194,12 +202,11 @@ template <typename T, int DP, bool NARROW, int BUFS = 2> struct AtShared {
     float unit4[4];
     float m[4][32], l[4][32];
 };
-template <typename T, int DP, bool MASKED, bool NARROW> struct AtSharedKeys {
+template <typename T, int DP, bool NARROW> struct AtSharedKeys {
     static constexpr int S = AtShape<NARROW>::STREAMS, TILE = AtShape<NARROW>::TILE;
     T tiles[S][2][2][TILE * DP];
     float lse[S][2][TILE], delta[S][2][TILE];
     int lim[S][2][TILE];
-    int64_t mask[S][MASKED ? 2 : 1][MASKED ? TILE : 1];
     float unit4[4];
 };
 
@@ -218,6 +225,20 @@ template <int REGS> __device__ __forceinline__ void at_sum_waves(const float* mi
 // The first channel of the four that accumulator values 4 n .. 4 n + 3 hold.
 __device__ __forceinline__ int at_channel(int n, int h) { return 32 * (n >> 2) + 8 * (n & 3) + 4 * h; }
 
+// Which tile, part, key head and sequence workgroup `id` of a launch has.  Tiles lie side by side, so that the workgroups of one XCD
+// (a consecutive range, by xcd_remap) share K and V in its L2; with lengths the sequences do, because a range of its own would leave the
+// XCDs of short ones idle (lengths 1031, 637, 243, 0: as long as with four of 1031).
+struct AtWhere { int tile, split, kh, b; };
+__device__ __forceinline__ AtWhere at_where(const AttendArgs& a, int id, int tiles, int splits) {
+    AtWhere w;
+    if (a.key_lengths) { w.b = id % a.B; id /= a.B; }
+    w.tile = id % tiles; id /= tiles;
+    w.split = id % splits; id /= splits;
+    w.kh = id % a.Hk; id /= a.Hk;
+    if (!a.key_lengths) w.b = id;
+    return w;
+}
+
 // ------------------------------------------------------------------------------------------------------------------- forward
 template <typename T, int DP, bool MASKED, bool NARROW>
 __global__ __launch_bounds__(256, 2) void at_fwd_kernel(AttendArgs a)
@@ -229,12 +250,8 @@ __global__ __launch_bounds__(256, 2) void at_fwd_kernel(AttendArgs a)
     __shared__ __attribute__((aligned(16))) AtShared<T, DP, NARROW, BUFS> sh;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, c = lane & 31, stream = NARROW ? wave : 0;
     const int R = a.G * a.Nq, tiles = (R + OWN - 1) / OWN;
-    int id = xcd_remap(blockIdx.x, gridDim.x);
-    const int tile = a.causal ? tiles - 1 - id % tiles : id % tiles; // the long rows of a causal call first
-    id /= tiles;
-    const int split = id % a.splits;
-    id /= a.splits;
-    const int kh = id % a.Hk, b = id / a.Hk;
+    const AtWhere where = at_where(a, xcd_remap(blockIdx.x, gridDim.x), tiles, a.splits);
+    const int tile = a.causal ? tiles - 1 - where.tile : where.tile, split = where.split, kh = where.kh, b = where.b; // the long rows of a causal call first
 
     const int len = a.key_lengths ? min(max(a.key_lengths[b], 0), a.Nk) : a.Nk;
     const int row = tile * OWN + (NARROW ? 0 : wave * 32) + c, rowc = min(row, R - 1), g = rowc / a.Nq, i = rowc - g * a.Nq;
@@ -260,8 +277,14 @@ __global__ __launch_bounds__(256, 2) void at_fwd_kernel(AttendArgs a)
     auto hide = [&](int t, T* tile) {
         if (MASKED && a.mask_by_key) Tile::hide(tile, mkey + (int64_t)t * TILE * a.m_sk, a.m_sk, len - t * TILE);
     };
+    AtMask16 raw[MASKED ? SUBS : 1];
+    auto ask = [&](int t) {
+        if (MASKED)
+#pragma unroll
+            for (int n = 0; n < SUBS; ++n) raw[n].ask(mrow, a.m_sk, t * TILE + 32 * n + 4 * h, a.Nk - 1, a.m_sk == 1 && (t + 1) * TILE <= a.Nk);
+    };
     Tile::pad(sh.tiles[0][0][0], BUFS, a.D);
-    if (t0 + stream < t1) { load_k(t0 + stream, 0); load_v(t0 + stream, 0); }
+    if (t0 + stream < t1) { load_k(t0 + stream, 0); load_v(t0 + stream, 0); ask(t0 + stream); }
     x8 qf[DP / 16];
     {
         const T* qp = static_cast<const T*>(a.q) + (int64_t)b * a.q_sb + (int64_t)head * a.q_sh + (int64_t)i * a.q_sn;
@@ -282,9 +305,13 @@ __global__ __launch_bounds__(256, 2) void at_fwd_kernel(AttendArgs a)
             hide(t, tk);
             hide(t, tv);
             __syncthreads(); // tile t is in place, and nobody reads the other buffer any more
-            if (t + 1 < t1) { load_k(t + 1, buf ^ 1); load_v(t + 1, buf ^ 1); }
-            if (t * TILE >= wave_top) continue;
         }
+        uint32_t seen[SUBS];
+#pragma unroll
+        for (int n = 0; n < SUBS; ++n) seen[n] = MASKED ? raw[n].bits() : 0;
+        if (!NARROW && t + 1 < t1) { load_k(t + 1, buf ^ 1); load_v(t + 1, buf ^ 1); }
+        if (t + STREAMS < t1) ask(t + STREAMS);
+        if (!NARROW && t * TILE >= wave_top) continue;
         at_f32x16 st[SUBS] = {};
 #pragma unroll
         for (int ks = 0; ks < DP / 16; ++ks)
@@ -295,7 +322,7 @@ __global__ __launch_bounds__(256, 2) void at_fwd_kernel(AttendArgs a)
             for (int n = 0; n < SUBS; ++n) {
                 const int k0 = t * TILE + 32 * n + 4 * h;
                 uint32_t see = at_below_bits(k0, lim);
-                if (MASKED) see &= at_mask_bits(mrow, a.m_sk, k0, a.Nk - 1, a.m_sk == 1 && (t + 1) * TILE <= a.Nk);
+                if (MASKED) see &= seen[n];
 #pragma unroll
                 for (int r = 0; r < 16; ++r) st[n][r] = (see >> r) & 1u ? st[n][r] : -INFINITY;
             }
@@ -490,9 +517,8 @@ template <typename T, int DP, bool MASKED, bool NARROW> __device__ __forceinline
     constexpr int OWN = AtShape<NARROW>::OWN, TILE = AtShape<NARROW>::TILE, STREAMS = AtShape<NARROW>::STREAMS, SUBS = TILE / 32;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, c = lane & 31, stream = NARROW ? wave : 0;
     const int R = a.G * a.Nq, tiles = (R + OWN - 1) / OWN;
-    const int tile = a.causal ? tiles - 1 - id % tiles : id % tiles;
-    id /= tiles;
-    const int kh = id % a.Hk, b = id / a.Hk;
+    const AtWhere where = at_where(a, id, tiles, 1);
+    const int tile = a.causal ? tiles - 1 - where.tile : where.tile, kh = where.kh, b = where.b;
     const float unit = at_grad_unit<T>(a, b, kh, sh.unit4);
 
     const int len = a.key_lengths ? min(max(a.key_lengths[b], 0), a.Nk) : a.Nk;
@@ -516,8 +542,14 @@ template <typename T, int DP, bool MASKED, bool NARROW> __device__ __forceinline
         Tile::load(sh.tiles[stream][buf][0], kb + (int64_t)t * TILE * a.k_sn, (int)a.k_sn, len - t * TILE, a.D);
         Tile::load(sh.tiles[stream][buf][1], vb + (int64_t)t * TILE * a.v_sn, (int)a.v_sn, len - t * TILE, a.D);
     };
+    AtMask16 raw[MASKED ? SUBS : 1];
+    auto ask = [&](int t) {
+        if (MASKED)
+#pragma unroll
+            for (int n = 0; n < SUBS; ++n) raw[n].ask(mrow, a.m_sk, t * TILE + 32 * n + 4 * h, a.Nk - 1, a.m_sk == 1 && (t + 1) * TILE <= a.Nk);
+    };
     Tile::pad(sh.tiles[0][0][0], 2, a.D);
-    if (stream < t1) load(stream, 0);
+    if (stream < t1) { load(stream, 0); ask(stream); }
     x8 qf[DP / 16], gf[DP / 16];
     {
         const T* qp = static_cast<const T*>(a.q) + (int64_t)b * a.q_sb + (int64_t)head * a.q_sh + (int64_t)i * a.q_sn;
@@ -538,7 +570,10 @@ template <typename T, int DP, bool MASKED, bool NARROW> __device__ __forceinline
             Tile::hide(tv, mkey + (int64_t)t * TILE * a.m_sk, a.m_sk, len - t * TILE);
         }
         if (!NARROW) __syncthreads();
-        if (t + STREAMS < t1) load(t + STREAMS, buf ^ 1);
+        uint32_t seen[SUBS];
+#pragma unroll
+        for (int n = 0; n < SUBS; ++n) seen[n] = MASKED ? raw[n].bits() : 0;
+        if (t + STREAMS < t1) { load(t + STREAMS, buf ^ 1); ask(t + STREAMS); }
         if (t * TILE >= wave_top) continue;
         at_f32x16 st[SUBS] = {}, dp[SUBS] = {};
 #pragma unroll
@@ -553,7 +588,7 @@ template <typename T, int DP, bool MASKED, bool NARROW> __device__ __forceinline
             for (int n = 0; n < SUBS; ++n) {
                 const int k0 = t * TILE + 32 * n + 4 * h;
                 uint32_t see = at_below_bits(k0, lim);
-                if (MASKED) see &= at_mask_bits(mrow, a.m_sk, k0, a.Nk - 1, a.m_sk == 1 && (t + 1) * TILE <= a.Nk);
+                if (MASKED) see &= seen[n];
 #pragma unroll
                 for (int r = 0; r < 16; ++r) st[n][r] = (see >> r) & 1u ? st[n][r] : -INFINITY;
             }
@@ -600,7 +635,7 @@ template <typename T, int DP, bool MASKED, bool NARROW> __device__ __forceinline
 }
 
 // dK, dV: a wave owns 32 keys and walks the rows that may see them.
-template <typename T, int DP, bool MASKED, bool NARROW> __device__ __forceinline__ void at_bwd_keys(const AttendArgs& a, AtSharedKeys<T, DP, MASKED, NARROW>& sh, int id)
+template <typename T, int DP, bool MASKED, bool NARROW> __device__ __forceinline__ void at_bwd_keys(const AttendArgs& a, AtSharedKeys<T, DP, NARROW>& sh, int id)
 {
     typedef typename AtEl<T>::x8 x8;
     typedef typename AtEl<T>::x4 x4;
@@ -608,9 +643,8 @@ template <typename T, int DP, bool MASKED, bool NARROW> __device__ __forceinline
     constexpr int OWN = AtShape<NARROW>::OWN, TILE = AtShape<NARROW>::TILE, STREAMS = AtShape<NARROW>::STREAMS, SUBS = TILE / 32;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, c = lane & 31, stream = NARROW ? wave : 0;
     const int R = a.G * a.Nq, tiles = (a.Nk + OWN - 1) / OWN, off = a.Nk - a.Nq;
-    const int tile = id % tiles; // causal: the first keys are seen by most rows, the long ones come first as they are
-    id /= tiles;
-    const int kh = id % a.Hk, b = id / a.Hk;
+    const AtWhere where = at_where(a, id, tiles, 1);
+    const int tile = where.tile, kh = where.kh, b = where.b; // causal: the first keys are seen by most rows, the long ones come first as they are
     const float unit = at_grad_unit<T>(a, b, kh, sh.unit4);
     const int len = a.key_lengths ? min(max(a.key_lengths[b], 0), a.Nk) : a.Nk;
     const int k0 = tile * OWN, wave_k0 = k0 + (NARROW ? 0 : wave * 32), key = wave_k0 + c;
@@ -628,7 +662,7 @@ template <typename T, int DP, bool MASKED, bool NARROW> __device__ __forceinline
         const bool brings = NARROW ? lane < TILE : threadIdx.x < TILE;
         float n_lse = 0.f, n_delta = 0.f;
         int n_lim = -1;
-        int64_t n_mask = 0;
+        uint8_t raw[MASKED ? 16 * SUBS : 1];
         int g_next = 0, j_next = stream; // the next tile: head and number in it
         while (j_next >= per_head && g_next < a.G) { j_next -= per_head; ++g_next; }
         auto load = [&](int buf) { // returns the first row of the tile
@@ -643,7 +677,11 @@ template <typename T, int DP, bool MASKED, bool NARROW> __device__ __forceinline
                 n_lse = a.lse[at]; // as they are: worked on in note(), when they have long arrived
                 n_delta = a.delta[at];
                 n_lim = i >= a.Nq ? -1 : a.causal ? min(len - 1, i + off) : len - 1; // the last key that the row sees
-                if (MASKED) n_mask = (int64_t)g * a.m_sh + (int64_t)ic * a.m_sq;
+            }
+            if (MASKED) { // this key's byte of each row
+#pragma unroll
+                for (int r = 0; r < 16 * SUBS; ++r)
+                    raw[r] = mkey[(int64_t)g * a.m_sh + (int64_t)min(i0 + 32 * (r >> 4) + 8 * (r >> 2 & 3) + 4 * h + (r & 3), a.Nq - 1) * a.m_sq];
             }
             return i0;
         };
@@ -652,7 +690,6 @@ template <typename T, int DP, bool MASKED, bool NARROW> __device__ __forceinline
                 sh.lse[stream][buf][slot] = n_lse == -INFINITY ? -INFINITY : -n_lse * 1.4426950408889634f;
                 sh.delta[stream][buf][slot] = -n_delta * unit;
                 sh.lim[stream][buf][slot] = n_lim;
-                if (MASKED) sh.mask[stream][buf][slot] = n_mask;
             }
         };
         Tile::pad(sh.tiles[0][0][0], 2, a.D);
@@ -675,6 +712,10 @@ template <typename T, int DP, bool MASKED, bool NARROW> __device__ __forceinline
             at_landed();
             if (!NARROW) __syncthreads();
             i0 = i0_next;
+            uint32_t seen = 0; // bit r: this key's row r of the tile, in the accumulators' order
+            if (MASKED)
+#pragma unroll
+                for (int r = 0; r < 16 * SUBS; ++r) seen |= (raw[r] ? 1u : 0u) << r;
             if (t + STREAMS < t1) i0_next = load(buf ^ 1);
             // unless every row of the tile sees every key of the wave
             const bool edge = MASKED || i0 + TILE > a.Nq || wave_k0 + 32 > len || (a.causal && i0 + off < wave_k0 + 31);
@@ -696,7 +737,7 @@ template <typename T, int DP, bool MASKED, bool NARROW> __device__ __forceinline
                 for (int r = 0; r < 16; ++r) {
                     const int q = 32 * n + 8 * (r >> 2) + 4 * h + (r & 3);
                     bool on = key <= sh.lim[stream][buf][q];
-                    if (MASKED) on = on & (mkey[sh.mask[stream][buf][q]] != 0);
+                    if (MASKED) on = on & ((seen >> (16 * n + r)) & 1u);
                     st[n][r] = on ? st[n][r] : -INFINITY;
                 }
             };
@@ -798,13 +839,13 @@ __global__ __launch_bounds__(256, PART > 1 && (DP == 128 || NARROW) ? 1 : 2) voi
 {
     union Shared {
         AtShared<T, DP, NARROW> rows;
-        AtSharedKeys<T, DP, MASKED, NARROW> keys;
+        AtSharedKeys<T, DP, NARROW> keys;
     };
     if constexpr (PART == 1) {
         __shared__ __attribute__((aligned(16))) AtShared<T, DP, NARROW> sh;
         at_bwd_rows<T, DP, MASKED, NARROW>(a, sh, xcd_remap(blockIdx.x, gridDim.x));
     } else if constexpr (PART == 2) {
-        __shared__ __attribute__((aligned(16))) AtSharedKeys<T, DP, MASKED, NARROW> sh;
+        __shared__ __attribute__((aligned(16))) AtSharedKeys<T, DP, NARROW> sh;
         at_bwd_keys<T, DP, MASKED, NARROW>(a, sh, xcd_remap(blockIdx.x, gridDim.x));
     } else {
         __shared__ __attribute__((aligned(16))) char raw[sizeof(Shared)];
@@ -816,12 +857,21 @@ __global__ __launch_bounds__(256, PART > 1 && (DP == 128 || NARROW) ? 1 : 2) voi
 }
 
 // -------------------------------------------------------------------------------------------------------------------- launches
-// The wide shape fills the chip from two workgroups a CU on.
-static bool at_narrow(int64_t B, int Hk, int64_t owned) { return B * Hk * ceil_div(owned, 128) < 512; }
+// Which shape, by the workgroups of 128 rows (or keys) that the wide one would have on the 256 CUs.  Measured on both sides, D 64 | 128:
+//   forward, 768 keys: 96 workgroups 11.1 narrow 18.1 wide us | 16.0 23.1;  192: 13.9 18.3 | 26.0 24.4;  384: 24.7 24.6 | 46.5 35.5;
+//   2048 keys, causal, 256: 23.9 39.9 | 37.6 52.1;  8192 keys, 256: 125 146 | 203 212
+//   backward (both parts alike), 768 x 768: 48 + 48 workgroups 15.7 25.6 | 33.6 62.8;  96 + 96: 25.8 26.4 | 49.0 63.6;  144 + 144: 32.2 30.3 |
+//   82.9 66.4;  192 + 192: 37.9 32.0 | 101 69;  2048 x 2048, 128 + 128: 48.5 55.1 | 128 141
+static int64_t at_groups(int64_t bh, int64_t owned) { return bh * ceil_div(owned, 128); }
+static bool at_narrow_fwd(int64_t bh, int64_t R, int Nk, int D) {
+    const int64_t g = at_groups(bh, R);
+    return D <= 64 ? g < 384 : g <= 128 || (g <= 256 && Nk >= 1024);
+}
+static bool at_narrow_bwd(int64_t bh, int64_t owned, int D) { return at_groups(bh, owned) < (D <= 64 ? 144 : 112); }
 // Parts that a row's keys are cut into where even the narrow shape's workgroups are few: two on each of the 256 CUs, at least 256 keys a part.
-static int at_splits(int64_t B, int Hk, int64_t R, int Nk) {
-    if (!at_narrow(B, Hk, R)) return 1;
-    int64_t s = 512 / (B * Hk * ceil_div(R, 32));
+static int at_splits(int64_t bh, int64_t R, int Nk, int D) {
+    if (!at_narrow_fwd(bh, R, Nk, D)) return 1;
+    int64_t s = 512 / (bh * ceil_div(R, 32));
     if (s > Nk / 256) s = Nk / 256;
     return (int)(s < 1 ? 1 : s > 64 ? 64 : s);
 }
@@ -845,22 +895,28 @@ static int at_tensor(const void* p, const int64_t* s) {
 
 template <typename T, int DP, bool MASKED> static void at_launch_fwd(const AttendArgs& a, hipStream_t stream) {
     const int64_t R = (int64_t)a.G * a.Nq;
-    if (at_narrow(a.B, a.Hk, R)) hipLaunchKernelGGL((at_fwd_kernel<T, DP, MASKED, true>), dim3((unsigned)(ceil_div(R, 32) * a.B * a.Hk * a.splits)), dim3(256), 0, stream, a);
+    if (at_narrow_fwd((int64_t)a.B * a.Hk, R, a.Nk, a.D)) hipLaunchKernelGGL((at_fwd_kernel<T, DP, MASKED, true>), dim3((unsigned)(ceil_div(R, 32) * a.B * a.Hk * a.splits)), dim3(256), 0, stream, a);
     else hipLaunchKernelGGL((at_fwd_kernel<T, DP, MASKED, false>), dim3((unsigned)(ceil_div(R, 128) * a.B * a.Hk)), dim3(256), 0, stream, a);
 }
 template <typename T, int DP, bool MASKED> static void at_launch_bwd(const AttendArgs& a, hipStream_t stream) {
     const int64_t R = (int64_t)a.G * a.Nq, bh = (int64_t)a.B * a.Hk;
-    if (at_narrow(a.B, a.Hk, R + a.Nk)) {
-        const int64_t groups = (ceil_div(a.Nk, 32) + ceil_div(R, 32)) * bh;
-        hipLaunchKernelGGL((at_bwd_kernel<T, DP, MASKED, true, 3>), dim3((unsigned)groups), dim3(256), 0, stream, a);
-    } else {
-        const int64_t groups = (ceil_div(a.Nk, 128) + ceil_div(R, 128)) * bh;
-        if (DP == 64 && groups < 2048) { // 8 a CU: below, the tails of two launches cost more than the rows' third wave a SIMD brings
-            hipLaunchKernelGGL((at_bwd_kernel<T, 64, MASKED, false, 3>), dim3((unsigned)groups), dim3(256), 0, stream, a);
-            return;
-        }
-        if (a.Nk) hipLaunchKernelGGL((at_bwd_kernel<T, DP, MASKED, false, 2>), dim3((unsigned)(ceil_div(a.Nk, 128) * bh)), dim3(256), 0, stream, a);
-        if (R) hipLaunchKernelGGL((at_bwd_kernel<T, DP, MASKED, false, 1>), dim3((unsigned)(ceil_div(R, 128) * bh)), dim3(256), 0, stream, a);
+    const bool nk = at_narrow_bwd(bh, a.Nk, a.D), nr = at_narrow_bwd(bh, R, a.D);
+    const int64_t gk = ceil_div(a.Nk, nk ? 32 : 128) * bh, gr = ceil_div(R, nr ? 32 : 128) * bh;
+    if (nk && nr) {
+        hipLaunchKernelGGL((at_bwd_kernel<T, DP, MASKED, true, 3>), dim3((unsigned)(gk + gr)), dim3(256), 0, stream, a);
+        return;
+    }
+    if (DP == 64 && !nk && !nr && gk + gr < 2048) { // 8 a CU: below, the tails of two launches cost more than the rows' third wave a SIMD brings
+        hipLaunchKernelGGL((at_bwd_kernel<T, 64, MASKED, false, 3>), dim3((unsigned)(gk + gr)), dim3(256), 0, stream, a);
+        return;
+    }
+    if (gk) {
+        if (nk) hipLaunchKernelGGL((at_bwd_kernel<T, DP, MASKED, true, 2>), dim3((unsigned)gk), dim3(256), 0, stream, a);
+        else hipLaunchKernelGGL((at_bwd_kernel<T, DP, MASKED, false, 2>), dim3((unsigned)gk), dim3(256), 0, stream, a);
+    }
+    if (gr) {
+        if (nr) hipLaunchKernelGGL((at_bwd_kernel<T, DP, MASKED, true, 1>), dim3((unsigned)gr), dim3(256), 0, stream, a);
+        else hipLaunchKernelGGL((at_bwd_kernel<T, DP, MASKED, false, 1>), dim3((unsigned)gr), dim3(256), 0, stream, a);
     }
 }
 
@@ -900,7 +956,7 @@ extern "C" int64_t adk_attend_fwd_workspace_bytes(int B, int H, int Hk, int Nq, 
     const int e = adk::at_check(0, B, H, Hk, Nq, Nk, D, 1.f);
     if (e) return e;
     const int64_t rows = (int64_t)B * H * Nq;
-    const int s = rows ? adk::at_splits(B, Hk, (int64_t)(H / Hk) * Nq, Nk) : 1;
+    const int s = rows ? adk::at_splits((int64_t)B * Hk, (int64_t)(H / Hk) * Nq, Nk, D) : 1;
     return s > 1 ? s * rows * (D + 2) * 4 : 0;
 }
 
@@ -918,7 +974,7 @@ extern "C" int adk_attend_fwd(const void* q, const void* k, const void* v, void*
     const int64_t need = adk_attend_fwd_workspace_bytes(B, H, Hk, Nq, Nk, D);
     if (need > 0) {
         if (!ws || ws_bytes < need || ((uintptr_t)ws & 15)) return ADK_EWORKSPACE;
-        a.splits = adk::at_splits(B, Hk, (int64_t)a.G * Nq, Nk);
+        a.splits = adk::at_splits((int64_t)B * Hk, (int64_t)a.G * Nq, Nk, D);
         a.part_o = static_cast<float*>(ws);
         a.part_ml = a.part_o + (int64_t)a.splits * B * H * Nq * D;
     }
