@@ -149,7 +149,7 @@ class on_device:
     def __enter__(self):
         import torch
         idx = self.dev.index
-        if idx is not None and idx != torch.cuda.current_device():
+        if idx is not None and idx != torch._C._cuda_getDevice():  # current_device() without its check that CUDA is initialised: dev is a CUDA tensor's
             self.ctx = torch.cuda.device(self.dev)
             self.ctx.__enter__()
         return self

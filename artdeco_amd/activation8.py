@@ -6,6 +6,7 @@ backward pass takes both from it.  int8 holds a value to 1/254 .. 1/127 of its b
 results are exact, gradients are those of the held values."""
 from __future__ import annotations
 
+import math
 from typing import NamedTuple
 
 import torch
@@ -32,10 +33,7 @@ def _rows_width(what, shape, gated):
     if not shape or (gated and shape[-1] % 2):
         raise _lib.AdkError(f"{what}: x [..., width]{', width even (gate and up halves),' if gated else ''} is required; got {tuple(shape)}")
     width = shape[-1] // 2 if gated else shape[-1]
-    rows = 1
-    for n in shape[:-1]:
-        rows *= n
-    return rows, width
+    return math.prod(shape[:-1]), width
 
 
 def _names(what, kind, format):
@@ -52,40 +50,43 @@ def activation8_forward(x, *, kind="gelu", gated=False, format="int8"):
     if x.dtype not in _DTYPES or not x.is_contiguous():
         raise _lib.AdkError(f"activation8: a contiguous float16, bfloat16 or float32 tensor is required; got {x.dtype}, strides {x.stride()}")
     rows, width = _rows_width("activation8", x.shape, gated)
-    _lib.require_cuda(x)
+    if not x.is_cuda:
+        _lib.require_cuda(x)
+    shape, dtype, device = x.shape, x.dtype, x.device
     blocks = -(-x.numel() // 32)
-    y = torch.empty(*x.shape[:-1], width, dtype=x.dtype, device=x.device)
-    codes = torch.empty(32 * blocks, dtype=torch.uint8, device=x.device)
-    units = torch.empty(blocks, dtype=torch.uint8, device=x.device)
+    y = torch.empty((*shape[:-1], width), dtype=dtype, device=device)
+    codes = torch.empty(32 * blocks, dtype=torch.uint8, device=device)
+    units = torch.empty(blocks, dtype=torch.uint8, device=device)
     lib = _lib.load()
-    with _lib.on_device(x.device):
-        rc = lib.adk_activation8_fwd(x.data_ptr(), _DTYPES[x.dtype], rows, width, _KINDS[kind], int(bool(gated)), _FORMATS[format], y.data_ptr(), codes.data_ptr(),
-                                     units.data_ptr(), _lib.stream_of(x))
+    with _lib.on_device(device):
+        rc = lib.adk_activation8_fwd(x.data_ptr(), _DTYPES[dtype], rows, width, _KINDS[kind], gated, _FORMATS[format], y.data_ptr(), codes.data_ptr(),
+                                     units.data_ptr(), _lib.raw_stream(device))
     _lib.check(rc, "adk_activation8_fwd")
-    return y, Packed8(codes, units, tuple(x.shape), x.dtype, format)
+    return y, Packed8(codes, units, shape, dtype, format)
 
 
 def activation8_backward(grad, packed, *, kind="gelu", gated=False, again=True):
     """The gradient of activation8_forward's result from its Packed8 -> (dx, the activation of the held values or None without `again`).
     grad of the result's shape and type."""
     _names("activation8_backward", kind, packed.format)
-    rows, width = _rows_width("activation8_backward", packed.shape, gated)
-    shape = (*packed.shape[:-1], width)
-    if tuple(grad.shape) != shape or grad.dtype != packed.dtype:
-        raise _lib.AdkError(f"activation8_backward: grad {shape} {packed.dtype} is required; got {tuple(grad.shape)} {grad.dtype}")
-    n = rows * width * (2 if gated else 1)
-    c, u = packed.codes, packed.units
-    if (c.dtype != torch.uint8 or u.dtype != torch.uint8 or c.numel() < -(-n // 32) * 32 or u.numel() < -(-n // 32) or not c.is_contiguous() or not u.is_contiguous()
-            or c.device != grad.device or u.device != grad.device or c.data_ptr() % 8 or packed.dtype not in _DTYPES):
+    codes, units, pshape, dtype, format = packed
+    rows, width = _rows_width("activation8_backward", pshape, gated)
+    shape, device = (*pshape[:-1], width), grad.device
+    if grad.shape != shape or grad.dtype != dtype:
+        raise _lib.AdkError(f"activation8_backward: grad {shape} {dtype} is required; got {tuple(grad.shape)} {grad.dtype}")
+    blocks = -(-rows * width * (2 if gated else 1) // 32)
+    if (codes.dtype != torch.uint8 or units.dtype != torch.uint8 or codes.numel() < 32 * blocks or units.numel() < blocks or not codes.is_contiguous()
+            or not units.is_contiguous() or codes.device != device or units.device != device or codes.data_ptr() & 7 or dtype not in _DTYPES):
         raise _lib.AdkError("activation8_backward: packed is not what activation8_forward returned, on grad's device")
-    _lib.require_cuda(grad, c, u)
+    if not grad.is_cuda:
+        _lib.require_cuda(grad)
     grad = grad.contiguous()
-    dx = torch.empty(packed.shape, dtype=packed.dtype, device=grad.device)
-    y = torch.empty(shape, dtype=packed.dtype, device=grad.device) if again else None
+    dx = torch.empty(pshape, dtype=dtype, device=device)
+    y = torch.empty(shape, dtype=dtype, device=device) if again else None
     lib = _lib.load()
-    with _lib.on_device(grad.device):
-        rc = lib.adk_activation8_bwd(grad.data_ptr(), c.data_ptr(), u.data_ptr(), _DTYPES[packed.dtype], rows, width, _KINDS[kind], int(bool(gated)),
-                                     _FORMATS[packed.format], dx.data_ptr(), _lib.ptr(y), _lib.stream_of(grad))
+    with _lib.on_device(device):
+        rc = lib.adk_activation8_bwd(grad.data_ptr(), codes.data_ptr(), units.data_ptr(), _DTYPES[dtype], rows, width, _KINDS[kind], gated, _FORMATS[format],
+                                     dx.data_ptr(), _lib.ptr(y), _lib.raw_stream(device))
     _lib.check(rc, "adk_activation8_bwd")
     return dx, y
 

@@ -52,18 +52,50 @@ _DTYPES = {torch.float16: 0, torch.bfloat16: 2}
 def _strides(t: torch.Tensor):
     """Element strides of the first three dimensions; a dimension of one element has none that matters."""
     a, b, c = t.shape[:3]
-    x, y, z, _ = t.stride()
-    return [x if a > 1 else 0, y if b > 1 else 0, z if c > 1 else 0]
+    x, y, z = t.stride()[:3]
+    return (x if a > 1 else 0, y if b > 1 else 0, z if c > 1 else 0)
 
 
-def _loadable(t: torch.Tensor, strides) -> bool:
-    a, b, c = strides
-    return t.stride(3) == 1 and not (a | b | c) & 7 and not t.data_ptr() & 15
-
-
-def _check_attend(what, q, k, v, scale, mask, key_lengths):
+def _prepare(what, q, k, v, scale, mask, key_lengths):
     """-> (scale, mask broadcast to [B, H, Nq, Nk] or None, the strides of q, k, v and the mask); raises AdkError for what the kernels do
-    not take."""
+    not take.  The usual call passes one test; _refuse says what is wrong with another."""
+    try:
+        B, H, Nq, D = q.shape
+        Bk, Hk, Nk, Dk = kshape = k.shape
+        qs, ks, vs = q.stride(), k.stride(), v.stride()
+        plain = (Bk == B and Dk == D and v.shape == kshape and Hk > 0 and H > 0 and H % Hk == 0 and not D & 7 and 8 <= D <= 128 and q.dtype in _DTYPES
+                 and q.dtype == k.dtype == v.dtype and q.device == k.device == v.device and qs[3] == ks[3] == vs[3] == 1
+                 and not (qs[0] | qs[1] | qs[2] | ks[0] | ks[1] | ks[2] | vs[0] | vs[1] | vs[2]) & 7 and not (q.data_ptr() | k.data_ptr() | v.data_ptr()) & 15)
+    except ValueError:
+        plain = False
+    if not plain:
+        _refuse(what, q, k, v)
+        B, H, Nq, D = q.shape
+        Nk = k.shape[2]
+        qs, ks, vs = _strides(q), _strides(k), _strides(v)
+    if scale is None:
+        scale = D ** -0.5
+    elif not 0.0 < scale < math.inf:
+        raise _lib.AdkError(f"{what}: scale is a positive number; got {scale}")
+    if key_lengths is not None and (key_lengths.dtype != torch.int32 or key_lengths.shape != (B,) or not key_lengths.is_contiguous() or key_lengths.device != q.device):
+        raise _lib.AdkError(f"{what}: key_lengths is a contiguous int32 tensor of the batch's size on q's device")
+    if mask is None:
+        ms = (0, 0, 0, 0)
+    else:
+        if mask.dtype != torch.bool or mask.device != q.device:
+            raise _lib.AdkError(f"{what}: mask is a boolean tensor on q's device, True where a query sees a key (biases that are added to the scores are not "
+                                "supported)")
+        try:
+            mask = mask.broadcast_to(B, H, Nq, Nk)
+        except RuntimeError:
+            raise _lib.AdkError(f"{what}: mask of shape {tuple(mask.shape)} does not broadcast to {(B, H, Nq, Nk)}") from None
+        ms = [0 if n == 1 else s for n, s in zip(mask.shape, mask.stride())]
+    if not q.is_cuda:
+        _lib.require_cuda(q)
+    return scale, mask, (*qs[:3], *ks[:3], *vs[:3], *ms)
+
+
+def _refuse(what, q, k, v):
     if not (q.dim() == k.dim() == v.dim() == 4):
         raise _lib.AdkError(f"{what}: q [B,H,Nq,D], k and v [B,Hk,Nk,D] are required")
     B, H, Nq, D = q.shape
@@ -74,39 +106,19 @@ def _check_attend(what, q, k, v, scale, mask, key_lengths):
         raise _lib.AdkError(f"{what}: q, k and v are float16 or bfloat16, all of one type; got {q.dtype}, {k.dtype}, {v.dtype}")
     if D % 8 or not 8 <= D <= 128:
         raise _lib.AdkError(f"{what}: head sizes 8 to 128, multiples of 8, are supported; got {D}")
-    strides = []
+    if not q.device == k.device == v.device:
+        raise _lib.AdkError(f"{what}: all tensors are on one device; got {q.device}, {k.device}, {v.device}")
     for name, t in (("q", q), ("k", k), ("v", v)):
-        s = _strides(t)
-        strides += s
-        if not _loadable(t, s) and t.numel():
+        a, b, c = _strides(t)
+        if t.numel() and (t.stride(3) != 1 or (a | b | c) & 7 or t.data_ptr() & 15):
             raise _lib.AdkError(f"{what}: {name} needs a dense last dimension, strides that are multiples of 8 elements and 16-byte aligned storage")
-    device = q.device
-    for t in (k, v, mask, key_lengths):
-        if t is not None and t.device != device:
-            raise _lib.AdkError(f"{what}: all tensors are on one device; got {q.device} and {t.device}")
-    scale = float(scale) if scale is not None else 1.0 / math.sqrt(D)
-    if not 0.0 < scale < math.inf:
-        raise _lib.AdkError(f"{what}: scale is a positive number; got {scale}")
-    if key_lengths is not None and (key_lengths.dtype != torch.int32 or key_lengths.shape != (B,) or not key_lengths.is_contiguous()):
-        raise _lib.AdkError(f"{what}: key_lengths is a contiguous int32 tensor of the batch's size")
-    if mask is not None:
-        if mask.dtype != torch.bool:
-            raise _lib.AdkError(f"{what}: mask is a boolean tensor, True where a query sees a key (biases that are added to the scores are not supported)")
-        try:
-            mask = mask.broadcast_to(B, H, Nq, k.shape[2])
-        except RuntimeError:
-            raise _lib.AdkError(f"{what}: mask of shape {tuple(mask.shape)} does not broadcast to {(B, H, Nq, k.shape[2])}") from None
-        strides += [0 if n == 1 else s for n, s in zip(mask.shape, mask.stride())]
-    else:
-        strides += (0, 0, 0, 0)
-    _lib.require_cuda(q)
-    return scale, mask, strides
 
 
 def _workspace(nbytes, what, device):
-    if nbytes < 0:
+    if nbytes <= 0:
         _lib.check(nbytes, what)
-    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+        return None
+    return torch.empty(nbytes, dtype=torch.uint8, device=device)
 
 
 def attend_forward(q, k, v, *, scale=None, causal=False, mask=None, key_lengths=None):
@@ -119,18 +131,18 @@ def attend_forward(q, k, v, *, scale=None, causal=False, mask=None, key_lengths=
     mask         bool, broadcastable to [B,H,Nq,Nk], True where a query sees a key; what it hides from a query has to hold finite
                  numbers, unless the mask is the same for all queries and heads.
     All three hold together.  A query that sees no key gives zeros and lse = -inf."""
-    scale, mask, strides = _check_attend("attend_forward", q, k, v, scale, mask, key_lengths)
+    scale, mask, strides = _prepare("attend_forward", q, k, v, scale, mask, key_lengths)
     B, H, Nq, D = q.shape
     Hk, Nk = k.shape[1], k.shape[2]
+    dtype, device = q.dtype, q.device
     held = array("q", strides)  # alive until the call returns
-    out = torch.empty(B, Nq, H * D, dtype=q.dtype, device=q.device)
-    lse = torch.empty(B, H, Nq, dtype=torch.float32, device=q.device)
+    out = torch.empty((B, Nq, H * D), dtype=dtype, device=device)
+    lse = torch.empty((B, H, Nq), dtype=torch.float32, device=device)
     lib = _lib.load()
-    with _lib.on_device(q.device):
-        ws = _workspace(lib.adk_attend_fwd_workspace_bytes(B, H, Hk, Nq, Nk, D), "adk_attend_fwd", q.device)
-        rc = lib.adk_attend_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), _lib.ptr(key_lengths), _lib.ptr(mask), _DTYPES[q.dtype],
-                                B, H, Hk, Nq, Nk, D, held.buffer_info()[0], scale, bool(causal), _lib.ptr(ws), 0 if ws is None else ws.numel(),
-                                _lib.stream_of(q))
+    with _lib.on_device(device):
+        ws = _workspace(lib.adk_attend_fwd_workspace_bytes(B, H, Hk, Nq, Nk, D), "adk_attend_fwd", device)
+        rc = lib.adk_attend_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), _lib.ptr(key_lengths), _lib.ptr(mask), _DTYPES[dtype],
+                                B, H, Hk, Nq, Nk, D, held.buffer_info()[0], scale, causal, _lib.ptr(ws), 0 if ws is None else ws.numel(), _lib.raw_stream(device))
     _lib.check(rc, "adk_attend_fwd")
     return out, lse
 
@@ -139,18 +151,19 @@ def _backward_into(grad_out, q, k, v, out, lse, scale, causal, mask, key_lengths
     B, H, Nq, D = q.shape
     Hk, Nk = k.shape[1], k.shape[2]
     a, b, c = grad_out.stride()
-    g = [a if B > 1 else 0, D if H > 1 else 0, b if Nq > 1 else 0]
-    if grad_out.numel() and (c != 1 or (g[0] | g[2]) & 7 or grad_out.data_ptr() & 15):  # an expanded gradient, of a sum for instance
+    g = (a if B > 1 else 0, D if H > 1 else 0, b if Nq > 1 else 0)
+    if (c != 1 or (g[0] | g[2]) & 7 or grad_out.data_ptr() & 15) and grad_out.numel():  # an expanded gradient, of a sum for instance
         grad_out = grad_out.contiguous()
         grad_out = grad_out.clone() if grad_out.data_ptr() & 15 else grad_out
-        g = [Nq * H * D, D, H * D]
+        g = (Nq * H * D, D, H * D)
+    device = q.device
     lib = _lib.load()
-    held = array("q", strides + g + _strides(dq) + _strides(dk) + _strides(dv))
-    with _lib.on_device(q.device):
-        ws = _workspace(lib.adk_attend_bwd_workspace_bytes(B, H, Hk, Nq, Nk, D), "adk_attend_bwd", q.device)
+    held = array("q", (*strides, *g, *dq.stride()[:3], *dk.stride()[:3], *dv.stride()[:3]))
+    with _lib.on_device(device):
+        ws = _workspace(lib.adk_attend_bwd_workspace_bytes(B, H, Hk, Nq, Nk, D), "adk_attend_bwd", device)
         rc = lib.adk_attend_bwd(grad_out.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), _lib.ptr(key_lengths), _lib.ptr(mask),
-                                _DTYPES[q.dtype], B, H, Hk, Nq, Nk, D, held.buffer_info()[0], scale, bool(causal), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
-                                _lib.ptr(ws), 0 if ws is None else ws.numel(), _lib.stream_of(q))
+                                _DTYPES[q.dtype], B, H, Hk, Nq, Nk, D, held.buffer_info()[0], scale, causal, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+                                _lib.ptr(ws), 0 if ws is None else ws.numel(), _lib.raw_stream(device))
     _lib.check(rc, "adk_attend_bwd")
 
 
@@ -158,18 +171,21 @@ def attend_backward(grad_out, q, k, v, out, lse, *, scale=None, causal=False, ma
     """The gradient of attend_forward's out, called with the same arguments and what it returned -> (dq, dk, dv) in the shapes and
     the type of q, k and v ([B,N,heads,D] in memory).  grad_out [B,Nq,H*D].  The heads that share a key head are summed in 32 bits, in a
     fixed order; keys behind a sequence's length get zeros."""
-    scale, mask, strides = _check_attend("attend_backward", q, k, v, scale, mask, key_lengths)
+    scale, mask, strides = _prepare("attend_backward", q, k, v, scale, mask, key_lengths)
     B, H, Nq, D = q.shape
-    for name, t, shape, dtype in (("grad_out", grad_out, (B, Nq, H * D), q.dtype), ("out", out, (B, Nq, H * D), q.dtype), ("lse", lse, (B, H, Nq), torch.float32)):
-        if tuple(t.shape) != shape or t.dtype != dtype or t.device != q.device:
-            raise _lib.AdkError(f"attend_backward: {name} {shape} {dtype} on {q.device} is required; got {tuple(t.shape)} {t.dtype} on {t.device}")
+    Hk, Nk = k.shape[1], k.shape[2]
+    dtype, device, shape = q.dtype, q.device, (B, Nq, H * D)
+    if not (grad_out.shape == shape and out.shape == shape and lse.shape == (B, H, Nq) and grad_out.dtype == out.dtype == dtype and lse.dtype == torch.float32
+            and grad_out.device == out.device == lse.device == device):
+        raise _lib.AdkError(f"attend_backward: grad_out and out {shape} {dtype} and lse {(B, H, Nq)} float32 on {device} are required; got {tuple(grad_out.shape)} "
+                            f"{grad_out.dtype}, {tuple(out.shape)} {out.dtype}, {tuple(lse.shape)} {lse.dtype}")
     out, lse = out.contiguous(), lse.contiguous()
     if out.data_ptr() & 15:
         out = out.clone()
-    Hk, Nk = k.shape[1], k.shape[2]
-    dq = torch.empty(B, Nq, H, D, dtype=q.dtype, device=q.device).transpose(1, 2)
-    dk = torch.empty(B, Nk, Hk, D, dtype=q.dtype, device=q.device).transpose(1, 2)
-    dv = torch.empty(B, Nk, Hk, D, dtype=q.dtype, device=q.device).transpose(1, 2)
+    like = ((Nq * H * D, D, H * D, 1), (Nk * Hk * D, D, Hk * D, 1))
+    dq = torch.empty_strided((B, H, Nq, D), like[0], dtype=dtype, device=device)
+    dk = torch.empty_strided((B, Hk, Nk, D), like[1], dtype=dtype, device=device)
+    dv = torch.empty_strided((B, Hk, Nk, D), like[1], dtype=dtype, device=device)
     _backward_into(grad_out, q, k, v, out, lse, scale, causal, mask, key_lengths, strides, dq, dk, dv)
     return dq, dk, dv
 
@@ -218,7 +234,7 @@ class _AttendPacked(torch.autograd.Function):
         qkv, out, lse, mask, key_lengths = ctx.saved_tensors
         heads, kv_heads, scale, causal = ctx.how
         q, k, v = _packed_views(qkv, heads, kv_heads)
-        scale, mask, strides = _check_attend("attend_packed", q, k, v, scale, mask, key_lengths)
+        scale, mask, strides = _prepare("attend_packed", q, k, v, scale, mask, key_lengths)
         grad = torch.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device)
         _backward_into(grad_out, q, k, v, out, lse, scale, causal, mask, key_lengths, strides, *_packed_views(grad, heads, kv_heads))
         return grad, None, None, None, None, None, None

@@ -179,14 +179,20 @@ struct AtMask16 {
             }
         }
     }
+    // four bytes of 0 or 1 to four bits: byte e times 2^(24 - 7 e) lands on bit 24 + e, every other product on a bit of its own below 24
+    // or past 31
     __device__ __forceinline__ uint32_t bits() const {
         uint32_t b = 0;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) b |= ((x[r >> 2] >> (8 * (r & 3))) & 255u ? 1u : 0u) << r;
+        for (int r4 = 0; r4 < 4; ++r4) b |= ((x[r4] * 0x01020408u >> 24) & 15u) << (4 * r4);
         return b;
     }
 };
 // Hiding is by selects on such bits: with a branch around the byte's load hipcc 7.2 lost the hiding of an accumulator's element 0.
+__device__ __forceinline__ float at_hidden_unless(uint32_t bits, int r, float s) { // s if bit r is set, else -inf
+    const uint32_t on = (uint32_t)__builtin_amdgcn_sbfe((int)bits, r, 1);
+    return __uint_as_float((__float_as_uint(s) & on) | (0xff800000u & ~on));
+}
 // Bits r of the keys k0 + 8 (r / 4) + r % 4 that lie below lim.
 __device__ __forceinline__ uint32_t at_below_bits(int k0, int lim) {
     uint32_t bits = 0;
@@ -324,7 +330,7 @@ __global__ __launch_bounds__(256, 2) void at_fwd_kernel(AttendArgs a)
                 uint32_t see = at_below_bits(k0, lim);
                 if (MASKED) see &= seen[n];
 #pragma unroll
-                for (int r = 0; r < 16; ++r) st[n][r] = (see >> r) & 1u ? st[n][r] : -INFINITY;
+                for (int r = 0; r < 16; ++r) st[n][r] = at_hidden_unless(see, r, st[n][r]);
             }
         }
         if (NARROW) { // one buffer: K's next tile as soon as this one is read, V's at the end; half the LDS, so twice the waves
@@ -590,7 +596,7 @@ template <typename T, int DP, bool MASKED, bool NARROW> __device__ __forceinline
                 uint32_t see = at_below_bits(k0, lim);
                 if (MASKED) see &= seen[n];
 #pragma unroll
-                for (int r = 0; r < 16; ++r) st[n][r] = (see >> r) & 1u ? st[n][r] : -INFINITY;
+                for (int r = 0; r < 16; ++r) st[n][r] = at_hidden_unless(see, r, st[n][r]);
             }
         }
         x8 ds[SUBS][2];
@@ -679,9 +685,15 @@ template <typename T, int DP, bool MASKED, bool NARROW> __device__ __forceinline
                 n_lim = i >= a.Nq ? -1 : a.causal ? min(len - 1, i + off) : len - 1; // the last key that the row sees
             }
             if (MASKED) { // this key's byte of each row
+                const uint8_t* p = mkey + ((int64_t)g * a.m_sh + (int64_t)i0 * a.m_sq);
+                if (i0 + TILE <= a.Nq) {
+                    p += 4 * h * a.m_sq;
 #pragma unroll
-                for (int r = 0; r < 16 * SUBS; ++r)
-                    raw[r] = mkey[(int64_t)g * a.m_sh + (int64_t)min(i0 + 32 * (r >> 4) + 8 * (r >> 2 & 3) + 4 * h + (r & 3), a.Nq - 1) * a.m_sq];
+                    for (int r = 0; r < 16 * SUBS; ++r) raw[r] = p[(int64_t)(32 * (r >> 4) + 8 * (r >> 2 & 3) + (r & 3)) * a.m_sq];
+                } else {
+#pragma unroll
+                    for (int r = 0; r < 16 * SUBS; ++r) raw[r] = p[(int64_t)min(32 * (r >> 4) + 8 * (r >> 2 & 3) + 4 * h + (r & 3), a.Nq - 1 - i0) * a.m_sq];
+                }
             }
             return i0;
         };
@@ -715,7 +727,7 @@ template <typename T, int DP, bool MASKED, bool NARROW> __device__ __forceinline
             uint32_t seen = 0; // bit r: this key's row r of the tile, in the accumulators' order
             if (MASKED)
 #pragma unroll
-                for (int r = 0; r < 16 * SUBS; ++r) seen |= (raw[r] ? 1u : 0u) << r;
+                for (int r = 0; r < 16 * SUBS; ++r) seen |= (uint32_t)raw[r] << r;
             if (t + STREAMS < t1) i0_next = load(buf ^ 1);
             // unless every row of the tile sees every key of the wave
             const bool edge = MASKED || i0 + TILE > a.Nq || wave_k0 + 32 > len || (a.causal && i0 + off < wave_k0 + 31);
@@ -736,9 +748,8 @@ template <typename T, int DP, bool MASKED, bool NARROW> __device__ __forceinline
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
                     const int q = 32 * n + 8 * (r >> 2) + 4 * h + (r & 3);
-                    bool on = key <= sh.lim[stream][buf][q];
-                    if (MASKED) on = on & ((seen >> (16 * n + r)) & 1u);
-                    st[n][r] = on ? st[n][r] : -INFINITY;
+                    st[n][r] = key <= sh.lim[stream][buf][q] ? st[n][r] : -INFINITY;
+                    if (MASKED) st[n][r] = at_hidden_unless(seen, 16 * n + r, st[n][r]);
                 }
             };
             auto probs = [&](int n) {
@@ -835,7 +846,7 @@ template <typename T, int DP, bool MASKED, bool NARROW> __device__ __forceinline
 
 // PART 1: the rows' workgroups, 2: the keys', 3: both in one launch, the keys' first (they are the longer ones).
 template <typename T, int DP, bool MASKED, bool NARROW, int PART>
-__global__ __launch_bounds__(256, PART > 1 && (DP == 128 || NARROW) ? 1 : 2) void at_bwd_kernel(AttendArgs a)
+__global__ __launch_bounds__(256, DP == 128 && (PART > 1 || NARROW) ? 1 : 2) void at_bwd_kernel(AttendArgs a)
 {
     union Shared {
         AtShared<T, DP, NARROW> rows;

@@ -50,67 +50,66 @@ def rotary_frequencies(rotary_dim, *, axes=1, base=10000.0, scaling="none", scal
 
 
 def _turn(x, y, positions, frequencies, factor, layout, heads, transpose):
-    """The kernel's call: y may be x."""
-    if x.dim() != 4:
-        raise _lib.AdkError(f"rotary: x [B,N,H,D] is required; got {tuple(x.shape)}")
-    B, N, H, D = x.shape
-    if x.dtype not in _DTYPES:
-        raise _lib.AdkError(f"rotary: float16, bfloat16 and float32 are supported; got {x.dtype}")
-    if D > 1 and x.stride(3) != 1:
+    """The kernel's call: y is x (in place), or None for a new tensor.  -> y."""
+    try:
+        B, N, H, D = shape = x.shape
+    except ValueError:
+        raise _lib.AdkError(f"rotary: x [B,N,H,D] is required; got {tuple(x.shape)}") from None
+    dtype, device = x.dtype, x.device
+    xb, xn, xh, xd = x.stride()
+    if dtype not in _DTYPES:
+        raise _lib.AdkError(f"rotary: float16, bfloat16 and float32 are supported; got {dtype}")
+    if xd != 1 and D > 1:
         raise _lib.AdkError("rotary: x needs a dense last dimension")
-    if y is x and any(n > 1 and s == 0 for n, s in zip(x.shape, x.stride())):
-        raise _lib.AdkError("rotary_: x has elements that share their place")
     if layout not in _LAYOUTS:
         raise _lib.AdkError(f"rotary: layout is half or interleaved; got {layout!r}")
-    if frequencies.dim() != 1 or frequencies.dtype != torch.float64 or not frequencies.is_contiguous() or frequencies.numel() == 0:
+    if frequencies.dim() != 1 or frequencies.dtype != torch.float64 or not frequencies.is_contiguous():
         raise _lib.AdkError("rotary: frequencies is a contiguous float64 vector, one entry a pair")
     if positions.dtype != torch.int64:
         raise _lib.AdkError(f"rotary: positions are int64; got {positions.dtype}")
-    if positions.dim() == 3:
-        p = positions
-    elif positions.dim() in (1, 2):
-        p = positions.unsqueeze(-1)
+    pshape, pstride = positions.shape, positions.stride()
+    if len(pshape) == 3:
+        (pB, pN, axes), (pb, pn, pa) = pshape, pstride
+    elif len(pshape) == 2:
+        (pB, pN), (pb, pn), axes, pa = pshape, pstride, 1, 0
+    elif len(pshape) == 1:
+        pB, pN, axes, pb, pn, pa = 1, pshape[0], 1, 0, pstride[0], 0
     else:
         raise _lib.AdkError("rotary: positions [N], [B,N] or [B,N,axes]")
-    axes = p.shape[-1]
-    if tuple(p.shape[-3:-1]) not in ((B, N), (1, N), (N,)) or axes < 1:
-        raise _lib.AdkError(f"rotary: positions of shape {tuple(positions.shape)} do not fit x {tuple(x.shape)}")
-    if 2 * axes * frequencies.numel() > D:
-        raise _lib.AdkError(f"rotary: {axes} axes of {frequencies.numel()} pairs do not fit heads of {D}")
-    heads = H if heads is None else heads
-    if not 0 <= heads <= H:
+    if pN != N or (pB != B and pB != 1) or axes < 1:
+        raise _lib.AdkError(f"rotary: positions of shape {tuple(pshape)} do not fit x {tuple(shape)}")
+    if pB == 1:
+        pb = 0
+    pairs = frequencies.shape[0]
+    if pairs < 1 or 2 * axes * pairs > D:
+        raise _lib.AdkError(f"rotary: {axes} axes of {pairs} pairs do not fit heads of {D}")
+    if heads is None:
+        heads = H
+    elif not 0 <= heads <= H:
         raise _lib.AdkError(f"rotary: {heads} of {H} heads to turn")
-    device = x.device
     if device != positions.device or device != frequencies.device:
         raise _lib.AdkError("rotary: all tensors are on one device")
-    _lib.require_cuda(x)
-    pb, pn, pa = p.stride()[-3:] if p.dim() == 3 else (0, *p.stride())
-    if p.dim() == 3 and p.shape[0] == 1:
-        pb = 0
-    held = array("q", (*_strides(x), *_strides(y), pb, pn, pa))  # alive until the call returns
+    if y is not None and ((xb == 0 and B > 1) or (xn == 0 and N > 1) or (xh == 0 and H > 1)):
+        raise _lib.AdkError("rotary_: x has elements that share their place")
+    if not x.is_cuda:
+        _lib.require_cuda(x)
+    # a dimension of one element has no stride that matters
+    xb, xn, xh = xb if B > 1 else 0, xn if N > 1 else 0, xh if H > 1 else 0
+    if y is None:
+        y = torch.empty(shape, dtype=dtype, device=device)
+        held = array("q", (xb, xn, xh, N * H * D, H * D, D, pb, pn, pa))  # alive until the call returns
+    else:
+        held = array("q", (xb, xn, xh, xb, xn, xh, pb, pn, pa))
     lib = _lib.load()
     with _lib.on_device(device):
-        rc = lib.adk_rotary(x.data_ptr(), y.data_ptr(), positions.data_ptr(), frequencies.data_ptr(), _DTYPES[x.dtype], B, N, H, D, heads, frequencies.numel(),
-                            axes, _LAYOUTS[layout], transpose, factor, held.buffer_info()[0], _lib.stream_of(x))
+        rc = lib.adk_rotary(x.data_ptr(), y.data_ptr(), positions.data_ptr(), frequencies.data_ptr(), _DTYPES[dtype], B, N, H, D, heads, pairs, axes,
+                            _LAYOUTS[layout], transpose, factor, held.buffer_info()[0], _lib.raw_stream(device))
     _lib.check(rc, "adk_rotary")
     return y
 
 
-def _strides(t):
-    """Element strides of (batch, token, head); a dimension of one element has none that matters."""
-    a, b, c = t.shape[:3]
-    x, y, z, _ = t.stride()
-    return (x if a > 1 else 0, y if b > 1 else 0, z if c > 1 else 0)
-
-
 def _recorded(x):
     return torch.is_grad_enabled() and x.requires_grad
-
-
-def _new(x, positions, frequencies, factor, layout, heads, transpose):
-    if x.dim() != 4 or x.dtype not in _DTYPES:
-        raise _lib.AdkError(f"rotary: x [B,N,H,D] is required, float16, bfloat16 and float32 are supported; got {tuple(x.shape)} {x.dtype}")
-    return _turn(x, torch.empty(x.shape, dtype=x.dtype, device=x.device), positions, frequencies, factor, layout, heads, transpose)
 
 
 class _Rotary(torch.autograd.Function):
@@ -121,7 +120,7 @@ class _Rotary(torch.autograd.Function):
         if inplace:
             ctx.mark_dirty(x)
             return _turn(x, x, positions, frequencies, factor, layout, heads, transpose)
-        return _new(x, positions, frequencies, factor, layout, heads, transpose)
+        return _turn(x, None, positions, frequencies, factor, layout, heads, transpose)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -130,7 +129,7 @@ class _Rotary(torch.autograd.Function):
         factor, layout, heads, transpose = ctx.how
         if grad.shape[-1] > 1 and grad.stride(-1) != 1:
             grad = grad.contiguous()
-        grad = _new(grad, positions, frequencies, factor, layout, heads, not transpose)
+        grad = _turn(grad, None, positions, frequencies, factor, layout, heads, not transpose)
         return (grad,) + (None,) * 7
 
 
@@ -138,7 +137,7 @@ def rotary(x, positions, frequencies, *, factor=1.0, layout="half", heads=None) 
     """x [B,N,H,D] (float16, bfloat16 or float32, dense last dimension) with the first `heads` heads (all if None) turned, as a new
     contiguous tensor; the other channels and heads are copied.  positions int64 [N], [B,N] or [B,N,axes].  Differentiable."""
     if not _recorded(x):
-        return _new(x, positions, frequencies, factor, layout, heads, False)
+        return _turn(x, None, positions, frequencies, factor, layout, heads, False)
     return _Rotary.apply(x, positions, frequencies, factor, layout, heads, False, False)
 
 
@@ -150,5 +149,5 @@ def rotary_(x, positions, frequencies, *, factor=1.0, layout="half", heads=None)
 def rotary_transpose(x, positions, frequencies, *, factor=1.0, layout="half", heads=None) -> torch.Tensor:
     """The transpose of rotary, which is the gradient's form: the same pairs turned back, times factor."""
     if not _recorded(x):
-        return _new(x, positions, frequencies, factor, layout, heads, True)
+        return _turn(x, None, positions, frequencies, factor, layout, heads, True)
     return _Rotary.apply(x, positions, frequencies, factor, layout, heads, True, False)
