@@ -107,7 +107,8 @@ template <typename T, int KIND, bool E4M3, bool GATED>
 __global__ __launch_bounds__(256) void a8_fwd_kernel(const T* __restrict__ x, int64_t n, int64_t width, T* __restrict__ y, uint8_t* __restrict__ codes,
                                                      uint8_t* __restrict__ units)
 {
-    const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8;
+    // neighbouring chunks on one XCD: a gate chunk reads the up values that its neighbours a row half further on have just brought to its L2
+    const int64_t i = ((int64_t)xcd_remap(blockIdx.x, gridDim.x) * 256 + threadIdx.x) * 8;
     float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     const bool whole = i + 8 <= n;
     if (whole) a8_load(x + i, v);
