@@ -208,7 +208,11 @@ class _Attend(torch.autograd.Function):
 
 
 def attend(q, k, v, *, scale=None, causal=False, mask=None, key_lengths=None) -> torch.Tensor:
-    """attend_forward's out as part of autograd: differentiable once with respect to q, k and v.  -> [B,Nq,H*D]."""
+    """attend_forward's out as part of autograd: differentiable once with respect to q, k and v.  -> [B,Nq,H*D].
+
+    A training step that is captured into a graph is captured whole, while no graph of the same leaves recorded outside it is alive
+    (autograd would wait for the stream that one was recorded on, which ends the capture); attend_forward and attend_backward have no
+    such tie."""
     if not (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)):
         return attend_forward(q, k, v, scale=scale, causal=causal, mask=mask, key_lengths=key_lengths)[0]
     return _Attend.apply(q, k, v, scale, causal, mask, key_lengths)

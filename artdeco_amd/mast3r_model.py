@@ -23,7 +23,8 @@ where the library flash kernel launches 96 workgroups), otherwise on torch's fus
 N x N softmax of blocks.py:105-109 is never materialised; RoPE runs on the HIP
 `curope.rope_2d` kernel when the tensors are on the GPU (pure-torch rotation otherwise, pos_embed.py:112-158);
 GEMMs are hipBLASLt (bf16/fp16 under autocast, fp32 otherwise).  Heads run in fp32 like the reference
-(model.py:205).  Inference only (the frontend never trains).
+(model.py:205).  ARTDECO's frontend never trains; for fine-tuning the trunk, to_training_dtype() puts the blocks on the
+differentiable kernels (csrc/attend.hip, csrc/rotary.hip, csrc/activation8.hip) and training_forward() is forward() with a graph.
 """
 from __future__ import annotations
 
@@ -42,6 +43,14 @@ class RoPE2D(nn.Module):
     def __init__(self, freq=100.0, F0=1.0):
         super().__init__()
         self.base, self.F0 = freq, F0
+
+    def frequencies(self, D, device):
+        """The rotation's angles per position for heads of D, as artdeco_amd.rotary takes them."""
+        held = getattr(self, "_frequencies", None)
+        if held is None or held.numel() != D // 4 or held.device != device:
+            from artdeco_amd.rotary import rotary_frequencies
+            held = self._frequencies = rotary_frequencies(D, axes=2, base=self.base, device=device)[0] * self.F0
+        return held
 
     def forward(self, tokens, positions):
         """tokens [B,heads,N,D] (any strides with (N? ,D) dense per head as produced below), positions [B,N,2]."""
@@ -92,7 +101,14 @@ def _attend(q, k, v):
     return x.transpose(1, 2).reshape(B, N, H * D)
 
 
+def _trains(module, x) -> bool:
+    """Whether a module that to_training_dtype() has set up is called for a gradient on the GPU."""
+    return getattr(module, "trains", False) and torch.is_grad_enabled() and x.is_cuda
+
+
 class Mlp(nn.Module):
+    kept8 = None   # "int8" / "e4m3": the hidden values are kept for the backward pass in 8 bits (to_training_dtype)
+
     def __init__(self, in_features, hidden_features=None, out_features=None):
         super().__init__()
         self.fc1 = nn.Linear(in_features, hidden_features or in_features)
@@ -100,6 +116,9 @@ class Mlp(nn.Module):
         self.fc2 = nn.Linear(hidden_features or in_features, out_features or in_features)
 
     def forward(self, x):
+        if self.kept8 is not None and _trains(self, x):
+            from artdeco_amd.activation8 import mlp8
+            return mlp8(x.to(self.fc1.weight.dtype), self.fc1.weight, self.fc1.bias, self.fc2.weight, self.fc2.bias, format=self.kept8)
         return self.fc2(self.act(self.fc1(x.to(self.fc1.weight.dtype))))
 
 
@@ -113,6 +132,12 @@ class Attention(nn.Module):
 
     def forward(self, x, xpos):
         B, N, C = x.shape
+        if _trains(self, x):
+            from artdeco_amd import attention, rotary
+            H, D = self.num_heads, C // self.num_heads
+            qkv = self.qkv(x.to(self.qkv.weight.dtype)).view(B, N, 3 * H, D)
+            qkv = rotary.rotary_(qkv, xpos, self.rope.frequencies(D, x.device), heads=2 * H)   # q's and k's heads, v's stay
+            return self.proj(attention.attend_packed(qkv, H))
         qkv5 = self.qkv(x.to(self.qkv.weight.dtype)).reshape(B, N, 3, self.num_heads, C // self.num_heads)
         # q and k are adjacent [H,D] slabs of every token: rotate both with ONE in-place rope launch over 2H "heads"
         if not self.rope.rotate_qk_inplace(qkv5, xpos):
@@ -149,6 +174,13 @@ class CrossAttention(nn.Module):
         H, D = self.num_heads, C // self.num_heads
         wd = self.projq.weight.dtype
         query, key, value = query.to(wd), key.to(wd), value.to(wd)
+        if _trains(self, query):
+            from artdeco_amd import attention, rotary
+            f = self.rope.frequencies(D, query.device)
+            q = rotary.rotary_(self.projq(query).view(B, Nq, H, D), qpos, f).transpose(1, 2)
+            k = rotary.rotary_(self.projk(key).view(B, key.shape[1], H, D), kpos, f).transpose(1, 2)
+            v = self.projv(value).view(B, value.shape[1], H, D).transpose(1, 2)
+            return self.proj(attention.attend(q, k, v))
         q = self.projq(query).reshape(B, Nq, H, D).permute(0, 2, 1, 3)
         if key is value and not torch.is_grad_enabled() and key.is_cuda:
             # the decoder passes the same normalised memory as key and value (blocks.py:188): ONE GEMM against the stacked
@@ -406,6 +438,8 @@ class AsymmetricMASt3R(nn.Module):
         """TF32-class mode on the GPU: residual add + LayerNorm + operand cast run as one HIP launch per sub-layer
         (ADK_MAST3R_FUSED_NORM=0 keeps the three torch kernels, for A/B measurements and the equivalence test)."""
         import os
+        if getattr(self, "_training_ops", False):   # that launch has no gradient
+            return False
         C = x.shape[-1]   # what adk_add_layernorm takes (fused_norm.supported); anything else keeps the torch kernels
         return bool(getattr(self, "_fp32_stream", False) and x.is_cuda and self.patch_embed.proj.weight.dtype == torch.float16
                     and C % 4 == 0 and C <= 2048 and os.environ.get("ADK_MAST3R_FUSED_NORM", "1") != "0")
@@ -492,8 +526,8 @@ class AsymmetricMASt3R(nn.Module):
     def _side_stream(self, t):
         """Second HIP stream for the independent halves of the decoder / the two heads (GPU only; ADK_MAST3R_STREAMS=0 disables)."""
         import os
-        if not t.is_cuda or os.environ.get("ADK_MAST3R_STREAMS", "1") == "0":
-            return None
+        if not t.is_cuda or os.environ.get("ADK_MAST3R_STREAMS", "1") == "0" or getattr(self, "_training_ops", False):
+            return None   # (training: what the graph keeps is freed in the order of one stream)
         st = getattr(self, "_side", None)
         if st is None or st.device != t.device:
             st = self._side = torch.cuda.Stream(device=t.device)
@@ -521,6 +555,32 @@ class AsymmetricMASt3R(nn.Module):
             v.record_stream(main)
         return res1, res2
 
+    def _trunk(self):
+        return (self.patch_embed, self.enc_blocks, self.enc_norm, self.decoder_embed, self.dec_blocks, self.dec_blocks2, self.dec_norm)
+
+    def _set_training_ops(self, on, kept8=None):
+        self._training_ops = on
+        for root in (self.enc_blocks, self.dec_blocks, self.dec_blocks2):
+            for m in root.modules():
+                if isinstance(m, (Attention, CrossAttention, Mlp)):
+                    m.trains = on
+                if isinstance(m, Mlp):
+                    m.kept8 = kept8
+
+    def to_training_dtype(self, dtype, kept8=None):
+        """For fine-tuning: the trunk's Linear and patch-embedding weights in `dtype` (float16 or bfloat16), products accumulated in
+        fp32, residual stream, LayerNorms and softmax in fp32 as to_inference_dtype(fp32_stream=True) has them, and the blocks'
+        attention, rotary positions and MLPs on kernels with a gradient.  kept8 ("int8" / "e4m3"): the MLPs keep their hidden values in 8
+        bits for the backward pass.  The heads stay fp32.  training_forward() then gives results with a graph; forward() stays
+        without."""
+        if dtype not in (torch.float16, torch.bfloat16):
+            raise ValueError(f"to_training_dtype: float16 or bfloat16; got {dtype}")
+        if kept8 not in (None, "int8", "e4m3"):
+            raise ValueError(f"to_training_dtype: kept8 is None, int8 or e4m3; got {kept8!r}")
+        self.to_inference_dtype(dtype, fp32_stream=True)
+        self._set_training_ops(True, kept8)
+        return self
+
     def to_inference_dtype(self, dtype, fp32_stream=False, heads=False):
         """Cast encoder + decoders ONCE to bf16/fp16 (autocast would re-cast every weight on every call);
         the heads stay fp32 like the reference (dust3r/model.py:205).
@@ -530,7 +590,8 @@ class AsymmetricMASt3R(nn.Module):
         fp32 on the matrix cores and the residual stream, every LayerNorm and the attention softmax stay fp32.  The
         reference runs the model under `torch.backends.cuda.matmul.allow_tf32 = True` (run_system.py:73), i.e. with
         10-bit GEMM operands; tools/frontend_precision.py measures this mode against an emulated TF32 forward."""
-        trunk = (self.patch_embed, self.enc_blocks, self.enc_norm, self.decoder_embed, self.dec_blocks, self.dec_blocks2, self.dec_norm)
+        trunk = self._trunk()
+        self._set_training_ops(False)
         if not fp32_stream:
             for m in trunk:
                 m.to(dtype)
@@ -569,6 +630,13 @@ class AsymmetricMASt3R(nn.Module):
 
     @torch.inference_mode()
     def forward(self, view1, view2):
+        return self._both_views(view1, view2)
+
+    def training_forward(self, view1, view2):
+        """forward() under the caller's grad mode."""
+        return self._both_views(view1, view2)
+
+    def _both_views(self, view1, view2):
         img1, img2 = view1["img"], view2["img"]
         td = getattr(self, "_trunk_dtype", None)
         if td is not None:
