@@ -117,19 +117,25 @@ class _Mlp8(torch.autograd.Function):
     def forward(ctx, x, w1, b1, w2, b2, kind, gated, format):
         y, packed = activation8_forward(F.linear(x, w1, b1), kind=kind, gated=gated, format=format)
         ctx.save_for_backward(x, w1, w2, packed.codes, packed.units)
-        ctx.how = (packed.shape, packed.dtype, format, kind, gated, b1 is not None, b2 is not None)
+        ctx.how = (packed.shape, packed.dtype, format, kind, gated)
         return F.linear(y, w2, b2)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
         x, w1, w2, codes, units = ctx.saved_tensors
-        shape, dtype, format, kind, gated, has1, has2 = ctx.how
+        shape, dtype, format, kind, gated = ctx.how
+        nx, nw1, nb1, nw2, nb2 = ctx.needs_input_grad[:5]
         g2 = grad.reshape(-1, grad.shape[-1])
-        dh, y = activation8_backward(torch.mm(g2, w2).view(*shape[:-1], w2.shape[1]), Packed8(codes, units, shape, dtype, format), kind=kind, gated=gated)
-        dh, y, x2 = dh.view(-1, dh.shape[-1]), y.view(-1, y.shape[-1]), x.reshape(-1, x.shape[-1])
-        return (torch.mm(dh, w1).view(x.shape), torch.mm(dh.t(), x2), dh.sum(0) if has1 else None, torch.mm(g2.t(), y), g2.sum(0) if has2 else None,
-                None, None, None)
+        dx = dw1 = db1 = dw2 = None
+        if nx or nw1 or nb1 or nw2:
+            dh, y = activation8_backward(torch.mm(g2, w2).view(*shape[:-1], w2.shape[1]), Packed8(codes, units, shape, dtype, format), kind=kind, gated=gated, again=nw2)
+            dh = dh.view(-1, dh.shape[-1])
+            dx = torch.mm(dh, w1).view(x.shape) if nx else None
+            dw1 = torch.mm(dh.t(), x.reshape(-1, x.shape[-1])) if nw1 else None
+            db1 = dh.sum(0) if nb1 else None
+            dw2 = torch.mm(g2.t(), y.view(-1, y.shape[-1])) if nw2 else None
+        return dx, dw1, db1, dw2, g2.sum(0) if nb2 else None, None, None, None
 
 
 def mlp8(x, w1, b1, w2, b2, *, kind="gelu", gated=False, format="int8") -> torch.Tensor:

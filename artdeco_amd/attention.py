@@ -75,8 +75,8 @@ def _prepare(what, q, k, v, scale, mask, key_lengths):
         qs, ks, vs = _strides(q), _strides(k), _strides(v)
     if scale is None:
         scale = D ** -0.5
-    elif not 0.0 < scale < math.inf:
-        raise _lib.AdkError(f"{what}: scale is a positive number; got {scale}")
+    elif not 0.0 < scale < 1e37:
+        raise _lib.AdkError(f"{what}: scale is a positive number below 1e37; got {scale}")
     if key_lengths is not None and (key_lengths.dtype != torch.int32 or key_lengths.shape != (B,) or not key_lengths.is_contiguous() or key_lengths.device != q.device):
         raise _lib.AdkError(f"{what}: key_lengths is a contiguous int32 tensor of the batch's size on q's device")
     if mask is None:
@@ -130,7 +130,7 @@ def attend_forward(q, k, v, *, scale=None, causal=False, mask=None, key_lengths=
     key_lengths  int32 [B]: sequence b has keys below key_lengths[b] (clamped to 0 .. Nk).  What lies behind is never read.
     mask         bool, broadcastable to [B,H,Nq,Nk], True where a query sees a key; what it hides from a query has to hold finite
                  numbers, unless the mask is the same for all queries and heads.
-    All three hold together.  A query that sees no key gives zeros and lse = -inf."""
+    All three hold together.  A query that sees no key gives zeros and lse = -inf; the queries of a padded sequence are all computed."""
     scale, mask, strides = _prepare("attend_forward", q, k, v, scale, mask, key_lengths)
     B, H, Nq, D = q.shape
     Hk, Nk = k.shape[1], k.shape[2]

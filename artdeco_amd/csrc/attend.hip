@@ -904,7 +904,7 @@ static int at_check(int dtype, int B, int H, int Hk, int Nq, int Nk, int D, floa
     if (dtype != 0 && dtype != 2) return ADK_EUNSUPPORTED;
     if (B < 0 || H < 1 || Hk < 1 || H % Hk || Nq < 0 || Nk < 0) return ADK_EINVAL;
     if (D < 8 || D > 128 || (D & 7)) return ADK_EUNSUPPORTED;
-    if (!(scale > 0.f) || !(scale < INFINITY)) return ADK_EINVAL;
+    if (!(scale > 0.f) || !(scale < 1e37f)) return ADK_EINVAL; // and scale log2 e a number
     const int64_t R = (int64_t)(H / Hk) * Nq; // row and key numbers, and a grid, in 31 bits
     if (R > 0x7fffff00ll || Nk > 0x7fffff00 || (int64_t)B * Hk * ceil_div(R + Nk, 32) > 0xffffff) return ADK_EUNSUPPORTED;
     if ((int64_t)B * H * Nq > 0x7fffff00ll * 8) return ADK_EUNSUPPORTED;

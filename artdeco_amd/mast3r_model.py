@@ -46,11 +46,11 @@ class RoPE2D(nn.Module):
 
     def frequencies(self, D, device):
         """The rotation's angles per position for heads of D, as artdeco_amd.rotary takes them."""
-        held = getattr(self, "_frequencies", None)
-        if held is None or held.numel() != D // 4 or held.device != device:
+        held = self.__dict__.setdefault("_frequencies", {})
+        if (D, device) not in held:
             from artdeco_amd.rotary import rotary_frequencies
-            held = self._frequencies = rotary_frequencies(D, axes=2, base=self.base, device=device)[0] * self.F0
-        return held
+            held[D, device] = rotary_frequencies(D, axes=2, base=self.base, device=device)[0] * self.F0
+        return held[D, device]
 
     def forward(self, tokens, positions):
         """tokens [B,heads,N,D] (any strides with (N? ,D) dense per head as produced below), positions [B,N,2]."""

@@ -143,6 +143,8 @@ def rotary(x, positions, frequencies, *, factor=1.0, layout="half", heads=None) 
 
 def rotary_(x, positions, frequencies, *, factor=1.0, layout="half", heads=None) -> torch.Tensor:
     """rotary in place: what is not turned is not touched.  -> x."""
+    if _recorded(x) and x.is_leaf:
+        raise _lib.AdkError("rotary_: x is a leaf that requires a gradient: turn it out of place, with rotary")
     return _Rotary.apply(x, positions, frequencies, factor, layout, heads, False, True)
 
 

@@ -226,6 +226,25 @@ def test_layouts_and_strides(dev):
 
 
 @pytest.mark.gpu
+def test_offsets_past_32_bits(dev):
+    """A cache whose tokens lie 2 MiB apart: 8 GiB from the first key to the last, queries likewise; and one whose mask does."""
+    room = torch.empty(4200 * 2 ** 20 // 2 * 2, dtype=torch.bfloat16, device=dev)
+    q, k, v, do = inputs(1, 4, 2, 3000, 4100, 64, torch.bfloat16, dev, seed=33)
+    far_k, far_v = (room[o:].as_strided((1, 2, 4100, 64), (8, 64, 2 ** 20, 1)) for o in (0, 256))
+    far_q = room[512:].as_strided((1, 4, 3000, 64), (8, 64, 2 ** 20, 1))
+    for a, b in ((far_k, k), (far_v, v), (far_q, q)):
+        a.copy_(b)
+    want = both(q, k, v, do, causal=True)
+    got = both(far_q, far_k, far_v, do, causal=True)
+    assert all(torch.equal(got[n], want[n]) for n in want)
+    mask = torch.rand(1, 1, 3000, 4100, device=dev) < 0.7
+    far_mask = room.view(torch.bool).as_strided((1, 1, 3000, 4100), (1, 1, 2 ** 21 + 2 ** 19, 1))
+    far_mask.copy_(mask)
+    want, got = both(q, k, v, do, mask=mask), both(q, k, v, do, mask=far_mask)
+    assert all(torch.equal(got[n], want[n]) for n in want)
+
+
+@pytest.mark.gpu
 def test_attend_in_autograd(dev):
     """The differentiable forms give attend_backward's gradients: leaves, an expanded incoming gradient, one packed projection, a broadcast
     key tensor whose gradient is summed; twice the same bits; no second derivative."""
@@ -350,6 +369,8 @@ def test_c_entry_refuses_before_any_launch(lib):
     fwd = lambda q=P, D=64, H=4, Hk=2, Nq=4, dtype=0, s=fine, scale=1.0, out=P, ws=None, n=0: lib.adk_attend_fwd(  # noqa: E731
         q, P, P, out, P, None, None, dtype, 1, H, Hk, Nq, 4096, D, s, scale, 0, ws, n, None)
     assert fwd(D=60) == -3 and fwd(D=256) == -3 and fwd(dtype=1) == -3
+    wide = (ctypes.c_int64 * 25)(8, 8, 1 << 24, *[8] * 22)
+    assert fwd(s=wide) == -3 and fwd(scale=1e38) == -1
     assert fwd(H=3) == -1 and fwd(scale=0.0) == -1 and fwd(scale=float("nan")) == -1 and fwd(q=None) == -1 and fwd(s=odd) == -1 and fwd(out=None) == -1
     assert fwd(q=ctypes.c_void_p((1 << 20) + 8)) == -1
     assert fwd() == -2 and fwd(ws=P, n=64) == -2

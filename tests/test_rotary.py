@@ -61,7 +61,8 @@ def test_turns_and_turns_back(case, layout, dtype, dev):
     check(ro.rotary_transpose(x, pos, f, **how), x, pos, f, factor, layout, heads, -1)
     assert torch.equal(x, keep)
     y = x.clone()
-    assert ro.rotary_(y, pos, f, **how) is y and torch.equal(y, ro.rotary(x, pos, f, **how))
+    version = y._version
+    assert ro.rotary_(y, pos, f, **how) is y and torch.equal(y, ro.rotary(x, pos, f, **how)) and y._version > version
 
 
 @pytest.mark.gpu
@@ -194,6 +195,8 @@ def test_refusals(lib):
     no("to turn", x, pos, f, heads=4)
     with pytest.raises(_lib.AdkError, match="share"):
         ro.rotary_(torch.zeros(1, 4, 3, 16).expand(2, 4, 3, 16), pos, f)
+    with pytest.raises(_lib.AdkError, match="leaf"):
+        ro.rotary_(torch.zeros(2, 4, 3, 16, requires_grad=True), pos, f)
     N = None
     assert lib.adk_rotary(N, N, N, N, 0, 1, 1, 1, 16, 1, 9, 1, 1, 0, 1.0, N, N) == -1      # 18 channels of 16
     assert lib.adk_rotary(N, N, N, N, 3, 1, 1, 1, 16, 1, 8, 1, 1, 0, 1.0, N, N) == -3
