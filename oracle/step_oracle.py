@@ -351,7 +351,8 @@ def _run(fn, chunks, workers, prefix):
 
 
 def default_workers():
-    return max(1, min(len(os.sched_getaffinity(0)) if hasattr(os, "sched_getaffinity") else (os.cpu_count() or 1), 96))
+    # 14: a worker opens the GPU when it imports torch, and machines that bound the processes on a card do so at 16
+    return max(1, min(len(os.sched_getaffinity(0)) if hasattr(os, "sched_getaffinity") else (os.cpu_count() or 1), 14))
 
 
 # ----------------------------------------------------------------------------- the step
