@@ -76,6 +76,7 @@ template <bool NARROW> struct AtShape {
 };
 
 template <int DP> __device__ __forceinline__ int at_swz(int row) {
+    if (DP == 96) return (row >> 2) & 3; // rows of 192 bytes: 4 of them lie on different quarters of the 64 banks as they are
     return DP == 64 ? ((((row >> 1) & 1) << 2) | ((row >> 2) & 3)) : (((row & 3) << 2) | ((row >> 2) & 3));
 }
 template <int DP> __device__ __forceinline__ int at_off(int row, int chunk) { return row * DP + ((chunk ^ at_swz<DP>(row)) << 3); }
@@ -131,7 +132,7 @@ template <typename T, int DP, bool NARROW> struct AtTile {
         const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)tile;
 #pragma unroll
         for (int i = 0; i < IT; ++i) {
-            const int row = (WAVES * i + wave) * (64 / CH) + lane / CH, chunk = (lane % CH) ^ at_swz<DP>(row);
+            const int at = (WAVES * i + wave) * 64 + lane, row = at / CH, chunk = (at % CH) ^ at_swz<DP>(row);
             const uint32_t off = (uint32_t)min(row, rows - 1) * (uint32_t)sn * 2u + chunk * 16;
             if (DP == D || chunk * 8 < D) at_lds16(lds + (WAVES * i + wave) * 1024, base, off);
         }
@@ -141,7 +142,7 @@ template <typename T, int DP, bool NARROW> struct AtTile {
         const int wave = NARROW ? 0 : threadIdx.x >> 6, lane = threadIdx.x & 63;
 #pragma unroll
         for (int i = 0; i < IT; ++i) {
-            const int row = (WAVES * i + wave) * (64 / CH) + lane / CH;
+            const int row = ((WAVES * i + wave) * 64 + lane) / CH;
             if (!mask[(int64_t)min(row, rows - 1) * sk]) *reinterpret_cast<at_u32x4*>(tile + (WAVES * i + wave) * 512 + lane * 8) = at_u32x4{0, 0, 0, 0};
         }
     }
@@ -856,7 +857,7 @@ template <typename T, int DP, bool MASKED, bool NARROW> __device__ __forceinline
 
 // PART 1: the rows' workgroups, 2: the keys', 3: both in one launch, the keys' first (they are the longer ones).
 template <typename T, int DP, bool MASKED, bool NARROW, int PART>
-__global__ __launch_bounds__(256, DP == 128 && (PART > 1 || NARROW) ? 1 : 2) void at_bwd_kernel(AttendArgs a)
+__global__ __launch_bounds__(256, (DP == 128 && PART > 1) || (DP > 64 && NARROW) || (DP == 96 && MASKED && PART > 1) ? 1 : 2) void at_bwd_kernel(AttendArgs a)
 {
     union Shared {
         AtShared<T, DP, NARROW> rows;
@@ -946,6 +947,7 @@ template <typename T, int DP, bool MASKED> static void at_launch_bwd(const Atten
 
 template <typename T> static int at_fwd(const AttendArgs& a, hipStream_t stream) {
     if (a.D <= 64) { if (a.mask) at_launch_fwd<T, 64, true>(a, stream); else at_launch_fwd<T, 64, false>(a, stream); }
+    else if (a.D <= 96) { if (a.mask) at_launch_fwd<T, 96, true>(a, stream); else at_launch_fwd<T, 96, false>(a, stream); }
     else { if (a.mask) at_launch_fwd<T, 128, true>(a, stream); else at_launch_fwd<T, 128, false>(a, stream); }
     if (a.splits > 1) hipLaunchKernelGGL((at_join_kernel<T>), dim3((unsigned)ceil_div((int64_t)a.B * a.H * a.Nq, 8)), dim3(256), 0, stream, a);
     ADK_RETURN_LAST_ERROR();
@@ -955,6 +957,7 @@ template <typename T> static int at_bwd(const AttendArgs& a, hipStream_t stream)
     const int64_t rows = (int64_t)a.B * a.H * a.Nq;
     if (rows) hipLaunchKernelGGL((at_delta_kernel<T>), dim3((unsigned)ceil_div(rows, AT_DELTA_ROWS)), dim3(256), 0, stream, a);
     if (a.D <= 64) { if (a.mask) at_launch_bwd<T, 64, true>(a, stream); else at_launch_bwd<T, 64, false>(a, stream); }
+    else if (a.D <= 96) { if (a.mask) at_launch_bwd<T, 96, true>(a, stream); else at_launch_bwd<T, 96, false>(a, stream); }
     else { if (a.mask) at_launch_bwd<T, 128, true>(a, stream); else at_launch_bwd<T, 128, false>(a, stream); }
     ADK_RETURN_LAST_ERROR();
 }
