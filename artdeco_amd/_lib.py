@@ -161,6 +161,20 @@ class on_device:
         return False
 
 
+def launch(fn, what: str, device, *args) -> None:
+    """fn(*args, stream) on torch's current stream of `device` (a tensor's device: it has an index), with that device current, and check().
+    One call for what on_device, stream_of and check do in three, at a third of their cost."""
+    import torch
+    idx = device.index
+    if idx == torch._C._cuda_getDevice():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(idx))
+    else:
+        with torch.cuda.device(idx):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(idx))
+    if rc:
+        check(rc, what)
+
+
 def require_cuda(*tensors) -> None:
     for t in tensors:
         if t is not None and not t.is_cuda:

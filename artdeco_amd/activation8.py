@@ -57,11 +57,8 @@ def activation8_forward(x, *, kind="gelu", gated=False, format="int8"):
     y = torch.empty((*shape[:-1], width), dtype=dtype, device=device)
     codes = torch.empty(32 * blocks, dtype=torch.uint8, device=device)
     units = torch.empty(blocks, dtype=torch.uint8, device=device)
-    lib = _lib.load()
-    with _lib.on_device(device):
-        rc = lib.adk_activation8_fwd(x.data_ptr(), _DTYPES[dtype], rows, width, _KINDS[kind], gated, _FORMATS[format], y.data_ptr(), codes.data_ptr(),
-                                     units.data_ptr(), _lib.raw_stream(device))
-    _lib.check(rc, "adk_activation8_fwd")
+    _lib.launch(_lib.load().adk_activation8_fwd, "adk_activation8_fwd", device, x.data_ptr(), _DTYPES[dtype], rows, width, _KINDS[kind], gated, _FORMATS[format],
+                y.data_ptr(), codes.data_ptr(), units.data_ptr())
     return y, Packed8(codes, units, shape, dtype, format)
 
 
@@ -83,11 +80,8 @@ def activation8_backward(grad, packed, *, kind="gelu", gated=False, again=True):
     grad = grad.contiguous()
     dx = torch.empty(pshape, dtype=dtype, device=device)
     y = torch.empty(shape, dtype=dtype, device=device) if again else None
-    lib = _lib.load()
-    with _lib.on_device(device):
-        rc = lib.adk_activation8_bwd(grad.data_ptr(), codes.data_ptr(), units.data_ptr(), _DTYPES[dtype], rows, width, _KINDS[kind], gated, _FORMATS[format],
-                                     dx.data_ptr(), _lib.ptr(y), _lib.raw_stream(device))
-    _lib.check(rc, "adk_activation8_bwd")
+    _lib.launch(_lib.load().adk_activation8_bwd, "adk_activation8_bwd", device, grad.data_ptr(), codes.data_ptr(), units.data_ptr(), _DTYPES[dtype], rows, width,
+                _KINDS[kind], gated, _FORMATS[format], dx.data_ptr(), _lib.ptr(y))
     return dx, y
 
 

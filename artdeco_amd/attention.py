@@ -117,8 +117,8 @@ def _refuse(what, q, k, v):
 def _workspace(nbytes, what, device):
     if nbytes <= 0:
         _lib.check(nbytes, what)
-        return None
-    return torch.empty(nbytes, dtype=torch.uint8, device=device)
+        return None, 0
+    return torch.empty(nbytes, dtype=torch.uint8, device=device), nbytes
 
 
 def attend_forward(q, k, v, *, scale=None, causal=False, mask=None, key_lengths=None):
@@ -139,11 +139,9 @@ def attend_forward(q, k, v, *, scale=None, causal=False, mask=None, key_lengths=
     out = torch.empty((B, Nq, H * D), dtype=dtype, device=device)
     lse = torch.empty((B, H, Nq), dtype=torch.float32, device=device)
     lib = _lib.load()
-    with _lib.on_device(device):
-        ws = _workspace(lib.adk_attend_fwd_workspace_bytes(B, H, Hk, Nq, Nk, D), "adk_attend_fwd", device)
-        rc = lib.adk_attend_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), _lib.ptr(key_lengths), _lib.ptr(mask), _DTYPES[dtype],
-                                B, H, Hk, Nq, Nk, D, held.buffer_info()[0], scale, causal, _lib.ptr(ws), 0 if ws is None else ws.numel(), _lib.raw_stream(device))
-    _lib.check(rc, "adk_attend_fwd")
+    ws, nbytes = _workspace(lib.adk_attend_fwd_workspace_bytes(B, H, Hk, Nq, Nk, D), "adk_attend_fwd", device)
+    _lib.launch(lib.adk_attend_fwd, "adk_attend_fwd", device, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), _lib.ptr(key_lengths),
+                _lib.ptr(mask), _DTYPES[dtype], B, H, Hk, Nq, Nk, D, held.buffer_info()[0], scale, causal, _lib.ptr(ws), nbytes)
     return out, lse
 
 
@@ -159,12 +157,10 @@ def _backward_into(grad_out, q, k, v, out, lse, scale, causal, mask, key_lengths
     device = q.device
     lib = _lib.load()
     held = array("q", (*strides, *g, *dq.stride()[:3], *dk.stride()[:3], *dv.stride()[:3]))
-    with _lib.on_device(device):
-        ws = _workspace(lib.adk_attend_bwd_workspace_bytes(B, H, Hk, Nq, Nk, D), "adk_attend_bwd", device)
-        rc = lib.adk_attend_bwd(grad_out.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), _lib.ptr(key_lengths), _lib.ptr(mask),
-                                _DTYPES[q.dtype], B, H, Hk, Nq, Nk, D, held.buffer_info()[0], scale, causal, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
-                                _lib.ptr(ws), 0 if ws is None else ws.numel(), _lib.raw_stream(device))
-    _lib.check(rc, "adk_attend_bwd")
+    ws, nbytes = _workspace(lib.adk_attend_bwd_workspace_bytes(B, H, Hk, Nq, Nk, D), "adk_attend_bwd", device)
+    _lib.launch(lib.adk_attend_bwd, "adk_attend_bwd", device, grad_out.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(),
+                _lib.ptr(key_lengths), _lib.ptr(mask), _DTYPES[q.dtype], B, H, Hk, Nq, Nk, D, held.buffer_info()[0], scale, causal, dq.data_ptr(), dk.data_ptr(),
+                dv.data_ptr(), _lib.ptr(ws), nbytes)
 
 
 def attend_backward(grad_out, q, k, v, out, lse, *, scale=None, causal=False, mask=None, key_lengths=None):

@@ -748,7 +748,7 @@ template <typename T, int DP, bool MASKED, bool NARROW> __device__ __forceinline
                 x8 qa[DP / 16], ga[DP / 16];
 #pragma unroll
                 for (int ks = 0; ks < DP / 16; ++ks) { qa[ks] = at_rowfrag<T, DP>(tq, 32 * n, ks, lane); ga[ks] = at_rowfrag<T, DP>(tg, 32 * n, ks, lane); }
-                if (DP == 128) __builtin_amdgcn_sched_barrier(0); // all reads under way before the first product
+                if (DP >= 96) __builtin_amdgcn_sched_barrier(0); // all reads under way before the first product
 #pragma unroll
                 for (int ks = 0; ks < DP / 16; ++ks) {
                     st[n] = AtEl<T>::mfma(qa[ks], kf[ks], st[n]);

@@ -100,11 +100,8 @@ def _turn(x, y, positions, frequencies, factor, layout, heads, transpose):
         held = array("q", (xb, xn, xh, N * H * D, H * D, D, pb, pn, pa))  # alive until the call returns
     else:
         held = array("q", (xb, xn, xh, xb, xn, xh, pb, pn, pa))
-    lib = _lib.load()
-    with _lib.on_device(device):
-        rc = lib.adk_rotary(x.data_ptr(), y.data_ptr(), positions.data_ptr(), frequencies.data_ptr(), _DTYPES[dtype], B, N, H, D, heads, pairs, axes,
-                            _LAYOUTS[layout], transpose, factor, held.buffer_info()[0], _lib.raw_stream(device))
-    _lib.check(rc, "adk_rotary")
+    _lib.launch(_lib.load().adk_rotary, "adk_rotary", device, x.data_ptr(), y.data_ptr(), positions.data_ptr(), frequencies.data_ptr(), _DTYPES[dtype], B, N, H, D,
+                heads, pairs, axes, _LAYOUTS[layout], transpose, factor, held.buffer_info()[0])
     return y
 
 
