@@ -19,9 +19,10 @@
 // e % 4, the order the accumulator has), and likewise S = Q K^T gives P, dS as B operands of dV^T = dO^T P, dK^T = Q^T dS.  The
 // transposed A operands come from row-major tiles through ds_read_b64_tr_b16.
 //
-// Two shapes.  Wide: a workgroup owns 128 rows (or keys), 32 a wave, and its four waves share tiles of 64 keys (or rows).  Narrow, for
+// Three shapes.  Wide: a workgroup owns 128 rows (or keys), 32 a wave, and its four waves share tiles of 64 keys (or rows).  Narrow, for
 // calls too small to fill the chip so: a workgroup owns 32, and each wave walks every fourth tile of 32 with LDS tiles of its own and
-// no barrier; the four partial results are joined through LDS at the end, in a fixed order.
+// no barrier; the four partial results are joined through LDS at the end, in a fixed order.  Half, for the backward pass between the two: it
+// owns 64, two waves share every second tile of 32, and two partial results are joined; its tiles are small enough for two workgroups a CU.
 //
 // LDS tiles hold 16-byte chunks at chunk ^ f(row): with f below, the 16 rows of a 128-bit fragment read and the 4 rows of a
 // transposing read fall on different banks without padding.
@@ -68,11 +69,12 @@ struct AttendArgs {
 };
 
 // A shape's numbers.
-template <bool NARROW> struct AtShape {
-    static constexpr int OWN = NARROW ? 32 : 128;   // rows (or keys) that a workgroup owns
-    static constexpr int TILE = NARROW ? 32 : 64;   // keys (or rows) of a staged tile
-    static constexpr int WAVES = NARROW ? 1 : 4;    // waves that share a tile
-    static constexpr int STREAMS = NARROW ? 4 : 1;  // tiles in work at once
+enum { AT_WIDE = 0, AT_NARROW = 1, AT_HALF = 2 };
+template <int SHAPE> struct AtShape {
+    static constexpr int WAVES = SHAPE == AT_WIDE ? 4 : SHAPE == AT_HALF ? 2 : 1; // waves that share a tile
+    static constexpr int STREAMS = 4 / WAVES;                                     // tiles in work at once
+    static constexpr int OWN = 32 * WAVES;                                        // rows (or keys) that a workgroup owns
+    static constexpr int TILE = SHAPE == AT_WIDE ? 64 : 32;                       // keys (or rows) of a staged tile
 };
 
 template <int DP> __device__ __forceinline__ int at_swz(int row) {
@@ -123,12 +125,12 @@ __device__ __forceinline__ void at_lds16(uint32_t lds, const void* base, uint32_
 // may take their place
 template <int later = 0> __device__ __forceinline__ void at_landed() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"i"(later) : "memory"); }
 
-template <typename T, int DP, bool NARROW> struct AtTile {
-    static constexpr int TILE = AtShape<NARROW>::TILE, WAVES = AtShape<NARROW>::WAVES, CH = DP / 8, IT = TILE * CH / (64 * WAVES);
+template <typename T, int DP, int SHAPE> struct AtTile {
+    static constexpr int TILE = AtShape<SHAPE>::TILE, WAVES = AtShape<SHAPE>::WAVES, CH = DP / 8, IT = TILE * CH / (64 * WAVES);
     // rows from base on; those past the `rows` (>= 1) that there are repeat the last (they are hidden in the scores, and what lies
     // there is never read); chunks past D are left as they are
     static __device__ __forceinline__ void load(T* tile, const T* base, int sn, int rows, int D) {
-        const int wave = NARROW ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % WAVES, lane = threadIdx.x & 63;
         const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)tile;
 #pragma unroll
         for (int i = 0; i < IT; ++i) {
@@ -139,7 +141,7 @@ template <typename T, int DP, bool NARROW> struct AtTile {
     }
     // a mask that is the same for every query hides a key altogether: zeros, whatever stands there (by the lanes that loaded it)
     static __device__ __forceinline__ void hide(T* tile, const uint8_t* mask, int64_t sk, int rows) {
-        const int wave = NARROW ? 0 : threadIdx.x >> 6, lane = threadIdx.x & 63;
+        const int wave = (threadIdx.x >> 6) % WAVES, lane = threadIdx.x & 63;
 #pragma unroll
         for (int i = 0; i < IT; ++i) {
             const int row = ((WAVES * i + wave) * 64 + lane) / CH;
@@ -149,7 +151,7 @@ template <typename T, int DP, bool NARROW> struct AtTile {
     // zeros in the chunks past D of the workgroup's tiles, which no load touches
     static __device__ __forceinline__ void pad(T* first, int bufs, int D) {
         if (D == DP) return;
-        for (int n = threadIdx.x; n < AtShape<NARROW>::STREAMS * 2 * bufs * TILE * CH; n += 256)
+        for (int n = threadIdx.x; n < AtShape<SHAPE>::STREAMS * 2 * bufs * TILE * CH; n += 256)
             if (((n % CH) ^ at_swz<DP>(n / CH % TILE)) * 8 >= D) *reinterpret_cast<at_u32x4*>(first + n * 8) = at_u32x4{0, 0, 0, 0};
         __syncthreads(); // narrow: a wave's tiles are its own from here on
     }
@@ -203,30 +205,33 @@ __device__ __forceinline__ uint32_t at_below_bits(int k0, int lim) {
 }
 
 // A workgroup's LDS.  Narrow: when the tiles are done with, their place takes the waves' partial results, 64 lanes a register.
-template <typename T, int DP, bool NARROW, int BUFS = 2> struct AtShared {
-    T tiles[AtShape<NARROW>::STREAMS][BUFS][2][AtShape<NARROW>::TILE * DP]; // stream, buffer, tensor
+template <typename T, int DP, int SHAPE, int BUFS = 2> struct AtShared {
+    T tiles[AtShape<SHAPE>::STREAMS][BUFS][2][AtShape<SHAPE>::TILE * DP]; // stream, buffer, tensor
     int tops[4];
     float unit4[4];
     float m[4][32], l[4][32];
 };
-template <typename T, int DP, bool NARROW> struct AtSharedKeys {
-    static constexpr int S = AtShape<NARROW>::STREAMS, TILE = AtShape<NARROW>::TILE;
+template <typename T, int DP, int SHAPE> struct AtSharedKeys {
+    static constexpr int S = AtShape<SHAPE>::STREAMS, TILE = AtShape<SHAPE>::TILE;
     T tiles[S][2][2][TILE * DP];
     float lse[S][2][TILE], delta[S][2][TILE];
     int lim[S][2][TILE];
     float unit4[4];
 };
 
-// Narrow: the sum of the four waves' `regs` values a lane; wave w gets the values w regs / 4 + 0 .. regs / 4 - 1.
-template <int REGS> __device__ __forceinline__ void at_sum_waves(const float* mine, float* room, float* sum) {
+// The sum of `regs` values a lane over the streams' waves that own the same rows (or keys); the wave of stream n gets the values
+// n regs / streams + 0 .. regs / streams - 1.
+template <int REGS, int SHAPE> __device__ __forceinline__ void at_sum_streams(const float* mine, float* room, float* sum) {
+    constexpr int WAVES = AtShape<SHAPE>::WAVES, STREAMS = AtShape<SHAPE>::STREAMS;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
 #pragma unroll
     for (int r = 0; r < REGS; ++r) room[(wave * REGS + r) * 64 + lane] = mine[r];
     __syncthreads();
 #pragma unroll
-    for (int r = 0; r < REGS / 4; ++r) {
-        const float* p = room + (wave * (REGS / 4) + r) * 64 + lane;
-        sum[r] = (p[0] + p[REGS * 64]) + (p[2 * REGS * 64] + p[3 * REGS * 64]);
+    for (int r = 0; r < REGS / STREAMS; ++r) {
+        const float* p = room + (wave % WAVES * REGS + wave / WAVES * (REGS / STREAMS) + r) * 64 + lane;
+        sum[r] = p[0] + p[WAVES * REGS * 64];
+        if (STREAMS == 4) sum[r] += p[2 * REGS * 64] + p[3 * REGS * 64];
     }
 }
 // The first channel of the four that accumulator values 4 n .. 4 n + 3 hold.
@@ -247,21 +252,23 @@ __device__ __forceinline__ AtWhere at_where(const AttendArgs& a, int id, int til
 }
 
 // ------------------------------------------------------------------------------------------------------------------- forward
-template <typename T, int DP, bool MASKED, bool NARROW>
+template <typename T, int DP, bool MASKED, int SHAPE>
 __global__ __launch_bounds__(256, 2) void at_fwd_kernel(AttendArgs a)
 {
     typedef typename AtEl<T>::x8 x8;
     typedef typename AtEl<T>::x4 x4;
-    typedef AtTile<T, DP, NARROW> Tile;
-    constexpr int OWN = AtShape<NARROW>::OWN, TILE = AtShape<NARROW>::TILE, STREAMS = AtShape<NARROW>::STREAMS, SUBS = TILE / 32, BUFS = NARROW ? 1 : 2;
-    __shared__ __attribute__((aligned(16))) AtShared<T, DP, NARROW, BUFS> sh;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, c = lane & 31, stream = NARROW ? wave : 0;
+    typedef AtTile<T, DP, SHAPE> Tile;
+    constexpr int OWN = AtShape<SHAPE>::OWN, TILE = AtShape<SHAPE>::TILE, STREAMS = AtShape<SHAPE>::STREAMS, SUBS = TILE / 32, BUFS = SHAPE == AT_NARROW ? 1 : 2;
+    constexpr bool NARROW = SHAPE == AT_NARROW;
+    static_assert(SHAPE != AT_HALF, "the forward has two shapes");
+    __shared__ __attribute__((aligned(16))) AtShared<T, DP, SHAPE, BUFS> sh;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, c = lane & 31, stream = wave / AtShape<SHAPE>::WAVES, sub = wave % AtShape<SHAPE>::WAVES;
     const int R = a.G * a.Nq, tiles = (R + OWN - 1) / OWN;
     const AtWhere where = at_where(a, xcd_remap(blockIdx.x, gridDim.x), tiles, a.splits);
     const int tile = a.causal ? tiles - 1 - where.tile : where.tile, split = where.split, kh = where.kh, b = where.b; // the long rows of a causal call first
 
     const int len = a.key_lengths ? min(max(a.key_lengths[b], 0), a.Nk) : a.Nk;
-    const int row = tile * OWN + (NARROW ? 0 : wave * 32) + c, rowc = min(row, R - 1), g = rowc / a.Nq, i = rowc - g * a.Nq;
+    const int row = tile * OWN + sub * 32 + c, rowc = min(row, R - 1), g = rowc / a.Nq, i = rowc - g * a.Nq;
     const int head = kh * a.G + g;
     const int lim = row >= R ? 0 : a.causal ? min(len, max(0, i + a.Nk - a.Nq + 1)) : len; // this row sees keys below lim
     const int wave_top = at_wave_max(lim), wave_low = at_wave_min(row < R ? lim : 0x7fffffff);
@@ -421,7 +428,7 @@ __global__ __launch_bounds__(256, 2) void at_fwd_kernel(AttendArgs a)
 #pragma unroll
         for (int r = 0; r < DP / 2; ++r) flat[r] *= weight;
         float sum[DP / 8];
-        at_sum_waves<DP / 2>(flat, reinterpret_cast<float*>(sh.tiles), sum);
+        at_sum_streams<DP / 2, SHAPE>(flat, reinterpret_cast<float*>(sh.tiles), sum);
         if (row >= R) return;
         if (wave == 0 && h == 0) statistics();
         const float inv = l == 0.f ? 0.f : 1.f / l;
@@ -526,20 +533,21 @@ template <typename T> __device__ __forceinline__ float at_grad_unit(const Attend
 }
 
 // dQ: a wave owns 32 rows and walks the keys that they see.
-template <typename T, int DP, bool MASKED, bool NARROW> __device__ __forceinline__ void at_bwd_rows(const AttendArgs& a, AtShared<T, DP, NARROW>& sh, int id)
+template <typename T, int DP, bool MASKED, int SHAPE> __device__ __forceinline__ void at_bwd_rows(const AttendArgs& a, AtShared<T, DP, SHAPE>& sh, int id)
 {
     typedef typename AtEl<T>::x8 x8;
     typedef typename AtEl<T>::x4 x4;
-    typedef AtTile<T, DP, NARROW> Tile;
-    constexpr int OWN = AtShape<NARROW>::OWN, TILE = AtShape<NARROW>::TILE, STREAMS = AtShape<NARROW>::STREAMS, SUBS = TILE / 32;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, c = lane & 31, stream = NARROW ? wave : 0;
+    typedef AtTile<T, DP, SHAPE> Tile;
+    constexpr int OWN = AtShape<SHAPE>::OWN, TILE = AtShape<SHAPE>::TILE, STREAMS = AtShape<SHAPE>::STREAMS, SUBS = TILE / 32;
+    constexpr bool NARROW = SHAPE == AT_NARROW;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, c = lane & 31, stream = wave / AtShape<SHAPE>::WAVES, sub = wave % AtShape<SHAPE>::WAVES;
     const int R = a.G * a.Nq, tiles = (R + OWN - 1) / OWN;
     const AtWhere where = at_where(a, id, tiles, 1);
     const int tile = a.causal ? tiles - 1 - where.tile : where.tile, kh = where.kh, b = where.b;
     const float unit = at_grad_unit<T>(a, b, kh, sh.unit4);
 
     const int len = a.key_lengths ? min(max(a.key_lengths[b], 0), a.Nk) : a.Nk;
-    const int row = tile * OWN + (NARROW ? 0 : wave * 32) + c, rowc = min(row, R - 1), g = rowc / a.Nq, i = rowc - g * a.Nq;
+    const int row = tile * OWN + sub * 32 + c, rowc = min(row, R - 1), g = rowc / a.Nq, i = rowc - g * a.Nq;
     const int head = kh * a.G + g;
     const int lim = row >= R ? 0 : a.causal ? min(len, max(0, i + a.Nk - a.Nq + 1)) : len;
     const int wave_top = at_wave_max(lim), wave_low = at_wave_min(row < R ? lim : 0x7fffffff);
@@ -579,10 +587,10 @@ template <typename T, int DP, bool MASKED, bool NARROW> __device__ __forceinline
     at_f32x16 acc[DP / 32] = {};
 
     int buf = 0;
-    for (int t = stream; t < t1; t += STREAMS, buf ^= 1) {
+    for (int t = stream; NARROW ? t < t1 : t - stream < t1; t += STREAMS, buf ^= 1) { // streams that share barriers take as many turns
         T *tk = sh.tiles[stream][buf][0], *tv = sh.tiles[stream][buf][1];
         at_landed();
-        if (MASKED && a.mask_by_key) {
+        if (MASKED && a.mask_by_key && t < t1) {
             Tile::hide(tk, mkey + (int64_t)t * TILE * a.m_sk, a.m_sk, len - t * TILE);
             Tile::hide(tv, mkey + (int64_t)t * TILE * a.m_sk, a.m_sk, len - t * TILE);
         }
@@ -591,7 +599,7 @@ template <typename T, int DP, bool MASKED, bool NARROW> __device__ __forceinline
 #pragma unroll
         for (int n = 0; n < SUBS; ++n) seen[n] = MASKED ? raw[n].bits() : 0;
         if (t + STREAMS < t1) { load(t + STREAMS, buf ^ 1); ask(t + STREAMS); }
-        if (t * TILE >= wave_top) continue;
+        if (t >= t1 || t * TILE >= wave_top) continue;
         at_f32x16 st[SUBS] = {}, dp[SUBS] = {};
 #pragma unroll
         for (int ks = 0; ks < DP / 16; ++ks)
@@ -637,13 +645,13 @@ template <typename T, int DP, bool MASKED, bool NARROW> __device__ __forceinline
     float flat[DP / 2];
 #pragma unroll
     for (int r = 0; r < DP / 2; ++r) flat[r] = acc[r >> 4][r & 15];
-    if (NARROW) {
-        float sum[DP / 8];
+    if (STREAMS > 1) {
+        float sum[DP / 2 / STREAMS];
         __syncthreads(); // every wave is done with its tiles
-        at_sum_waves<DP / 2>(flat, reinterpret_cast<float*>(sh.tiles), sum);
+        at_sum_streams<DP / 2, SHAPE>(flat, reinterpret_cast<float*>(sh.tiles), sum);
         if (row >= R) return;
 #pragma unroll
-        for (int n = 0; n < DP / 32; ++n) store(wave * (DP / 32) + n, sum + 4 * n);
+        for (int n = 0; n < DP / 8 / STREAMS; ++n) store(stream * (DP / 8 / STREAMS) + n, sum + 4 * n);
         return;
     }
     if (row >= R) return;
@@ -652,19 +660,20 @@ template <typename T, int DP, bool MASKED, bool NARROW> __device__ __forceinline
 }
 
 // dK, dV: a wave owns 32 keys and walks the rows that may see them.
-template <typename T, int DP, bool MASKED, bool NARROW> __device__ __forceinline__ void at_bwd_keys(const AttendArgs& a, AtSharedKeys<T, DP, NARROW>& sh, int id)
+template <typename T, int DP, bool MASKED, int SHAPE> __device__ __forceinline__ void at_bwd_keys(const AttendArgs& a, AtSharedKeys<T, DP, SHAPE>& sh, int id)
 {
     typedef typename AtEl<T>::x8 x8;
     typedef typename AtEl<T>::x4 x4;
-    typedef AtTile<T, DP, NARROW> Tile;
-    constexpr int OWN = AtShape<NARROW>::OWN, TILE = AtShape<NARROW>::TILE, STREAMS = AtShape<NARROW>::STREAMS, SUBS = TILE / 32;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, c = lane & 31, stream = NARROW ? wave : 0;
+    typedef AtTile<T, DP, SHAPE> Tile;
+    constexpr int OWN = AtShape<SHAPE>::OWN, TILE = AtShape<SHAPE>::TILE, STREAMS = AtShape<SHAPE>::STREAMS, SUBS = TILE / 32;
+    constexpr bool NARROW = SHAPE == AT_NARROW;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, c = lane & 31, stream = wave / AtShape<SHAPE>::WAVES, sub = wave % AtShape<SHAPE>::WAVES;
     const int R = a.G * a.Nq, tiles = (a.Nk + OWN - 1) / OWN, off = a.Nk - a.Nq;
     const AtWhere where = at_where(a, id, tiles, 1);
     const int tile = where.tile, kh = where.kh, b = where.b; // causal: the first keys are seen by most rows, the long ones come first as they are
     const float unit = at_grad_unit<T>(a, b, kh, sh.unit4);
     const int len = a.key_lengths ? min(max(a.key_lengths[b], 0), a.Nk) : a.Nk;
-    const int k0 = tile * OWN, wave_k0 = k0 + (NARROW ? 0 : wave * 32), key = wave_k0 + c;
+    const int k0 = tile * OWN, wave_k0 = k0 + sub * 32, key = wave_k0 + c;
 
     at_f32x16 dk[DP / 32] = {}, dv[DP / 32] = {};
     if (k0 < len) {
@@ -676,7 +685,7 @@ template <typename T, int DP, bool MASKED, bool NARROW> __device__ __forceinline
         // the tiles: head by head, from the first query that sees a key of this workgroup
         const int i_first = a.causal ? max(0, k0 - off) : 0, per_head = a.Nq > i_first ? (a.Nq - i_first + TILE - 1) / TILE : 0, t1 = a.G * per_head;
         const int slot = threadIdx.x & (TILE - 1);                       // the row whose numbers this thread brings
-        const bool brings = NARROW ? lane < TILE : threadIdx.x < TILE;
+        const bool brings = sub == 0 && lane < TILE;
         float n_lse = 0.f, n_delta = 0.f;
         int n_lim = -1;
         uint8_t raw[MASKED ? 16 * SUBS : 1];
@@ -730,7 +739,7 @@ template <typename T, int DP, bool MASKED, bool NARROW> __device__ __forceinline
             for (int ks = 0; ks < DP / 16; ++ks) { kf[ks] = x8{}; vf[ks] = x8{}; }
         }
         int buf = 0;
-        for (int t = stream; t < t1; t += STREAMS, buf ^= 1) {
+        for (int t = stream; NARROW ? t < t1 : t - stream < t1; t += STREAMS, buf ^= 1) {
             const T *tq = sh.tiles[stream][buf][0], *tg = sh.tiles[stream][buf][1];
             at_landed();
             if (!NARROW) __syncthreads();
@@ -740,6 +749,7 @@ template <typename T, int DP, bool MASKED, bool NARROW> __device__ __forceinline
 #pragma unroll
                 for (int r = 0; r < 16 * SUBS; ++r) seen |= (uint32_t)raw[r] << r;
             if (t + STREAMS < t1) i0_next = load(buf ^ 1);
+            if (STREAMS > 1 && t >= t1) continue;
             // unless every row of the tile sees every key of the wave
             const bool edge = MASKED || i0 + TILE > a.Nq || wave_k0 + 32 > len || (a.causal && i0 + off < wave_k0 + 31);
             at_f32x16 st[SUBS] = {}, dp[SUBS] = {};
@@ -839,15 +849,15 @@ template <typename T, int DP, bool MASKED, bool NARROW> __device__ __forceinline
     float fk[DP / 2], fv[DP / 2];
 #pragma unroll
     for (int r = 0; r < DP / 2; ++r) { fk[r] = dk[r >> 4][r & 15]; fv[r] = dv[r >> 4][r & 15]; }
-    if (NARROW) {
-        float sk[DP / 8], sv[DP / 8];
+    if (STREAMS > 1) {
+        float sk[DP / 2 / STREAMS], sv[DP / 2 / STREAMS];
         __syncthreads(); // every wave is done with its tiles
-        at_sum_waves<DP / 2>(fk, reinterpret_cast<float*>(sh.tiles), sk);
+        at_sum_streams<DP / 2, SHAPE>(fk, reinterpret_cast<float*>(sh.tiles), sk);
         __syncthreads();
-        at_sum_waves<DP / 2>(fv, reinterpret_cast<float*>(sh.tiles), sv);
+        at_sum_streams<DP / 2, SHAPE>(fv, reinterpret_cast<float*>(sh.tiles), sv);
         if (key >= a.Nk) return;
 #pragma unroll
-        for (int n = 0; n < DP / 32; ++n) store(wave * (DP / 32) + n, sk + 4 * n, sv + 4 * n);
+        for (int n = 0; n < DP / 8 / STREAMS; ++n) store(stream * (DP / 8 / STREAMS) + n, sk + 4 * n, sv + 4 * n);
         return;
     }
     if (key >= a.Nk) return;
@@ -856,40 +866,48 @@ template <typename T, int DP, bool MASKED, bool NARROW> __device__ __forceinline
 }
 
 // PART 1: the rows' workgroups, 2: the keys', 3: both in one launch, the keys' first (they are the longer ones).
-template <typename T, int DP, bool MASKED, bool NARROW, int PART>
-__global__ __launch_bounds__(256, (DP == 128 && PART > 1) || (DP > 64 && NARROW) || (DP == 96 && MASKED && PART > 1) ? 1 : 2) void at_bwd_kernel(AttendArgs a)
+template <typename T, int DP, bool MASKED, int SHAPE, int PART>
+__global__ __launch_bounds__(256, (DP == 128 && PART > 1) || (DP > 64 && SHAPE == AT_NARROW) || (DP == 96 && MASKED && PART > 1 && SHAPE != AT_HALF) ? 1 : 2) void at_bwd_kernel(AttendArgs a)
 {
     union Shared {
-        AtShared<T, DP, NARROW> rows;
-        AtSharedKeys<T, DP, NARROW> keys;
+        AtShared<T, DP, SHAPE> rows;
+        AtSharedKeys<T, DP, SHAPE> keys;
     };
     if constexpr (PART == 1) {
-        __shared__ __attribute__((aligned(16))) AtShared<T, DP, NARROW> sh;
-        at_bwd_rows<T, DP, MASKED, NARROW>(a, sh, xcd_remap(blockIdx.x, gridDim.x));
+        __shared__ __attribute__((aligned(16))) AtShared<T, DP, SHAPE> sh;
+        at_bwd_rows<T, DP, MASKED, SHAPE>(a, sh, xcd_remap(blockIdx.x, gridDim.x));
     } else if constexpr (PART == 2) {
-        __shared__ __attribute__((aligned(16))) AtSharedKeys<T, DP, NARROW> sh;
-        at_bwd_keys<T, DP, MASKED, NARROW>(a, sh, xcd_remap(blockIdx.x, gridDim.x));
+        __shared__ __attribute__((aligned(16))) AtSharedKeys<T, DP, SHAPE> sh;
+        at_bwd_keys<T, DP, MASKED, SHAPE>(a, sh, xcd_remap(blockIdx.x, gridDim.x));
     } else {
         __shared__ __attribute__((aligned(16))) char raw[sizeof(Shared)];
         Shared& sh = *reinterpret_cast<Shared*>(raw);
-        const int first = (a.Nk + AtShape<NARROW>::OWN - 1) / AtShape<NARROW>::OWN * a.B * a.Hk, id = blockIdx.x;
-        if (id < first) at_bwd_keys<T, DP, MASKED, NARROW>(a, sh.keys, xcd_remap(id, first));
-        else at_bwd_rows<T, DP, MASKED, NARROW>(a, sh.rows, xcd_remap(id - first, gridDim.x - first));
+        const int first = (a.Nk + AtShape<SHAPE>::OWN - 1) / AtShape<SHAPE>::OWN * a.B * a.Hk, id = blockIdx.x;
+        if (id < first) at_bwd_keys<T, DP, MASKED, SHAPE>(a, sh.keys, xcd_remap(id, first));
+        else at_bwd_rows<T, DP, MASKED, SHAPE>(a, sh.rows, xcd_remap(id - first, gridDim.x - first));
     }
 }
 
 // -------------------------------------------------------------------------------------------------------------------- launches
-// Which shape, by the workgroups of 128 rows (or keys) that the wide one would have on the 256 CUs.  Measured on both sides, D 64 | 128:
-//   forward, 768 keys: 96 workgroups 11.1 narrow 18.1 wide us | 16.0 23.1;  192: 13.9 18.3 | 26.0 24.4;  384: 24.7 24.6 | 46.5 35.5;
-//   2048 keys, causal, 256: 23.9 39.9 | 37.6 52.1;  8192 keys, 256: 125 146 | 203 212
-//   backward (both parts alike), 768 x 768: 48 + 48 workgroups 15.7 25.6 | 33.6 62.8;  96 + 96: 25.8 26.4 | 49.0 63.6;  144 + 144: 32.2 30.3 |
-//   82.9 66.4;  192 + 192: 37.9 32.0 | 101 69;  2048 x 2048, 128 + 128: 48.5 55.1 | 128 141
+// Which shape, by the workgroups of 128 rows (or keys) that the wide one would have on the 256 CUs.
+// Forward, us, narrow | wide, at D 64; 128:  768 keys, 96 workgroups 11.1 | 18.1; 16.0 | 23.1.  192: 13.9 | 18.3; 26.0 | 24.4.  384: 24.7 |
+//   24.6; 46.5 | 35.5.  2048 keys, causal, 256: 23.9 | 39.9; 37.6 | 52.1.  8192 keys, 256: 125 | 146; 203 | 212.
+// Backward, us, narrow | half | wide, at D 64; 80; 128, as many workgroups for rows as for keys:  768 x 768, 24: 13 | 19 | 26; 19 | 26 | 56; 19 |
+//   28 | 64.  48: 16 | 19 | 26; 32 | 26 | 57; 34 | 29 | 65.  96: 24 | 22 | 27; 48 | 28 | 58; 50 | 47 | 66.  144: 34 | 35 | 30; 77 | 47 | 59; 83 | 67 | 69.
+//   192: 39 | 38 | 31; 95 | 49 | 60; 101 | 75 | 71.  384: 75 | 60 | 54; 191 | 82 | 81; 198 | 139 | 122.  8192 x 8192, 128: 173 | 155 | 217; 513 | 210 |
+//   454; 549 | 352 | 534.  256: 328 | 289 | 248; 1052 | 405 | 468; 1059 | 702 | 541.
 static int64_t at_groups(int64_t bh, int64_t owned) { return bh * ceil_div(owned, 128); }
 static bool at_narrow_fwd(int64_t bh, int64_t R, int Nk, int D) {
     const int64_t g = at_groups(bh, R);
     return D <= 64 ? g < 384 : g <= 128 || (g <= 256 && Nk >= 1024);
 }
-static bool at_narrow_bwd(int64_t bh, int64_t owned, int D) { return at_groups(bh, owned) < (D <= 64 ? 144 : 112); }
+// A causal call has half the work, unevenly spread, so its workgroups count half (16 heads of 2048 x 2048, backward, us, narrow | half | wide at
+// D 64; 80; 128: 60 | 60 | 63; 158 | 80 | 126; 175 | 123 | 149).
+static int at_shape_bwd(int64_t bh, int64_t owned, int D, int causal) {
+    const int64_t g = at_groups(bh, owned) / (causal ? 2 : 1);
+    if (g < (D <= 64 ? 60 : 36)) return AT_NARROW;
+    return g < (D <= 64 ? 140 : D <= 96 ? 384 : 200) ? AT_HALF : AT_WIDE;
+}
 // Parts that a row's keys are cut into where even the narrow shape's workgroups are few.  A single tile of rows (token by token) is bound
 // by memory: four workgroups a CU, so that sequences of different lengths even out (16 caches of 0 to 8192: 75.3 us with two, 71.5, 72.7 with
 // eight, 84.1 with sixteen); more rows: two, as the parts have to be joined.  At
@@ -920,29 +938,31 @@ static int at_tensor(const void* p, const int64_t* s) {
 
 template <typename T, int DP, bool MASKED> static void at_launch_fwd(const AttendArgs& a, hipStream_t stream) {
     const int64_t R = (int64_t)a.G * a.Nq;
-    if (at_narrow_fwd((int64_t)a.B * a.Hk, R, a.Nk, a.D)) hipLaunchKernelGGL((at_fwd_kernel<T, DP, MASKED, true>), dim3((unsigned)(ceil_div(R, 32) * a.B * a.Hk * a.splits)), dim3(256), 0, stream, a);
-    else hipLaunchKernelGGL((at_fwd_kernel<T, DP, MASKED, false>), dim3((unsigned)(ceil_div(R, 128) * a.B * a.Hk)), dim3(256), 0, stream, a);
+    if (at_narrow_fwd((int64_t)a.B * a.Hk, R, a.Nk, a.D)) hipLaunchKernelGGL((at_fwd_kernel<T, DP, MASKED, AT_NARROW>), dim3((unsigned)(ceil_div(R, 32) * a.B * a.Hk * a.splits)), dim3(256), 0, stream, a);
+    else hipLaunchKernelGGL((at_fwd_kernel<T, DP, MASKED, AT_WIDE>), dim3((unsigned)(ceil_div(R, 128) * a.B * a.Hk)), dim3(256), 0, stream, a);
 }
 template <typename T, int DP, bool MASKED> static void at_launch_bwd(const AttendArgs& a, hipStream_t stream) {
     const int64_t R = (int64_t)a.G * a.Nq, bh = (int64_t)a.B * a.Hk;
-    const bool nk = at_narrow_bwd(bh, a.Nk, a.D), nr = at_narrow_bwd(bh, R, a.D);
-    const int64_t gk = ceil_div(a.Nk, nk ? 32 : 128) * bh, gr = ceil_div(R, nr ? 32 : 128) * bh;
-    if (nk && nr) {
-        hipLaunchKernelGGL((at_bwd_kernel<T, DP, MASKED, true, 3>), dim3((unsigned)(gk + gr)), dim3(256), 0, stream, a);
-        return;
-    }
-    if (DP == 64 && !nk && !nr && gk + gr < 2048) { // 8 a CU: below, the tails of two launches cost more than the rows' third wave a SIMD brings
-        hipLaunchKernelGGL((at_bwd_kernel<T, 64, MASKED, false, 3>), dim3((unsigned)(gk + gr)), dim3(256), 0, stream, a);
-        return;
-    }
+    // With fewer keys than rows the keys' workgroups are few and walk far: their shape for both (512 x 512 causal, 64 / 16 heads, D 64: 30 us
+    // narrow, 53 in two launches); with fewer rows each part has its own (256 rows x 8192 keys x 8 heads: 79 us; 91, 113 and 150 alike).
+    const int sk = at_shape_bwd(bh, a.Nk, a.D, a.causal), sr = a.Nk <= R ? sk : at_shape_bwd(bh, R, a.D, a.causal), own[3] = {AtShape<AT_WIDE>::OWN, AtShape<AT_NARROW>::OWN, AtShape<AT_HALF>::OWN};
+    const int64_t gk = ceil_div(a.Nk, own[sk]) * bh, gr = ceil_div(R, own[sr]) * bh;
+#define AT_BWD(SHAPE, PART, GROUPS) hipLaunchKernelGGL((at_bwd_kernel<T, DP, MASKED, SHAPE, PART>), dim3((unsigned)(GROUPS)), dim3(256), 0, stream, a)
+    if (sk == sr && sk == AT_NARROW) { AT_BWD(AT_NARROW, 3, gk + gr); return; }
+    if (sk == sr && sk == AT_HALF) { AT_BWD(AT_HALF, 3, gk + gr); return; }
+    if constexpr (DP == 64) // 8 a CU: below, the tails of two launches cost more than the rows' third wave a SIMD brings
+        if (sk == sr && gk + gr < 2048) { AT_BWD(AT_WIDE, 3, gk + gr); return; }
     if (gk) {
-        if (nk) hipLaunchKernelGGL((at_bwd_kernel<T, DP, MASKED, true, 2>), dim3((unsigned)gk), dim3(256), 0, stream, a);
-        else hipLaunchKernelGGL((at_bwd_kernel<T, DP, MASKED, false, 2>), dim3((unsigned)gk), dim3(256), 0, stream, a);
+        if (sk == AT_NARROW) AT_BWD(AT_NARROW, 2, gk);
+        else if (sk == AT_HALF) AT_BWD(AT_HALF, 2, gk);
+        else AT_BWD(AT_WIDE, 2, gk);
     }
     if (gr) {
-        if (nr) hipLaunchKernelGGL((at_bwd_kernel<T, DP, MASKED, true, 1>), dim3((unsigned)gr), dim3(256), 0, stream, a);
-        else hipLaunchKernelGGL((at_bwd_kernel<T, DP, MASKED, false, 1>), dim3((unsigned)gr), dim3(256), 0, stream, a);
+        if (sr == AT_NARROW) AT_BWD(AT_NARROW, 1, gr);
+        else if (sr == AT_HALF) AT_BWD(AT_HALF, 1, gr);
+        else AT_BWD(AT_WIDE, 1, gr);
     }
+#undef AT_BWD
 }
 
 template <typename T> static int at_fwd(const AttendArgs& a, hipStream_t stream) {
