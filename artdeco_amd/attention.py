@@ -157,7 +157,10 @@ def _backward_into(grad_out, q, k, v, out, lse, scale, causal, mask, key_lengths
     device = q.device
     lib = _lib.load()
     held = array("q", (*strides, *g, *dq.stride()[:3], *dk.stride()[:3], *dv.stride()[:3]))
-    ws, nbytes = _workspace(lib.adk_attend_bwd_workspace_bytes(B, H, Hk, Nq, Nk, D), "adk_attend_bwd", device)
+    nbytes = lib.adk_attend_bwd_workspace_bytes(B, H, Hk, Nq, Nk, D)
+    if mask is not None and nbytes > 0:
+        nbytes += lib.adk_attend_mask_bytes(B, H, Nq, Nk, held.buffer_info()[0] + 72)  # strides: the mask's come after q's, k's and v's
+    ws, nbytes = _workspace(nbytes, "adk_attend_bwd", device)
     _lib.launch(lib.adk_attend_bwd, "adk_attend_bwd", device, grad_out.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(),
                 _lib.ptr(key_lengths), _lib.ptr(mask), _DTYPES[q.dtype], B, H, Hk, Nq, Nk, D, held.buffer_info()[0], scale, causal, dq.data_ptr(), dk.data_ptr(),
                 dv.data_ptr(), _lib.ptr(ws), nbytes)

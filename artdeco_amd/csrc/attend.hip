@@ -59,9 +59,10 @@ struct AttendArgs {
     float* part_o;          // [splits, B, Hk, G Nq, D] (splits > 1)
     float* part_ml;         // [splits, B, Hk, G Nq, 2]
     float* amax;            // largest |dout| of each block of at_delta_kernel
+    uint32_t *by_row, *by_key; // the mask's bits, as at_mask_bits writes them
     const int* key_lengths; // [B] or null
     const uint8_t* mask;    // or null
-    int B, H, Hk, G, Nq, Nk, D, splits, causal, mask_by_key;
+    int B, H, Hk, G, Nq, Nk, D, splits, causal, mask_by_key, mask_rows, delta_blocks;
     int64_t q_sb, q_sh, q_sn, k_sb, k_sh, k_sn, v_sb, v_sh, v_sn, g_sb, g_sh, g_sn; // element strides: batch, head, token
     int64_t dq_sb, dq_sh, dq_sn, dk_sb, dk_sh, dk_sn, dv_sb, dv_sh, dv_sn;
     int64_t m_sb, m_sh, m_sq, m_sk;
@@ -163,45 +164,47 @@ template <typename T> __device__ __forceinline__ typename AtEl<T>::x8 at_global_
     return col < D ? *reinterpret_cast<const typename AtEl<T>::x8*>(row + col) : z;
 }
 
-// Which of a row's keys k0 + 8 (r / 4) + r % 4 a mask shows.  Asked for a tile ahead: 16 bytes stay on their way until bits() wants them
-// (bit r for key r).  Where 4 keys lie side by side in memory and the whole range is inside the tensor, four at a time; otherwise bytes,
-// at keys of the tensor (`last` repeats).
-struct __attribute__((packed, aligned(1))) AtFour { uint32_t x; };
-struct AtMask16 {
+// Which of 32 keys a row sees, bit k for key k0 + k, alike in lanes c and c + 32.  Asked for a tile ahead: lane (h, c) brings the bytes
+// of its 16 keys from k0 + 16 h on, and they stay on their way until bits() wants them.  Where keys lie side by side in memory and all 32
+// are inside the tensor that is one load; otherwise bytes, at keys of the tensor (`last` repeats).  (4 loads of 4 bytes in the accumulator's
+// order ask for 4 times the cache lines: 517 x 1031 x 12/4 heads, D 80, 43.3 us against 40.6.  Bits packed by a launch before, as for the
+// backward pass: 42.0; 16 heads of 4096 x 4096, D 64: 131 against 123.)
+struct __attribute__((packed, aligned(1))) AtSixteen { uint32_t x[4]; };
+struct AtMask32 {
     uint32_t x[4];
-    __device__ __forceinline__ void ask(const uint8_t* row, int64_t sk, int k0, int last, bool four) {
-        if (four) {
+    __device__ __forceinline__ void ask(const uint8_t* row, int64_t sk, int k0, int last, bool together) { // k0: of this lane's 16
+        if (together) {
+            const AtSixteen v = *reinterpret_cast<const AtSixteen*>(row + k0);
 #pragma unroll
-            for (int r4 = 0; r4 < 4; ++r4) x[r4] = reinterpret_cast<const AtFour*>(row + k0 + 8 * r4)->x;
+            for (int n = 0; n < 4; ++n) x[n] = v.x[n];
         } else {
 #pragma unroll
-            for (int r4 = 0; r4 < 4; ++r4) {
-                x[r4] = 0;
+            for (int n = 0; n < 4; ++n) {
+                x[n] = 0;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) x[r4] |= (uint32_t)row[(int64_t)min(k0 + 8 * r4 + e, last) * sk] << (8 * e);
+                for (int e = 0; e < 4; ++e) x[n] |= (uint32_t)row[(int64_t)min(k0 + 4 * n + e, last) * sk] << (8 * e);
             }
         }
     }
-    // four bytes of 0 or 1 to four bits: byte e times 2^(24 - 7 e) lands on bit 24 + e, every other product on a bit of its own below 24
-    // or past 31
-    __device__ __forceinline__ uint32_t bits() const {
-        uint32_t b = 0;
-#pragma unroll
-        for (int r4 = 0; r4 < 4; ++r4) b |= ((x[r4] * 0x01020408u >> 24) & 15u) << (4 * r4);
-        return b;
+    __device__ __forceinline__ uint32_t bits() const { // bytes of 0 or 1: sums of powers of two
+        typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
+        const uint32_t lo = __builtin_amdgcn_udot4(x[1], 0x80402010u, __builtin_amdgcn_udot4(x[0], 0x08040201u, 0u, false), false);
+        const uint32_t hi = __builtin_amdgcn_udot4(x[3], 0x80402010u, __builtin_amdgcn_udot4(x[2], 0x08040201u, 0u, false), false);
+        const uint32_t mine = lo | hi << 8;
+        const u32x2 both = __builtin_amdgcn_permlane32_swap(mine, mine, false, false); // lane c's and lane c + 32's
+        return both.x | both.y << 16;
     }
 };
 // Hiding is by selects on such bits: with a branch around the byte's load hipcc 7.2 lost the hiding of an accumulator's element 0.
-__device__ __forceinline__ float at_hidden_unless(uint32_t bits, int r, float s) { // s if bit r is set, else -inf
-    const uint32_t on = (uint32_t)__builtin_amdgcn_sbfe((int)bits, r, 1);
+__device__ __forceinline__ float at_hidden_unless(uint32_t bits, int n, float s) { // s if bit n is set, else -inf
+    const uint32_t on = (uint32_t)__builtin_amdgcn_sbfe((int)bits, n, 1);
     return __uint_as_float((__float_as_uint(s) & on) | (0xff800000u & ~on));
 }
-// Bits r of the keys k0 + 8 (r / 4) + r % 4 that lie below lim.
+__device__ __forceinline__ int at_key(int r) { return 8 * (r >> 2) + (r & 3); } // accumulator element r of lane half h has key at_key(r) + 4 h
+// Bits k of the 32 numbers k0 + k that lie below lim.
 __device__ __forceinline__ uint32_t at_below_bits(int k0, int lim) {
-    uint32_t bits = 0;
-#pragma unroll
-    for (int r4 = 0; r4 < 4; ++r4) bits |= ((1u << min(max(lim - k0 - 8 * r4, 0), 4)) - 1u) << (4 * r4);
-    return bits;
+    const int n = lim - k0;
+    return n >= 32 ? 0xffffffffu : (1u << max(n, 0)) - 1u;
 }
 
 // A workgroup's LDS.  Narrow: when the tiles are done with, their place takes the waves' partial results, 64 lanes a register.
@@ -215,7 +218,6 @@ template <typename T, int DP, int SHAPE> struct AtSharedKeys {
     static constexpr int S = AtShape<SHAPE>::STREAMS, TILE = AtShape<SHAPE>::TILE;
     T tiles[S][2][2][TILE * DP];
     float lse[S][2][TILE], delta[S][2][TILE];
-    int lim[S][2][TILE];
     float unit4[4];
 };
 
@@ -301,11 +303,11 @@ __global__ __launch_bounds__(256, 2) void at_fwd_kernel(AttendArgs a)
     auto hide = [&](int t, T* tile) {
         if (MASKED && a.mask_by_key) Tile::hide(tile, mkey + (int64_t)t * TILE * a.m_sk, a.m_sk, len - t * TILE);
     };
-    AtMask16 raw[MASKED ? SUBS : 1];
+    AtMask32 raw[MASKED ? SUBS : 1];
     auto ask = [&](int t) {
         if (MASKED)
 #pragma unroll
-            for (int n = 0; n < SUBS; ++n) raw[n].ask(mrow, a.m_sk, t * TILE + 32 * n + 4 * h, a.Nk - 1, a.m_sk == 1 && (t + 1) * TILE <= a.Nk);
+            for (int n = 0; n < SUBS; ++n) raw[n].ask(mrow, a.m_sk, t * TILE + 32 * n + 16 * h, a.Nk - 1, a.m_sk == 1 && (t + 1) * TILE <= a.Nk);
     };
     Tile::pad(sh.tiles[0][0][0], BUFS, a.D);
     if (t0 + stream < t1) { load_k(t0 + stream, 0); load_v(t0 + stream, 0); ask(t0 + stream); }
@@ -344,11 +346,11 @@ __global__ __launch_bounds__(256, 2) void at_fwd_kernel(AttendArgs a)
         if (MASKED || (t + 1) * TILE > wave_low) {
 #pragma unroll
             for (int n = 0; n < SUBS; ++n) {
-                const int k0 = t * TILE + 32 * n + 4 * h;
-                uint32_t see = at_below_bits(k0, lim);
+                uint32_t see = at_below_bits(t * TILE + 32 * n, lim);
                 if (MASKED) see &= seen[n];
+                see >>= 4 * h;
 #pragma unroll
-                for (int r = 0; r < 16; ++r) st[n][r] = at_hidden_unless(see, r, st[n][r]);
+                for (int r = 0; r < 16; ++r) st[n][r] = at_hidden_unless(see, at_key(r), st[n][r]);
             }
         }
         if (NARROW) { // one buffer: K's next tile as soon as this one is read, V's at the end; half the LDS, so twice the waves
@@ -491,10 +493,45 @@ __global__ __launch_bounds__(256) void at_join_kernel(AttendArgs a)
 // delta_i = <dO_i, o_i>, 16 lanes a row; and the largest |dO| of each block of 16 rows, from which the fp16 kernels take the
 // power of two that brings dS into fp16's range.
 #define AT_DELTA_ROWS 16
+// The mask as bits: by row, word (set, n, i) the keys 32 n + k of row i; by key, word (set, n, j) the rows 32 n + r that show key j.  A set
+// is a sequence's or a head's mask, one for all of them where it is broadcast; a mask that is the same for every query has one row, and its
+// words by key say so for 32.  The owners of rows and of keys then ask for one word each, side by side in memory, where the bytes of a
+// tile of 32 rows lie in 32 cache lines: 517 x 1031 x 12/4 heads, D 80, 101 us with bytes, 73 with bits.
+__host__ __device__ __forceinline__ int at_words(int n) { return (n + 31) / 32; }
+__host__ __device__ __forceinline__ int64_t at_mask_set(const AttendArgs& a, int b, int head) {
+    return (int64_t)(a.m_sb ? b : 0) * (a.m_sh ? a.H : 1) + (a.m_sh ? head : 0);
+}
+__host__ __device__ __forceinline__ int64_t at_mask_waves(const AttendArgs& a) { // one for 32 rows x 64 keys
+    return (at_mask_set(a, a.B - 1, a.H - 1) + 1) * at_words(a.mask_rows) * ((a.Nk + 63) / 64);
+}
+static __device__ __forceinline__ void at_mask_bits(const AttendArgs& a, int64_t id) {
+    if (id >= at_mask_waves(a)) return;
+    const int lane = threadIdx.x & 63, rt = at_words(a.mask_rows), kt = at_words(a.Nk), pairs = (a.Nk + 63) / 64;
+    const int pair = (int)(id % pairs), n = (int)(id / pairs % rt);
+    const int64_t set = id / pairs / rt, b = a.m_sh ? set / a.H : set, head = a.m_sh ? set % a.H : 0;
+    const int key = 64 * pair + lane;
+    const uint8_t* p = a.mask + b * a.m_sb + head * a.m_sh + (int64_t)min(key, a.Nk - 1) * a.m_sk;
+    uint32_t rows = 0, keys = 0; // of this lane's key; of row 32 n + lane % 32, keys 64 pair + 32 (lane / 32) ..
+#pragma unroll
+    for (int r = 0; r < 32; ++r) {
+        const bool on = p[(int64_t)min(32 * n + r, a.mask_rows - 1) * a.m_sq] != 0 && key < a.Nk && 32 * n + r < a.mask_rows;
+        const uint64_t all = __builtin_amdgcn_ballot_w64(on);
+        rows |= (uint32_t)on << r;
+        if ((lane & 31) == r) keys = lane < 32 ? (uint32_t)all : (uint32_t)(all >> 32);
+    }
+    if (a.mask_rows == 1) rows = rows ? 0xffffffffu : 0u;
+    if (key < a.Nk) a.by_key[(set * rt + n) * a.Nk + key] = rows;
+    const int row = 32 * n + (lane & 31), word = 2 * pair + (lane >> 5);
+    if (row < a.mask_rows && word < kt) a.by_row[(set * kt + word) * a.mask_rows + row] = keys;
+}
 template <typename T>
 __global__ __launch_bounds__(256) void at_delta_kernel(AttendArgs a)
 {
     typedef typename AtEl<T>::x8 x8;
+    if ((int)blockIdx.x >= a.delta_blocks) {
+        at_mask_bits(a, 4 * (int64_t)(blockIdx.x - a.delta_blocks) + (threadIdx.x >> 6));
+        return;
+    }
     const int64_t rows = (int64_t)a.B * a.H * a.Nq, at = (int64_t)blockIdx.x * AT_DELTA_ROWS + (threadIdx.x >> 4);
     const int d = (threadIdx.x & 15) * 8;
     float sum = 0.f, top = 0.f;
@@ -561,17 +598,17 @@ template <typename T, int DP, bool MASKED, int SHAPE> __device__ __forceinline__
 
     const T* kb = static_cast<const T*>(a.k) + (int64_t)b * a.k_sb + (int64_t)kh * a.k_sh;
     const T* vb = static_cast<const T*>(a.v) + (int64_t)b * a.v_sb + (int64_t)kh * a.v_sh;
-    const uint8_t* mrow = MASKED ? a.mask + (int64_t)b * a.m_sb + (int64_t)head * a.m_sh + (int64_t)i * a.m_sq : nullptr;
+    const uint32_t* words = MASKED ? a.by_row + at_mask_set(a, b, head) * at_words(a.Nk) * a.mask_rows + (a.mask_rows > 1 ? i : 0) : nullptr; // this row's
     const uint8_t* mkey = MASKED ? a.mask + (int64_t)b * a.m_sb + (int64_t)kh * a.G * a.m_sh : nullptr;
     auto load = [&](int t, int buf) {
         Tile::load(sh.tiles[stream][buf][0], kb + (int64_t)t * TILE * a.k_sn, (int)a.k_sn, len - t * TILE, a.D);
         Tile::load(sh.tiles[stream][buf][1], vb + (int64_t)t * TILE * a.v_sn, (int)a.v_sn, len - t * TILE, a.D);
     };
-    AtMask16 raw[MASKED ? SUBS : 1];
-    auto ask = [&](int t) {
+    uint32_t coming[MASKED ? SUBS : 1];
+    auto ask = [&](int t) { // a tile ahead
         if (MASKED)
 #pragma unroll
-            for (int n = 0; n < SUBS; ++n) raw[n].ask(mrow, a.m_sk, t * TILE + 32 * n + 4 * h, a.Nk - 1, a.m_sk == 1 && (t + 1) * TILE <= a.Nk);
+            for (int n = 0; n < SUBS; ++n) coming[n] = words[(int64_t)min(t * SUBS + n, at_words(a.Nk) - 1) * a.mask_rows];
     };
     Tile::pad(sh.tiles[0][0][0], 2, a.D);
     if (stream < t1) { load(stream, 0); ask(stream); }
@@ -597,7 +634,7 @@ template <typename T, int DP, bool MASKED, int SHAPE> __device__ __forceinline__
         if (!NARROW) __syncthreads();
         uint32_t seen[SUBS];
 #pragma unroll
-        for (int n = 0; n < SUBS; ++n) seen[n] = MASKED ? raw[n].bits() : 0;
+        for (int n = 0; n < SUBS; ++n) seen[n] = MASKED ? coming[n] : 0;
         if (t + STREAMS < t1) { load(t + STREAMS, buf ^ 1); ask(t + STREAMS); }
         if (t >= t1 || t * TILE >= wave_top) continue;
         at_f32x16 st[SUBS] = {}, dp[SUBS] = {};
@@ -611,11 +648,11 @@ template <typename T, int DP, bool MASKED, int SHAPE> __device__ __forceinline__
         if (MASKED || (t + 1) * TILE > wave_low) {
 #pragma unroll
             for (int n = 0; n < SUBS; ++n) {
-                const int k0 = t * TILE + 32 * n + 4 * h;
-                uint32_t see = at_below_bits(k0, lim);
+                uint32_t see = at_below_bits(t * TILE + 32 * n, lim);
                 if (MASKED) see &= seen[n];
+                see >>= 4 * h;
 #pragma unroll
-                for (int r = 0; r < 16; ++r) st[n][r] = at_hidden_unless(see, r, st[n][r]);
+                for (int r = 0; r < 16; ++r) st[n][r] = at_hidden_unless(see, at_key(r), st[n][r]);
             }
         }
         x8 ds[SUBS][2];
@@ -682,13 +719,12 @@ template <typename T, int DP, bool MASKED, int SHAPE> __device__ __forceinline__
         const T* gb = static_cast<const T*>(a.dout) + (int64_t)b * a.g_sb + (int64_t)kh * a.G * a.g_sh;
         const int64_t at0 = ((int64_t)b * a.Hk + kh) * R;
         const uint8_t* mkey = MASKED ? a.mask + (int64_t)b * a.m_sb + (int64_t)kh * a.G * a.m_sh + (int64_t)keyc * a.m_sk : nullptr;
-        // the tiles: head by head, from the first query that sees a key of this workgroup
-        const int i_first = a.causal ? max(0, k0 - off) : 0, per_head = a.Nq > i_first ? (a.Nq - i_first + TILE - 1) / TILE : 0, t1 = a.G * per_head;
+        // the tiles: head by head, from the first query that sees a key of this workgroup (where there is a mask, of its word's rows)
+        const int i_first = a.causal ? MASKED ? max(0, k0 - off) & ~31 : max(0, k0 - off) : 0, per_head = a.Nq > i_first ? (a.Nq - i_first + TILE - 1) / TILE : 0, t1 = a.G * per_head;
         const int slot = threadIdx.x & (TILE - 1);                       // the row whose numbers this thread brings
         const bool brings = sub == 0 && lane < TILE;
         float n_lse = 0.f, n_delta = 0.f;
-        int n_lim = -1;
-        uint8_t raw[MASKED ? 16 * SUBS : 1];
+        uint32_t coming[MASKED ? SUBS : 1];
         int g_next = 0, j_next = stream; // the next tile: head and number in it
         while (j_next >= per_head && g_next < a.G) { j_next -= per_head; ++g_next; }
         auto load = [&](int buf) { // returns the first row of the tile
@@ -698,30 +734,20 @@ template <typename T, int DP, bool MASKED, int SHAPE> __device__ __forceinline__
             Tile::load(sh.tiles[stream][buf][0], qb + (int64_t)g * a.q_sh + (int64_t)i0 * a.q_sn, (int)a.q_sn, a.Nq - i0, a.D);
             Tile::load(sh.tiles[stream][buf][1], gb + (int64_t)g * a.g_sh + (int64_t)i0 * a.g_sn, (int)a.g_sn, a.Nq - i0, a.D);
             if (brings) {
-                const int i = i0 + slot, ic = min(i, a.Nq - 1);
-                const int64_t at = at0 + (int64_t)g * a.Nq + ic;
+                const int64_t at = at0 + (int64_t)g * a.Nq + min(i0 + slot, a.Nq - 1);
                 n_lse = a.lse[at]; // as they are: worked on in note(), when they have long arrived
                 n_delta = a.delta[at];
-                n_lim = i >= a.Nq ? -1 : a.causal ? min(len - 1, i + off) : len - 1; // the last key that the row sees
             }
-            if (MASKED) { // this key's byte of each row
-                const uint8_t* p = mkey + ((int64_t)g * a.m_sh + (int64_t)i0 * a.m_sq);
-                if (i0 + TILE <= a.Nq) {
-                    p += 4 * h * a.m_sq;
+            if (MASKED)
 #pragma unroll
-                    for (int r = 0; r < 16 * SUBS; ++r) raw[r] = p[(int64_t)(32 * (r >> 4) + 8 * (r >> 2 & 3) + (r & 3)) * a.m_sq];
-                } else {
-#pragma unroll
-                    for (int r = 0; r < 16 * SUBS; ++r) raw[r] = p[(int64_t)min(32 * (r >> 4) + 8 * (r >> 2 & 3) + 4 * h + (r & 3), a.Nq - 1 - i0) * a.m_sq];
-                }
-            }
+                for (int n = 0; n < SUBS; ++n)
+                    coming[n] = a.by_key[(at_mask_set(a, b, kh * a.G + g) * at_words(a.mask_rows) + min(i0 / 32 + n, at_words(a.mask_rows) - 1)) * a.Nk + keyc];
             return i0;
         };
         auto note = [&](int buf) {
             if (brings) {
                 sh.lse[stream][buf][slot] = n_lse == -INFINITY ? -INFINITY : -n_lse * 1.4426950408889634f;
                 sh.delta[stream][buf][slot] = -n_delta * unit;
-                sh.lim[stream][buf][slot] = n_lim;
             }
         };
         Tile::pad(sh.tiles[0][0][0], 2, a.D);
@@ -744,10 +770,9 @@ template <typename T, int DP, bool MASKED, int SHAPE> __device__ __forceinline__
             at_landed();
             if (!NARROW) __syncthreads();
             i0 = i0_next;
-            uint32_t seen = 0; // bit r: this key's row r of the tile, in the accumulators' order
-            if (MASKED)
+            uint32_t seen[SUBS];
 #pragma unroll
-                for (int r = 0; r < 16 * SUBS; ++r) seen |= (uint32_t)raw[r] << r;
+            for (int n = 0; n < SUBS; ++n) seen[n] = MASKED ? coming[n] : 0;
             if (t + STREAMS < t1) i0_next = load(buf ^ 1);
             if (STREAMS > 1 && t >= t1) continue;
             // unless every row of the tile sees every key of the wave
@@ -766,12 +791,12 @@ template <typename T, int DP, bool MASKED, int SHAPE> __device__ __forceinline__
                 }
             };
             auto hide = [&](int n) {
+                uint32_t see = key < len ? at_below_bits(i0 + 32 * n, a.Nq) : 0; // which rows see this lane's key
+                if (a.causal) see &= ~at_below_bits(i0 + 32 * n, key - off);
+                if (MASKED) see &= seen[n];
+                see >>= 4 * h;
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int q = 32 * n + 8 * (r >> 2) + 4 * h + (r & 3);
-                    st[n][r] = key <= sh.lim[stream][buf][q] ? st[n][r] : -INFINITY;
-                    if (MASKED) st[n][r] = at_hidden_unless(seen, 16 * n + r, st[n][r]);
-                }
+                for (int r = 0; r < 16; ++r) st[n][r] = at_hidden_unless(see, at_key(r), st[n][r]);
             };
             auto probs = [&](int n) {
 #pragma unroll
@@ -867,7 +892,7 @@ template <typename T, int DP, bool MASKED, int SHAPE> __device__ __forceinline__
 
 // PART 1: the rows' workgroups, 2: the keys', 3: both in one launch, the keys' first (they are the longer ones).
 template <typename T, int DP, bool MASKED, int SHAPE, int PART>
-__global__ __launch_bounds__(256, (DP == 128 && PART > 1) || (DP > 64 && SHAPE == AT_NARROW) || (DP == 96 && MASKED && PART > 1 && SHAPE != AT_HALF) ? 1 : 2) void at_bwd_kernel(AttendArgs a)
+__global__ __launch_bounds__(256, (DP == 128 && PART > 1) || (DP > 64 && SHAPE == AT_NARROW) ? 1 : 2) void at_bwd_kernel(AttendArgs a)
 {
     union Shared {
         AtShared<T, DP, SHAPE> rows;
@@ -974,8 +999,8 @@ template <typename T> static int at_fwd(const AttendArgs& a, hipStream_t stream)
 }
 
 template <typename T> static int at_bwd(const AttendArgs& a, hipStream_t stream) {
-    const int64_t rows = (int64_t)a.B * a.H * a.Nq;
-    if (rows) hipLaunchKernelGGL((at_delta_kernel<T>), dim3((unsigned)ceil_div(rows, AT_DELTA_ROWS)), dim3(256), 0, stream, a);
+    const int64_t blocks = a.delta_blocks + (a.mask ? ceil_div(at_mask_waves(a), 4) : 0);
+    if (blocks) hipLaunchKernelGGL((at_delta_kernel<T>), dim3((unsigned)blocks), dim3(256), 0, stream, a);
     if (a.D <= 64) { if (a.mask) at_launch_bwd<T, 64, true>(a, stream); else at_launch_bwd<T, 64, false>(a, stream); }
     else if (a.D <= 96) { if (a.mask) at_launch_bwd<T, 96, true>(a, stream); else at_launch_bwd<T, 96, false>(a, stream); }
     else { if (a.mask) at_launch_bwd<T, 128, true>(a, stream); else at_launch_bwd<T, 128, false>(a, stream); }
@@ -992,6 +1017,7 @@ static void at_fill(AttendArgs& a, const void* q, const void* k, const void* v, 
     a.k_sb = s[3]; a.k_sh = s[4]; a.k_sn = s[5];
     a.v_sb = s[6]; a.v_sh = s[7]; a.v_sn = s[8];
     if (mask) { a.m_sb = s[9]; a.m_sh = s[10]; a.m_sq = s[11]; a.m_sk = s[12]; }
+    a.mask_rows = a.m_sq ? Nq : 1;
     a.mask_by_key = a.mask && a.m_sq == 0 && (a.m_sh == 0 || a.G == 1);
     a.scale = scale; a.scale_log2e = scale * 1.4426950408889634f;
 }
@@ -1036,6 +1062,14 @@ extern "C" int64_t adk_attend_bwd_workspace_bytes(int B, int H, int Hk, int Nq, 
     return 4 * (rows + adk::ceil_div(rows, AT_DELTA_ROWS));
 }
 
+extern "C" int64_t adk_attend_mask_bytes(int B, int H, int Nq, int Nk, const int64_t* strides)
+{
+    if (B < 1 || H < 1 || Nq < 1 || Nk < 1) return 0;
+    if (!strides) return ADK_EINVAL;
+    const int64_t sets = (int64_t)(strides[0] ? B : 1) * (strides[1] ? H : 1), rows = strides[2] ? Nq : 1;
+    return 4 * sets * (adk::at_words(Nk) * rows + adk::at_words((int)rows) * (int64_t)Nk);
+}
+
 extern "C" int adk_attend_bwd(const void* dout, const void* q, const void* k, const void* v, const void* out, const float* lse, const int32_t* key_lengths,
                               const uint8_t* mask, int dtype, int B, int H, int Hk, int Nq, int Nk, int D, const int64_t* strides, float scale, int causal, void* dq,
                               void* dk, void* dv, void* ws, int64_t ws_bytes, hipStream_t stream)
@@ -1057,9 +1091,17 @@ extern "C" int adk_attend_bwd(const void* dout, const void* q, const void* k, co
     a.dv_sb = s[9]; a.dv_sh = s[10]; a.dv_sn = s[11];
     const int64_t rows = (int64_t)B * H * Nq;
     if (rows) {
-        if (!ws || ws_bytes < adk_attend_bwd_workspace_bytes(B, H, Hk, Nq, Nk, D) || ((uintptr_t)ws & 15)) return ADK_EWORKSPACE;
+        int64_t need = adk_attend_bwd_workspace_bytes(B, H, Hk, Nq, Nk, D);
         a.delta = static_cast<float*>(ws);
         a.amax = a.delta + rows;
+        a.delta_blocks = (int)adk::ceil_div(rows, AT_DELTA_ROWS);
+        if (a.mask) {
+            if (a.delta_blocks + adk::at_mask_waves(a) / 4 > 0x7ffffff0ll) return ADK_EUNSUPPORTED;
+            a.by_row = reinterpret_cast<uint32_t*>(a.amax + a.delta_blocks);
+            a.by_key = a.by_row + (adk::at_mask_set(a, B - 1, H - 1) + 1) * adk::at_words(Nk) * a.mask_rows;
+            need += adk_attend_mask_bytes(B, H, Nq, Nk, strides + 9);
+        }
+        if (!ws || ws_bytes < need || ((uintptr_t)ws & 15)) return ADK_EWORKSPACE;
     }
     return dtype == 0 ? adk::at_bwd<_Float16>(a, stream) : adk::at_bwd<__bf16>(a, stream);
 }

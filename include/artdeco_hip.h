@@ -316,13 +316,15 @@ int adk_attention_fwd_f16(const void* q, const void* k, const void* v, void* out
  * causal: query i sees keys j <= i + Nk - Nq.  key_lengths [B] int32 or NULL: sequence b has keys below key_lengths[b]; what
  * lies behind is never read, its dk and dv are 0.  mask or NULL: one byte a pair, 1 shows and 0 hides it, no other value (a
  * stride of 0 broadcasts).  A query without a visible key: out 0, lse -inf, no gradient.  scale > 0.  No atomics: the same bits on every run.
- * ws: *_workspace_bytes() bytes (may be 0), 16-byte aligned, contents free after the call.
+ * ws: *_workspace_bytes() bytes (may be 0), in the backward with a mask adk_attend_mask_bytes() more (of the mask's four
+ * strides), 16-byte aligned, contents free after the call.
  */
 int64_t adk_attend_fwd_workspace_bytes(int B, int H, int Hk, int Nq, int Nk, int D);
 int adk_attend_fwd(const void* q, const void* k, const void* v, void* out, float* lse, const int32_t* key_lengths, const uint8_t* mask,
                    int dtype, int B, int H, int Hk, int Nq, int Nk, int D, const int64_t* strides, float scale, int causal, void* ws,
                    int64_t ws_bytes, adk_stream_t stream);
 int64_t adk_attend_bwd_workspace_bytes(int B, int H, int Hk, int Nq, int Nk, int D);
+int64_t adk_attend_mask_bytes(int B, int H, int Nq, int Nk, const int64_t* mask_strides);
 int adk_attend_bwd(const void* dout, const void* q, const void* k, const void* v, const void* out, const float* lse,
                    const int32_t* key_lengths, const uint8_t* mask, int dtype, int B, int H, int Hk, int Nq, int Nk, int D,
                    const int64_t* strides, float scale, int causal, void* dq, void* dk, void* dv, void* ws, int64_t ws_bytes,

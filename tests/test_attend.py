@@ -151,6 +151,21 @@ def test_free_masks_with_rows_that_see_nothing(shape, dtype, dev):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["batch", "heads", "queries alone", "transposed"])
+@pytest.mark.parametrize("size", [(2, 2, 1, 100, 333, 64), (1, 32, 32, 300, 1133, 64), (3, 8, 4, 270, 523, 96), (2, 24, 24, 300, 1133, 96), (1, 12, 12, 290, 777, 128),
+                                  (2, 24, 24, 301, 1134, 128)], ids=str)
+def test_masks_in_small_and_large_calls(size, kind, dev):
+    """More keys than queries, so that a causal call begins inside a word of the mask's bits; from a few workgroups to several for each CU."""
+    B, H, Hk, Nq, Nk, D = size
+    q, k, v, do = inputs(*size, torch.bfloat16, dev, seed=7)
+    g = torch.Generator().manual_seed(2)
+    shape = {"batch": (B, 1, Nq, Nk), "heads": (1, H, Nq, Nk), "queries alone": (B, 1, Nq, 1), "transposed": (B, 1, Nk, Nq)}[kind]
+    mask = (torch.rand(shape, generator=g) < 0.7).to(dev)
+    mask = mask.transpose(2, 3) if kind == "transposed" else mask
+    run(q, k, v, do, mask=mask, causal=kind != "heads")
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("bad", [math.nan, math.inf])
 def test_a_mask_over_keys_alone_hides_what_is_not_finite(bad, dev):
     q, k, v, do = inputs(2, 4, 2, 50, 100, 64, torch.bfloat16, dev, seed=8)
@@ -377,6 +392,11 @@ def test_c_entry_refuses_before_any_launch(lib):
     assert fwd(Nq=0) == 0
     assert lib.adk_attend_fwd_workspace_bytes(1, 4, 2, 4, 4096, 64) > 0 and lib.adk_attend_fwd_workspace_bytes(1, 4, 3, 4, 4, 64) == -1
     assert lib.adk_attend_bwd_workspace_bytes(2, 4, 2, 8, 8, 64) == 4 * (64 + 4)
+    per_head, for_keys = (ctypes.c_int64 * 4)(0, 33 * 65, 65, 1), (ctypes.c_int64 * 4)(65, 0, 0, 1)
+    assert lib.adk_attend_mask_bytes(2, 4, 33, 65, per_head) == 4 * 4 * (3 * 33 + 2 * 65) and lib.adk_attend_mask_bytes(2, 4, 33, 65, for_keys) == 4 * 2 * (3 + 65)
+    assert lib.adk_attend_mask_bytes(2, 4, 0, 65, per_head) == 0 and lib.adk_attend_mask_bytes(2, 4, 33, 65, None) == -1
+    masked = (P, P, P, P, P, P, None, P, 0, 1, 4, 2, 4, 4, 64, fine, 1.0, 0, P, P, P, P)  # a workspace without room for the mask's bits
+    assert lib.adk_attend_bwd(*masked, lib.adk_attend_bwd_workspace_bytes(1, 4, 2, 4, 4, 64), None) == -2
     assert lib.adk_attend_bwd(P, P, P, P, P, P, None, None, 0, 1, 4, 2, 4, 4, 64, fine, 1.0, 0, P, P, P, None, 0, None) == -2
 
 
