@@ -23,6 +23,8 @@
 // calls too small to fill the chip so: a workgroup owns 32, and each wave walks every fourth tile of 32 with LDS tiles of its own and
 // no barrier; the four partial results are joined through LDS at the end, in a fixed order.  Half, for the backward pass between the two: it
 // owns 64, two waves share every second tile of 32, and two partial results are joined; its tiles are small enough for two workgroups a CU.
+// Where even these are few for what they walk (a token over a long cache, a few keys that thousands of queries read), the walk is cut
+// into parts whose 32-bit results a last launch adds in their order.
 //
 // LDS tiles hold 16-byte chunks at chunk ^ f(row): with f below, the 16 rows of a 128-bit fragment read and the 4 rows of a
 // transposing read fall on different banks without padding.
@@ -59,10 +61,11 @@ struct AttendArgs {
     float* part_o;          // [splits, B, Hk, G Nq, D] (splits > 1)
     float* part_ml;         // [splits, B, Hk, G Nq, 2]
     float* amax;            // largest |dout| of each block of at_delta_kernel
+    float *part_dq, *part_dk, *part_dv; // [row_splits, B, H, Nq, D], [key_splits, B, Hk, Nk, D] where there are several
     uint32_t *by_row, *by_key; // the mask's bits, as at_mask_bits writes them
     const int* key_lengths; // [B] or null
     const uint8_t* mask;    // or null
-    int B, H, Hk, G, Nq, Nk, D, splits, causal, mask_by_key, mask_rows, delta_blocks;
+    int B, H, Hk, G, Nq, Nk, D, splits, causal, mask_by_key, mask_rows, delta_blocks, row_splits, key_splits;
     int64_t q_sb, q_sh, q_sn, k_sb, k_sh, k_sn, v_sb, v_sh, v_sn, g_sb, g_sh, g_sn; // element strides: batch, head, token
     int64_t dq_sb, dq_sh, dq_sn, dk_sb, dk_sh, dk_sn, dv_sb, dv_sh, dv_sn;
     int64_t m_sb, m_sh, m_sq, m_sk;
@@ -570,7 +573,7 @@ template <typename T> __device__ __forceinline__ float at_grad_unit(const Attend
 }
 
 // dQ: a wave owns 32 rows and walks the keys that they see.
-template <typename T, int DP, bool MASKED, int SHAPE> __device__ __forceinline__ void at_bwd_rows(const AttendArgs& a, AtShared<T, DP, SHAPE>& sh, int id)
+template <typename T, int DP, bool MASKED, int SHAPE, bool SPLIT> __device__ __forceinline__ void at_bwd_rows(const AttendArgs& a, AtShared<T, DP, SHAPE>& sh, int id)
 {
     typedef typename AtEl<T>::x8 x8;
     typedef typename AtEl<T>::x4 x4;
@@ -579,7 +582,7 @@ template <typename T, int DP, bool MASKED, int SHAPE> __device__ __forceinline__
     constexpr bool NARROW = SHAPE == AT_NARROW;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, c = lane & 31, stream = wave / AtShape<SHAPE>::WAVES, sub = wave % AtShape<SHAPE>::WAVES;
     const int R = a.G * a.Nq, tiles = (R + OWN - 1) / OWN;
-    const AtWhere where = at_where(a, id, tiles, 1);
+    const AtWhere where = at_where(a, id, tiles, SPLIT ? a.row_splits : 1);
     const int tile = a.causal ? tiles - 1 - where.tile : where.tile, kh = where.kh, b = where.b;
     const float unit = at_grad_unit<T>(a, b, kh, sh.unit4);
 
@@ -594,7 +597,12 @@ template <typename T, int DP, bool MASKED, int SHAPE> __device__ __forceinline__
         __syncthreads();
         top = __builtin_amdgcn_readfirstlane(max(max(sh.tops[0], sh.tops[1]), max(sh.tops[2], sh.tops[3])));
     }
-    const int t1 = (top + TILE - 1) / TILE;
+    int t0 = 0, t1 = (top + TILE - 1) / TILE;
+    if (SPLIT) {
+        const int per = ((a.Nk + TILE - 1) / TILE + a.row_splits - 1) / a.row_splits;
+        t0 = where.split * per;
+        t1 = min(t1, t0 + per);
+    }
 
     const T* kb = static_cast<const T*>(a.k) + (int64_t)b * a.k_sb + (int64_t)kh * a.k_sh;
     const T* vb = static_cast<const T*>(a.v) + (int64_t)b * a.v_sb + (int64_t)kh * a.v_sh;
@@ -611,7 +619,7 @@ template <typename T, int DP, bool MASKED, int SHAPE> __device__ __forceinline__
             for (int n = 0; n < SUBS; ++n) coming[n] = words[(int64_t)min(t * SUBS + n, at_words(a.Nk) - 1) * a.mask_rows];
     };
     Tile::pad(sh.tiles[0][0][0], 2, a.D);
-    if (stream < t1) { load(stream, 0); ask(stream); }
+    if (t0 + stream < t1) { load(t0 + stream, 0); ask(t0 + stream); }
     x8 qf[DP / 16], gf[DP / 16];
     {
         const T* qp = static_cast<const T*>(a.q) + (int64_t)b * a.q_sb + (int64_t)head * a.q_sh + (int64_t)i * a.q_sn;
@@ -624,7 +632,7 @@ template <typename T, int DP, bool MASKED, int SHAPE> __device__ __forceinline__
     at_f32x16 acc[DP / 32] = {};
 
     int buf = 0;
-    for (int t = stream; NARROW ? t < t1 : t - stream < t1; t += STREAMS, buf ^= 1) { // streams that share barriers take as many turns
+    for (int t = t0 + stream; NARROW ? t < t1 : t - stream < t1; t += STREAMS, buf ^= 1) { // streams that share barriers take as many turns
         T *tk = sh.tiles[stream][buf][0], *tv = sh.tiles[stream][buf][1];
         at_landed();
         if (MASKED && a.mask_by_key && t < t1) {
@@ -674,6 +682,10 @@ template <typename T, int DP, bool MASKED, int SHAPE> __device__ __forceinline__
     const bool blind = lse == -INFINITY; // sees nothing: a gradient of zero whatever the (unread) products gave
     auto store = [&](int n, const float* o) {
         const int d = at_channel(n, h);
+        if (SPLIT && a.row_splits > 1) {
+            if (d < a.D) *reinterpret_cast<at_f32x4*>(a.part_dq + (((int64_t)(where.split * a.B + b) * a.Hk + kh) * R + row) * a.D + d) = blind ? at_f32x4{0.f, 0.f, 0.f, 0.f} : at_f32x4{o[0] * f, o[1] * f, o[2] * f, o[3] * f};
+            return;
+        }
         x4 y;
 #pragma unroll
         for (int e = 0; e < 4; ++e) y[e] = blind ? (T)0.f : (T)(o[e] * f);
@@ -697,7 +709,7 @@ template <typename T, int DP, bool MASKED, int SHAPE> __device__ __forceinline__
 }
 
 // dK, dV: a wave owns 32 keys and walks the rows that may see them.
-template <typename T, int DP, bool MASKED, int SHAPE> __device__ __forceinline__ void at_bwd_keys(const AttendArgs& a, AtSharedKeys<T, DP, SHAPE>& sh, int id)
+template <typename T, int DP, bool MASKED, int SHAPE, bool SPLIT> __device__ __forceinline__ void at_bwd_keys(const AttendArgs& a, AtSharedKeys<T, DP, SHAPE>& sh, int id)
 {
     typedef typename AtEl<T>::x8 x8;
     typedef typename AtEl<T>::x4 x4;
@@ -706,7 +718,7 @@ template <typename T, int DP, bool MASKED, int SHAPE> __device__ __forceinline__
     constexpr bool NARROW = SHAPE == AT_NARROW;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, c = lane & 31, stream = wave / AtShape<SHAPE>::WAVES, sub = wave % AtShape<SHAPE>::WAVES;
     const int R = a.G * a.Nq, tiles = (a.Nk + OWN - 1) / OWN, off = a.Nk - a.Nq;
-    const AtWhere where = at_where(a, id, tiles, 1);
+    const AtWhere where = at_where(a, id, tiles, SPLIT ? a.key_splits : 1);
     const int tile = where.tile, kh = where.kh, b = where.b; // causal: the first keys are seen by most rows, the long ones come first as they are
     const float unit = at_grad_unit<T>(a, b, kh, sh.unit4);
     const int len = a.key_lengths ? min(max(a.key_lengths[b], 0), a.Nk) : a.Nk;
@@ -720,12 +732,19 @@ template <typename T, int DP, bool MASKED, int SHAPE> __device__ __forceinline__
         const int64_t at0 = ((int64_t)b * a.Hk + kh) * R;
         const uint8_t* mkey = MASKED ? a.mask + (int64_t)b * a.m_sb + (int64_t)kh * a.G * a.m_sh + (int64_t)keyc * a.m_sk : nullptr;
         // the tiles: head by head, from the first query that sees a key of this workgroup (where there is a mask, of its word's rows)
-        const int i_first = a.causal ? MASKED ? max(0, k0 - off) & ~31 : max(0, k0 - off) : 0, per_head = a.Nq > i_first ? (a.Nq - i_first + TILE - 1) / TILE : 0, t1 = a.G * per_head;
+        const int i_first = a.causal ? MASKED ? max(0, k0 - off) & ~31 : max(0, k0 - off) : 0, per_head = a.Nq > i_first ? (a.Nq - i_first + TILE - 1) / TILE : 0;
+        int t0 = 0, t1 = a.G * per_head, g_next = 0, j_next = stream; // the next tile: head and number in it
         const int slot = threadIdx.x & (TILE - 1);                       // the row whose numbers this thread brings
         const bool brings = sub == 0 && lane < TILE;
         float n_lse = 0.f, n_delta = 0.f;
         uint32_t coming[MASKED ? SUBS : 1];
-        int g_next = 0, j_next = stream; // the next tile: head and number in it
+        if (SPLIT && t1) {
+            const int per = (t1 + a.key_splits - 1) / a.key_splits;
+            t0 = where.split * per;
+            t1 = min(t1, t0 + per);
+            g_next = t0 / per_head;
+            j_next = t0 - g_next * per_head + stream;
+        }
         while (j_next >= per_head && g_next < a.G) { j_next -= per_head; ++g_next; }
         auto load = [&](int buf) { // returns the first row of the tile
             const int g = g_next, i0 = i_first + j_next * TILE;
@@ -752,7 +771,7 @@ template <typename T, int DP, bool MASKED, int SHAPE> __device__ __forceinline__
         };
         Tile::pad(sh.tiles[0][0][0], 2, a.D);
         int i0 = 0, i0_next = 0;
-        if (stream < t1) { i0_next = load(0); note(0); }
+        if (t0 + stream < t1) { i0_next = load(0); note(0); }
         x8 kf[DP / 16], vf[DP / 16];
         {
             const T* kp = static_cast<const T*>(a.k) + (int64_t)b * a.k_sb + (int64_t)kh * a.k_sh + (int64_t)keyc * a.k_sn;
@@ -765,7 +784,7 @@ template <typename T, int DP, bool MASKED, int SHAPE> __device__ __forceinline__
             for (int ks = 0; ks < DP / 16; ++ks) { kf[ks] = x8{}; vf[ks] = x8{}; }
         }
         int buf = 0;
-        for (int t = stream; NARROW ? t < t1 : t - stream < t1; t += STREAMS, buf ^= 1) {
+        for (int t = t0 + stream; NARROW ? t < t1 : t - stream < t1; t += STREAMS, buf ^= 1) {
             const T *tq = sh.tiles[stream][buf][0], *tg = sh.tiles[stream][buf][1];
             at_landed();
             if (!NARROW) __syncthreads();
@@ -863,6 +882,14 @@ template <typename T, int DP, bool MASKED, int SHAPE> __device__ __forceinline__
     const float f = a.scale / unit;
     auto store = [&](int n, const float* x, const float* y) {
         const int d = at_channel(n, h);
+        if (SPLIT && a.key_splits > 1) {
+            const int64_t to = (((int64_t)(where.split * a.B + b) * a.Hk + kh) * a.Nk + key) * a.D + d;
+            if (d < a.D) {
+                *reinterpret_cast<at_f32x4*>(a.part_dk + to) = at_f32x4{x[0] * f, x[1] * f, x[2] * f, x[3] * f};
+                *reinterpret_cast<at_f32x4*>(a.part_dv + to) = at_f32x4{y[0], y[1], y[2], y[3]};
+            }
+            return;
+        }
         x4 k4, v4;
 #pragma unroll
         for (int e = 0; e < 4; ++e) { k4[e] = (T)(x[e] * f); v4[e] = (T)y[e]; }
@@ -891,7 +918,7 @@ template <typename T, int DP, bool MASKED, int SHAPE> __device__ __forceinline__
 }
 
 // PART 1: the rows' workgroups, 2: the keys', 3: both in one launch, the keys' first (they are the longer ones).
-template <typename T, int DP, bool MASKED, int SHAPE, int PART>
+template <typename T, int DP, bool MASKED, int SHAPE, int PART, bool SPLIT>
 __global__ __launch_bounds__(256, (DP == 128 && PART > 1) || (DP > 64 && SHAPE == AT_NARROW) ? 1 : 2) void at_bwd_kernel(AttendArgs a)
 {
     union Shared {
@@ -900,17 +927,40 @@ __global__ __launch_bounds__(256, (DP == 128 && PART > 1) || (DP > 64 && SHAPE =
     };
     if constexpr (PART == 1) {
         __shared__ __attribute__((aligned(16))) AtShared<T, DP, SHAPE> sh;
-        at_bwd_rows<T, DP, MASKED, SHAPE>(a, sh, xcd_remap(blockIdx.x, gridDim.x));
+        at_bwd_rows<T, DP, MASKED, SHAPE, SPLIT>(a, sh, xcd_remap(blockIdx.x, gridDim.x));
     } else if constexpr (PART == 2) {
         __shared__ __attribute__((aligned(16))) AtSharedKeys<T, DP, SHAPE> sh;
-        at_bwd_keys<T, DP, MASKED, SHAPE>(a, sh, xcd_remap(blockIdx.x, gridDim.x));
+        at_bwd_keys<T, DP, MASKED, SHAPE, SPLIT>(a, sh, xcd_remap(blockIdx.x, gridDim.x));
     } else {
         __shared__ __attribute__((aligned(16))) char raw[sizeof(Shared)];
         Shared& sh = *reinterpret_cast<Shared*>(raw);
-        const int first = (a.Nk + AtShape<SHAPE>::OWN - 1) / AtShape<SHAPE>::OWN * a.B * a.Hk, id = blockIdx.x;
-        if (id < first) at_bwd_keys<T, DP, MASKED, SHAPE>(a, sh.keys, xcd_remap(id, first));
-        else at_bwd_rows<T, DP, MASKED, SHAPE>(a, sh.rows, xcd_remap(id - first, gridDim.x - first));
+        const int first = (a.Nk + AtShape<SHAPE>::OWN - 1) / AtShape<SHAPE>::OWN * a.B * a.Hk * (SPLIT ? a.key_splits : 1), id = blockIdx.x;
+        if (id < first) at_bwd_keys<T, DP, MASKED, SHAPE, SPLIT>(a, sh.keys, xcd_remap(id, first));
+        else at_bwd_rows<T, DP, MASKED, SHAPE, SPLIT>(a, sh.rows, xcd_remap(id - first, gridDim.x - first));
     }
+}
+
+// The parts of a gradient, added in their order: four channels a thread, the rows' before the keys'.
+template <typename T> __global__ __launch_bounds__(256) void at_bwd_join_kernel(AttendArgs a)
+{
+    typedef typename AtEl<T>::x4 x4;
+    const int q4 = a.D / 4;
+    const int64_t rows = a.row_splits > 1 ? (int64_t)a.B * a.H * a.Nq * q4 : 0, keys = a.key_splits > 1 ? (int64_t)a.B * a.Hk * a.Nk * q4 : 0;
+    int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (at >= rows + 2 * keys) return;
+    const bool is_q = at < rows, is_k = at - rows < keys;
+    at -= is_q ? 0 : is_k ? rows : rows + keys;
+    const float* p = (is_q ? a.part_dq : is_k ? a.part_dk : a.part_dv) + at * 4;
+    const int64_t part = 4 * (is_q ? rows : keys);
+    at_f32x4 sum = *reinterpret_cast<const at_f32x4*>(p);
+    for (int n = 1; n < (is_q ? a.row_splits : a.key_splits); ++n) sum += *reinterpret_cast<const at_f32x4*>(p + n * part);
+    const int d = (int)(at % q4) * 4, heads = is_q ? a.H : a.Hk, count = is_q ? a.Nq : a.Nk;
+    const int64_t i = at / q4 % count, head = at / q4 / count % heads, b = at / q4 / count / heads;
+    const int64_t to = is_q ? b * a.dq_sb + head * a.dq_sh + i * a.dq_sn : is_k ? b * a.dk_sb + head * a.dk_sh + i * a.dk_sn : b * a.dv_sb + head * a.dv_sh + i * a.dv_sn;
+    x4 y;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] = (T)sum[e];
+    *reinterpret_cast<x4*>(static_cast<T*>(is_q ? a.dq : is_k ? a.dk : a.dv) + to + d) = y;
 }
 
 // -------------------------------------------------------------------------------------------------------------------- launches
@@ -944,6 +994,39 @@ static int at_splits(int64_t bh, int64_t R, int Nk, int D) {
     return (int)(s < 1 ? 1 : s > 64 ? 64 : s);
 }
 
+// The backward pass's launches: shapes of the keys' and the rows' owners, and the parts that their walks are cut into (by the sizes alone, so
+// that the workspace is the same for a causal call).  Cut, whole, us, D 64: 8192 keys x 16 queries x 4 heads 24, 69; 33 keys x 4096 queries x 16/2
+// heads 49, 330; 7 keys x 5000 x 8/1 41, 389.
+struct AtBwdPlan { int keys, rows, key_splits, row_splits; };
+static AtBwdPlan at_plan_bwd(int64_t bh, int64_t R, int64_t Nk, int D, int causal) {
+    AtBwdPlan p = {at_shape_bwd(bh, Nk, D, 0), at_shape_bwd(bh, R, D, 0), 1, 1};
+    const int64_t wr = bh * ceil_div(R, 32), wk = bh * ceil_div(Nk, 32);
+    if (!wr || !wk) return p;
+    auto parts = [](int64_t s, int64_t walked) { // of 512 at least: four waves' four tiles
+        s = s < walked / 512 ? s : walked / 512;
+        return (int)(s < 1 ? 1 : s > 64 ? 64 : s);
+    };
+    if (p.keys != p.rows && Nk > R) { // launches of their own, each to fill the chip four times
+        p.key_splits = parts(1024 / wk, R); // 128 x 4096 x 4 x 16 heads, D 64; 128, us, rows whole: 107; 201.  In 2: 86; 171.  4: 77; 165
+        p.row_splits = parts(1024 / wr, Nk);
+    } else { // together: none is to walk much further than a 512th of the whole, where that is worth the join (1024 x 1024 x 4 heads, D 64; 128:
+             // whole 16; 24 us, in 2 20; 38)
+        const int64_t fair = ceil_div(wr * Nk + wk * R, 512);
+        auto worth = [&](int64_t walked) { const int n = parts(walked / fair, walked); return n >= 3 || walked / n >= 4096 ? n : 1; };
+        p.key_splits = worth(R);
+        p.row_splits = worth(Nk);
+    }
+    p.keys = at_shape_bwd(bh, Nk, D, causal);
+    p.rows = at_shape_bwd(bh, R, D, causal);
+    // keys that are fewer than the rows walk far: their shape for both, in one launch; unless their walk is cut and the rows' is short (rows x
+    // keys x heads / key heads, us together | apart, at D 64; 80; 128:  4096 x 33 x 16/2: 53 | 49; 101 | 56; 96 | 61.  8192 x 256 x 8: 56 | 62;
+    // 123 | 69; 117 | 74.  1200 x 700 x 8/2: 29 | 34; 49 | 44; 55 | 49.  2048 x 2048 x 8/2, causal: 46 | 76; 89 | 97; 97 | 109)
+    if (Nk <= R && p.row_splits == 1 && (p.key_splits == 1 || Nk > (D <= 64 ? 192 : 1024))) p.rows = p.keys;
+    if (p.key_splits > 1 && p.keys == AT_WIDE) p.keys = AT_HALF;
+    if (p.row_splits > 1 && p.rows == AT_WIDE) p.rows = AT_HALF;
+    return p;
+}
+
 static int at_check(int dtype, int B, int H, int Hk, int Nq, int Nk, int D, float scale) {
     if (dtype != 0 && dtype != 2) return ADK_EUNSUPPORTED;
     if (B < 0 || H < 1 || Hk < 1 || H % Hk || Nq < 0 || Nk < 0) return ADK_EINVAL;
@@ -968,25 +1051,26 @@ template <typename T, int DP, bool MASKED> static void at_launch_fwd(const Atten
 }
 template <typename T, int DP, bool MASKED> static void at_launch_bwd(const AttendArgs& a, hipStream_t stream) {
     const int64_t R = (int64_t)a.G * a.Nq, bh = (int64_t)a.B * a.Hk;
-    // With fewer keys than rows the keys' workgroups are few and walk far: their shape for both (512 x 512 causal, 64 / 16 heads, D 64: 30 us
-    // narrow, 53 in two launches); with fewer rows each part has its own (256 rows x 8192 keys x 8 heads: 79 us; 91, 113 and 150 alike).
-    const int sk = at_shape_bwd(bh, a.Nk, a.D, a.causal), sr = a.Nk <= R ? sk : at_shape_bwd(bh, R, a.D, a.causal), own[3] = {AtShape<AT_WIDE>::OWN, AtShape<AT_NARROW>::OWN, AtShape<AT_HALF>::OWN};
-    const int64_t gk = ceil_div(a.Nk, own[sk]) * bh, gr = ceil_div(R, own[sr]) * bh;
-#define AT_BWD(SHAPE, PART, GROUPS) hipLaunchKernelGGL((at_bwd_kernel<T, DP, MASKED, SHAPE, PART>), dim3((unsigned)(GROUPS)), dim3(256), 0, stream, a)
-    if (sk == sr && sk == AT_NARROW) { AT_BWD(AT_NARROW, 3, gk + gr); return; }
-    if (sk == sr && sk == AT_HALF) { AT_BWD(AT_HALF, 3, gk + gr); return; }
+    const AtBwdPlan plan = at_plan_bwd(bh, R, a.Nk, a.D, a.causal);
+    const int sk = plan.keys, sr = plan.rows, own[3] = {AtShape<AT_WIDE>::OWN, AtShape<AT_NARROW>::OWN, AtShape<AT_HALF>::OWN};
+    const int64_t gk = ceil_div(a.Nk, own[sk]) * bh * a.key_splits, gr = ceil_div(R, own[sr]) * bh * a.row_splits;
+#define AT_BWD(SHAPE, PART, SPLIT, GROUPS) hipLaunchKernelGGL((at_bwd_kernel<T, DP, MASKED, SHAPE, PART, SPLIT>), dim3((unsigned)(GROUPS)), dim3(256), 0, stream, a)
+#define AT_BWD_CUT(SHAPE, PART, SPLITS, GROUPS) if ((SPLITS) > 1) AT_BWD(SHAPE, PART, true, GROUPS); else AT_BWD(SHAPE, PART, false, GROUPS)
+    if (sk == sr && sk == AT_NARROW) { AT_BWD_CUT(AT_NARROW, 3, a.key_splits * a.row_splits, gk + gr); return; }
+    if (sk == sr && sk == AT_HALF) { AT_BWD_CUT(AT_HALF, 3, a.key_splits * a.row_splits, gk + gr); return; }
     if constexpr (DP == 64) // 8 a CU: below, the tails of two launches cost more than the rows' third wave a SIMD brings
-        if (sk == sr && gk + gr < 2048) { AT_BWD(AT_WIDE, 3, gk + gr); return; }
+        if (sk == sr && gk + gr < 2048) { AT_BWD(AT_WIDE, 3, false, gk + gr); return; }
     if (gk) {
-        if (sk == AT_NARROW) AT_BWD(AT_NARROW, 2, gk);
-        else if (sk == AT_HALF) AT_BWD(AT_HALF, 2, gk);
-        else AT_BWD(AT_WIDE, 2, gk);
+        if (sk == AT_NARROW) { AT_BWD_CUT(AT_NARROW, 2, a.key_splits, gk); }
+        else if (sk == AT_HALF) { AT_BWD_CUT(AT_HALF, 2, a.key_splits, gk); }
+        else AT_BWD(AT_WIDE, 2, false, gk);
     }
     if (gr) {
-        if (sr == AT_NARROW) AT_BWD(AT_NARROW, 1, gr);
-        else if (sr == AT_HALF) AT_BWD(AT_HALF, 1, gr);
-        else AT_BWD(AT_WIDE, 1, gr);
+        if (sr == AT_NARROW) { AT_BWD_CUT(AT_NARROW, 1, a.row_splits, gr); }
+        else if (sr == AT_HALF) { AT_BWD_CUT(AT_HALF, 1, a.row_splits, gr); }
+        else AT_BWD(AT_WIDE, 1, false, gr);
     }
+#undef AT_BWD_CUT
 #undef AT_BWD
 }
 
@@ -1004,6 +1088,8 @@ template <typename T> static int at_bwd(const AttendArgs& a, hipStream_t stream)
     if (a.D <= 64) { if (a.mask) at_launch_bwd<T, 64, true>(a, stream); else at_launch_bwd<T, 64, false>(a, stream); }
     else if (a.D <= 96) { if (a.mask) at_launch_bwd<T, 96, true>(a, stream); else at_launch_bwd<T, 96, false>(a, stream); }
     else { if (a.mask) at_launch_bwd<T, 128, true>(a, stream); else at_launch_bwd<T, 128, false>(a, stream); }
+    const int64_t parts = ((a.row_splits > 1 ? (int64_t)a.B * a.H * a.Nq : 0) + (a.key_splits > 1 ? 2 * (int64_t)a.B * a.Hk * a.Nk : 0)) * (a.D / 4);
+    if (parts) hipLaunchKernelGGL((at_bwd_join_kernel<T>), dim3((unsigned)ceil_div(parts, 256)), dim3(256), 0, stream, a);
     ADK_RETURN_LAST_ERROR();
 }
 
@@ -1012,7 +1098,7 @@ static void at_fill(AttendArgs& a, const void* q, const void* k, const void* v, 
                     int Nq, int Nk, int D, const int64_t* s, float scale, int causal) {
     a.q = q; a.k = k; a.v = v; a.lse = const_cast<float*>(lse);
     a.key_lengths = key_lengths; a.mask = Nq && Nk ? mask : nullptr;
-    a.B = B; a.H = H; a.Hk = Hk; a.G = H / Hk; a.Nq = Nq; a.Nk = Nk; a.D = D; a.splits = 1; a.causal = causal;
+    a.B = B; a.H = H; a.Hk = Hk; a.G = H / Hk; a.Nq = Nq; a.Nk = Nk; a.D = D; a.splits = a.row_splits = a.key_splits = 1; a.causal = causal;
     a.q_sb = s[0]; a.q_sh = s[1]; a.q_sn = s[2];
     a.k_sb = s[3]; a.k_sh = s[4]; a.k_sn = s[5];
     a.v_sb = s[6]; a.v_sh = s[7]; a.v_sn = s[8];
@@ -1058,8 +1144,11 @@ extern "C" int64_t adk_attend_bwd_workspace_bytes(int B, int H, int Hk, int Nq, 
 {
     const int e = adk::at_check(0, B, H, Hk, Nq, Nk, D, 1.f);
     if (e) return e;
-    const int64_t rows = (int64_t)B * H * Nq;
-    return 4 * (rows + adk::ceil_div(rows, AT_DELTA_ROWS));
+    const int64_t rows = (int64_t)B * H * Nq, keys = (int64_t)B * Hk * Nk, R = (int64_t)(H / Hk) * Nq;
+    const adk::AtBwdPlan p = adk::at_plan_bwd((int64_t)B * Hk, R, Nk, D, 0);
+    const int rs = p.row_splits, ks = p.key_splits;
+    const int64_t parts = (rs > 1 ? rs * rows * D : 0) + (ks > 1 ? 2 * ks * keys * D : 0);
+    return 4 * (parts + rows + adk::ceil_div(rows, AT_DELTA_ROWS));
 }
 
 extern "C" int64_t adk_attend_mask_bytes(int B, int H, int Nq, int Nk, const int64_t* strides)
@@ -1092,7 +1181,13 @@ extern "C" int adk_attend_bwd(const void* dout, const void* q, const void* k, co
     const int64_t rows = (int64_t)B * H * Nq;
     if (rows) {
         int64_t need = adk_attend_bwd_workspace_bytes(B, H, Hk, Nq, Nk, D);
-        a.delta = static_cast<float*>(ws);
+        const adk::AtBwdPlan p = adk::at_plan_bwd((int64_t)B * Hk, (int64_t)a.G * Nq, Nk, D, causal);
+        a.row_splits = p.row_splits;
+        a.key_splits = p.key_splits;
+        a.part_dq = static_cast<float*>(ws); // first: 16-byte aligned
+        a.part_dk = a.part_dq + (a.row_splits > 1 ? a.row_splits * rows * D : 0);
+        a.part_dv = a.part_dk + (a.key_splits > 1 ? a.key_splits * (int64_t)B * Hk * Nk * D : 0);
+        a.delta = a.part_dv + (a.key_splits > 1 ? a.key_splits * (int64_t)B * Hk * Nk * D : 0);
         a.amax = a.delta + rows;
         a.delta_blocks = (int)adk::ceil_div(rows, AT_DELTA_ROWS);
         if (a.mask) {

@@ -166,6 +166,24 @@ def test_masks_in_small_and_large_calls(size, kind, dev):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("how", ["whole", "causal", "lengths and mask"])
+@pytest.mark.parametrize("size", [(1, 8, 1, 2100, 7, 64), (2, 4, 2, 16, 4100, 96), (1, 16, 2, 900, 150, 128), (1, 1, 1, 2001, 1999, 40), (2, 20, 20, 128, 2100, 128),
+                                  (1, 12, 12, 1, 3000, 64), (1, 2, 1, 4000, 1, 8)], ids=str)
+def test_few_keys_or_few_queries_beside_many(size, how, dev):
+    """Walks that are cut into parts and joined: of the keys' owners, of the rows', of both."""
+    B, H, Hk, Nq, Nk, D = size
+    q, k, v, do = inputs(*size, torch.bfloat16 if D > 64 else torch.float16, dev, seed=11)
+    mask = lengths = None
+    if how == "lengths and mask":
+        g = torch.Generator().manual_seed(4)
+        mask = (torch.rand(1, 1, Nq, Nk, generator=g) < 0.8).to(dev)
+        lengths = torch.tensor([Nk // 3, Nk][:B], dtype=torch.int32, device=dev)
+    first = run(q, k, v, do, causal=how == "causal", mask=mask, lengths=lengths)
+    again = both(q, k, v, do, causal=how == "causal", mask=mask, lengths=lengths)
+    assert all(torch.equal(first[n], again[n]) for n in first)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("bad", [math.nan, math.inf])
 def test_a_mask_over_keys_alone_hides_what_is_not_finite(bad, dev):
     q, k, v, do = inputs(2, 4, 2, 50, 100, 64, torch.bfloat16, dev, seed=8)
