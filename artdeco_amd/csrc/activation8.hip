@@ -40,9 +40,10 @@ template <int KIND> __device__ __forceinline__ float a8_slope(float x, float& va
         value = x * c;
         return c + x * 0.39894228040143268f * __builtin_amdgcn_exp2f(-0.72134752044448170f * x * x);
     }
-    const float s = a8_sigmoid(x * (1.5957691216057308f + 0.071354816272600385f * x * x));
+    const float xx = fminf(x * x, 1e30f); // an infinite square would meet a zero below
+    const float s = a8_sigmoid(x * (1.5957691216057308f + 0.071354816272600385f * xx));
     value = x * s;
-    return s + x * s * (1.f - s) * (1.5957691216057308f + 0.21406444881780115f * x * x);
+    return s + x * s * (1.f - s) * (1.5957691216057308f + 0.21406444881780115f * xx);
 }
 
 template <typename T> __device__ __forceinline__ void a8_load(const T* p, float* v) {

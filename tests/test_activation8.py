@@ -112,6 +112,22 @@ def test_zeros_tiny_huge_and_not_finite(fmt, dev):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["gelu", "gelu_tanh", "silu"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_values_whose_squares_are_infinite(kind, dtype, dev):
+    """Far out the slope is 1 or 0; each value in a block of its own unit."""
+    from artdeco_amd import activation8 as a8
+    x = torch.zeros(8, 32)
+    x[:, 0] = torch.tensor([1e19, -1e19, 2e19, -2e19, 1e25, -1e25, 1e37, -1e37])
+    y, packed = a8.activation8_forward(x.to(dtype).to(dev), kind=kind)
+    dx, again = a8.activation8_backward(torch.ones(8, 32, dtype=dtype, device=dev), packed, kind=kind)
+    z = decode(packed)
+    close(dx, slope(z, kind), torch.ones_like(z), dtype)
+    close(again, act(z, kind), z.abs(), dtype)
+    close(y, act(x.to(dtype).double(), kind), x.double().abs(), dtype)
+
+
+@pytest.mark.gpu
 def test_rows_of_odd_width_at_odd_addresses(dev):
     """A contiguous tensor whose storage starts between 16-byte lines."""
     from artdeco_amd import activation8 as a8
