@@ -118,7 +118,7 @@ template <typename T, int W> static int rotary_launch(RotaryArgs& a, int half, h
     const int64_t units = a.axes * a.pairs / np + (a.copy ? (a.D - 2 * a.axes * a.pairs) / W : 0);
     const int64_t rest = a.copy ? (int64_t)(a.H - a.turned) * (a.D / W) : 0;
     a.slices = 1;
-    // Threads for two waves a SIMD, and at least 8 heads side by side.  More slices repeat the trigonometry (3072 tokens x 32 of 48 heads of 64:
+    // Threads for two waves a SIMD, and at least 8 heads side by side.  More slices repeat the trigonometry (4 x 768 tokens, 32 of 48 heads of 64:
     // 11.4 us with 32 slices, 9.8 with 16, 11.5 with 8), fewer leave a wave 256 bytes at a time (32749 x 32 heads of 128: 130 us with one, 113
     // with two, 99.7 with eight, 5.4 TB/s; 110 with sixteen); element by element (W = 1) the trigonometry is all that counts.
     while (a.slices < a.turned && (a.tokens * units * a.slices < 128 * 1024 || (W > 1 && a.slices < 8))) a.slices *= 2;
