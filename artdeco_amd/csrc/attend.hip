@@ -965,16 +965,21 @@ template <typename T> __global__ __launch_bounds__(256) void at_bwd_join_kernel(
 
 // -------------------------------------------------------------------------------------------------------------------- launches
 // Which shape, by the workgroups of 128 rows (or keys) that the wide one would have on the 256 CUs.
-// Forward, us, narrow | wide, at D 64; 128:  768 keys, 96 workgroups 11.1 | 18.1; 16.0 | 23.1.  192: 13.9 | 18.3; 26.0 | 24.4.  384: 24.7 |
-//   24.6; 46.5 | 35.5.  2048 keys, causal, 256: 23.9 | 39.9; 37.6 | 52.1.  8192 keys, 256: 125 | 146; 203 | 212.
+// Forward, us, narrow | wide, at D 64; 80; 128:  768 keys, 96 workgroups 11 | 18; 14 | 24; 16 | 23.  192: 15 | 19; 20 | 25; 25 | 24.  288: 20 | 25;
+//   30 | 32; 39 | 34.  384: 25 | 26; 37 | 34; 45 | 37.  480: 33 | 28; 45 | 34; 57 | 38.  2048 keys, 384: 49 | 55; 73 | 71; 90 | 73.  8192 keys, 256: 109 |
+//   146; 176 | 221; 199 | 210.  384: 163 | 198; 244 | 238; 299 | 256.  512: 210 | 195; 320 | 238; 391 | 284.  Causal (half the work, uneven), 2048 keys, 512: 40 |
+//   55; 57 | 70; 72 | 71.  8192 keys, 768: 185 | 212; 289 | 280; 339 | 280.  1024: 212 | 232; 330 | 297; 410 | 297; but 512 keys, 512: 20 | 18; 31 | 24; 39 | 26.
+//   Up to 32 rows (token by token in a large batch) three of the wide shape's four waves would have none: 4 rows, 2048 keys, 1024 key heads 116 | 116;
+//   124 | 161; 197 | 201.  (A half shape, as the backward has, gained at most 5 % at any of these.)
 // Backward, us, narrow | half | wide, at D 64; 80; 128, as many workgroups for rows as for keys:  768 x 768, 24: 13 | 19 | 26; 19 | 26 | 56; 19 |
 //   28 | 64.  48: 16 | 19 | 26; 32 | 26 | 57; 34 | 29 | 65.  96: 24 | 22 | 27; 48 | 28 | 58; 50 | 47 | 66.  144: 34 | 35 | 30; 77 | 47 | 59; 83 | 67 | 69.
 //   192: 39 | 38 | 31; 95 | 49 | 60; 101 | 75 | 71.  384: 75 | 60 | 54; 191 | 82 | 81; 198 | 139 | 122.  8192 x 8192, 128: 173 | 155 | 217; 513 | 210 |
 //   454; 549 | 352 | 534.  256: 328 | 289 | 248; 1052 | 405 | 468; 1059 | 702 | 541.
 static int64_t at_groups(int64_t bh, int64_t owned) { return bh * ceil_div(owned, 128); }
-static bool at_narrow_fwd(int64_t bh, int64_t R, int Nk, int D) {
-    const int64_t g = at_groups(bh, R);
-    return D <= 64 ? g < 384 : g <= 128 || (g <= 256 && Nk >= 1024);
+static bool at_narrow_fwd(int64_t bh, int64_t R, int Nk, int D, int causal) {
+    const int64_t g = at_groups(bh, R) / (causal && Nk >= 1024 ? 2 : 1);
+    if (R <= 32) return true;
+    return D <= 64 ? g <= 448 : D <= 96 ? g <= 320 : g <= 128 || (g <= 256 && Nk >= 4096);
 }
 // A causal call has half the work, unevenly spread, so its workgroups count half (16 heads of 2048 x 2048, backward, us, narrow | half | wide at
 // D 64; 80; 128: 60 | 60 | 63; 158 | 80 | 126; 175 | 123 | 149).
@@ -988,7 +993,7 @@ static int at_shape_bwd(int64_t bh, int64_t owned, int D, int causal) {
 // eight, 84.1 with sixteen); more rows: two, as the parts have to be joined.  At
 // least 256 keys a part.
 static int at_splits(int64_t bh, int64_t R, int Nk, int D) {
-    if (!at_narrow_fwd(bh, R, Nk, D)) return 1;
+    if (!at_narrow_fwd(bh, R, Nk, D, 0)) return 1; // whatever the order, so that the workspace is the same
     int64_t s = R <= 32 ? 1024 / bh : 512 / (bh * ceil_div(R, 32));
     if (s > Nk / 256) s = Nk / 256;
     return (int)(s < 1 ? 1 : s > 64 ? 64 : s);
@@ -1046,7 +1051,7 @@ static int at_tensor(const void* p, const int64_t* s) {
 
 template <typename T, int DP, bool MASKED> static void at_launch_fwd(const AttendArgs& a, hipStream_t stream) {
     const int64_t R = (int64_t)a.G * a.Nq;
-    if (at_narrow_fwd((int64_t)a.B * a.Hk, R, a.Nk, a.D)) hipLaunchKernelGGL((at_fwd_kernel<T, DP, MASKED, AT_NARROW>), dim3((unsigned)(ceil_div(R, 32) * a.B * a.Hk * a.splits)), dim3(256), 0, stream, a);
+    if (at_narrow_fwd((int64_t)a.B * a.Hk, R, a.Nk, a.D, a.causal)) hipLaunchKernelGGL((at_fwd_kernel<T, DP, MASKED, AT_NARROW>), dim3((unsigned)(ceil_div(R, 32) * a.B * a.Hk * a.splits)), dim3(256), 0, stream, a);
     else hipLaunchKernelGGL((at_fwd_kernel<T, DP, MASKED, AT_WIDE>), dim3((unsigned)(ceil_div(R, 128) * a.B * a.Hk)), dim3(256), 0, stream, a);
 }
 template <typename T, int DP, bool MASKED> static void at_launch_bwd(const AttendArgs& a, hipStream_t stream) {
