@@ -493,9 +493,6 @@ __global__ __launch_bounds__(256) void at_join_kernel(AttendArgs a)
 }
 
 // ------------------------------------------------------------------------------------------------------------------ backward
-// delta_i = <dO_i, o_i>, 16 lanes a row; and the largest |dO| of each block of 16 rows, from which the fp16 kernels take the
-// power of two that brings dS into fp16's range.
-#define AT_DELTA_ROWS 16
 // The mask as bits: by row, word (set, n, i) the keys 32 n + k of row i; by key, word (set, n, j) the rows 32 n + r that show key j.  A set
 // is a sequence's or a head's mask, one for all of them where it is broadcast; a mask that is the same for every query has one row, and its
 // words by key say so for 32.  The owners of rows and of keys then ask for one word each, side by side in memory, where the bytes of a
@@ -527,6 +524,10 @@ static __device__ __forceinline__ void at_mask_bits(const AttendArgs& a, int64_t
     const int row = 32 * n + (lane & 31), word = 2 * pair + (lane >> 5);
     if (row < a.mask_rows && word < kt) a.by_row[(set * kt + word) * a.mask_rows + row] = keys;
 }
+
+// delta_i = <dO_i, o_i>, 16 lanes a row; and the largest |dO| of each block of 16 rows, from which the fp16 kernels take the
+// power of two that brings dS into fp16's range.  Its last workgroups pack the mask.
+#define AT_DELTA_ROWS 16
 template <typename T>
 __global__ __launch_bounds__(256) void at_delta_kernel(AttendArgs a)
 {
