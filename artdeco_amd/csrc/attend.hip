@@ -1016,9 +1016,10 @@ static AtBwdPlan at_plan_bwd(int64_t bh, int64_t R, int64_t Nk, int D, int causa
         p.key_splits = parts(1024 / wk, R); // 128 x 4096 x 4 x 16 heads, D 64; 128, us, rows whole: 107; 201.  In 2: 86; 171.  4: 77; 165
         p.row_splits = parts(1024 / wr, Nk);
     } else { // together: none is to walk much further than a 512th of the whole, where that is worth the join (1024 x 1024 x 4 heads, D 64; 128:
-             // whole 16; 24 us, in 2 20; 38)
-        const int64_t fair = ceil_div(wr * Nk + wk * R, 512);
-        auto worth = [&](int64_t walked) { const int n = parts(walked / fair, walked); return n >= 3 || walked / n >= 4096 ? n : 1; };
+             // whole 16; 24 us, in 2 20; 38.  512 x 512 x 64/8 causal: 42; 64, in 2 36; 73.  6708 queries x 81 keys x 4 x 96/12, D 80; 128: 1910;
+             // 2220, in 2 1598; 1860)
+        const int64_t fair = ceil_div(wr * Nk + wk * R, 512), join = D <= 64 ? 1100 : 2100; // what the join costs, in rows (or keys) walked
+        auto worth = [&](int64_t walked) { return walked > fair + join ? parts(walked >= 2 * fair ? walked / fair : 2, walked) : 1; };
         p.key_splits = worth(R);
         p.row_splits = worth(Nk);
     }
