@@ -1068,7 +1068,7 @@ template <typename T, int DP, bool MASKED> static void at_launch_bwd(const Atten
     if constexpr (DP == 64) // 8 a CU: below, the tails of two launches cost more than the rows' third wave a SIMD brings
         if (sk == sr && gk + gr < 2048) { AT_BWD(AT_WIDE, 3, false, gk + gr); return; }
     if (gk) {
-        if (sk == AT_NARROW) { AT_BWD_CUT(AT_NARROW, 2, a.key_splits, gk); }
+        if (sk == AT_NARROW) AT_BWD(AT_NARROW, 2, true, gk); // few keys in a launch of their own: their walk is cut
         else if (sk == AT_HALF) { AT_BWD_CUT(AT_HALF, 2, a.key_splits, gk); }
         else AT_BWD(AT_WIDE, 2, false, gk);
     }
