@@ -60,12 +60,12 @@ struct AttendArgs {
     float* delta;           // [B, H, Nq]
     float* part_o;          // [splits, B, Hk, G Nq, D] (splits > 1)
     float* part_ml;         // [splits, B, Hk, G Nq, 2]
-    float* amax;            // largest |dout| of each block of at_delta_kernel
+    uint32_t* tops;         // fp16: from each block of at_delta_kernel, as at_top_word has them
     float *part_dq, *part_dk, *part_dv; // [row_splits, B, H, Nq, D], [key_splits, B, Hk, Nk, D] where there are several
     uint32_t *by_row, *by_key; // the mask's bits, as at_mask_bits writes them
     const int* key_lengths; // [B] or null
     const uint8_t* mask;    // or null
-    int B, H, Hk, G, Nq, Nk, D, splits, causal, mask_by_key, mask_rows, delta_blocks, row_splits, key_splits;
+    int B, H, Hk, G, Nq, Nk, D, splits, causal, mask_by_key, mask_rows, delta_blocks, unit_blocks, row_splits, key_splits;
     int64_t q_sb, q_sh, q_sn, k_sb, k_sh, k_sn, v_sb, v_sh, v_sn, g_sb, g_sh, g_sn; // element strides: batch, head, token
     int64_t dq_sb, dq_sh, dq_sn, dk_sb, dk_sh, dk_sn, dv_sb, dv_sh, dv_sn;
     int64_t m_sb, m_sh, m_sq, m_sk;
@@ -214,14 +214,14 @@ __device__ __forceinline__ uint32_t at_below_bits(int k0, int lim) {
 template <typename T, int DP, int SHAPE, int BUFS = 2> struct AtShared {
     T tiles[AtShape<SHAPE>::STREAMS][BUFS][2][AtShape<SHAPE>::TILE * DP]; // stream, buffer, tensor
     int tops[4];
-    float unit4[4];
+    uint32_t top4[4];
     float m[4][32], l[4][32];
 };
 template <typename T, int DP, int SHAPE> struct AtSharedKeys {
     static constexpr int S = AtShape<SHAPE>::STREAMS, TILE = AtShape<SHAPE>::TILE;
     T tiles[S][2][2][TILE * DP];
     float lse[S][2][TILE], delta[S][2][TILE];
-    float unit4[4];
+    uint32_t top4[4];
 };
 
 // The sum of `regs` values a lane over the streams' waves that own the same rows (or keys); the wave of stream n gets the values
@@ -525,52 +525,96 @@ static __device__ __forceinline__ void at_mask_bits(const AttendArgs& a, int64_t
     if (row < a.mask_rows && word < kt) a.by_row[(set * kt + word) * a.mask_rows + row] = keys;
 }
 
-// delta_i = <dO_i, o_i>, 16 lanes a row; and the largest |dO| of each block of 16 rows, from which the fp16 kernels take the
-// power of two that brings dS into fp16's range.  Its last workgroups pack the mask.
+// delta_i = <dO_i, o_i>, 16 lanes a row.  Its last workgroups pack the mask.
+//
+// fp16 holds dS = P (dP - delta) in a power of two that the launch also prepares: |dP - delta| is at most 2 |dO_i| |v_j| (2-norms; o is a mean
+// of the v), P at most 1, so the unit takes twice the largest |dO| times the largest |v| of a key head to 2^15 and nothing can leave fp16's
+// range.  An even softmax over 8192 keys then has its dS around 2^-2 of 2^15 / 8192 / sqrt(D), eleven binary places above the end of
+// fp16's normal range.  Both norms are of the key head's own rows and keys, so what a sequence gets does not depend on its neighbours in the
+// batch; rows that see no key, keys that no query sees and rows that are not finite do not count.  bf16 has fp32's range and needs none.
 #define AT_DELTA_ROWS 16
-template <typename T>
+#define AT_DELTA_KEYS 64
+typedef unsigned short at_u16x2 __attribute__((ext_vector_type(2))); // exponents (biased) of the largest |dO|^2 and |v|^2
+__device__ __forceinline__ at_u16x2 at_top_word(uint32_t w) { return __builtin_bit_cast(at_u16x2, w); }
+__device__ __forceinline__ unsigned short at_exponent(float square) { return square < INFINITY ? (unsigned short)(__float_as_uint(square) >> 23) : (unsigned short)0; }
+__device__ __forceinline__ at_u16x2 at_larger(at_u16x2 t, uint32_t w) { return __builtin_elementwise_max(t, at_top_word(w)); }
+template <int FROM> __device__ __forceinline__ at_u16x2 at_lanes_top(at_u16x2 t) { // of lanes FROM apart and more
+    for (int o = 32; o >= FROM; o >>= 1) t = at_larger(t, (uint32_t)__shfl_xor((int)__builtin_bit_cast(uint32_t, t), o));
+    return t;
+}
+// 2^(15 - x) with 2 |dO| |v| < 2^x
+__device__ __forceinline__ float at_unit(int grad, int value) {
+    if (grad == 0 || value == 0) return 1.f; // dP - delta is 0
+    return __uint_as_float((uint32_t)(127 + 14 - ((grad + value - 252 + 1) >> 1)) << 23);
+}
+
+template <typename T, bool WIDE> // WIDE: head sizes above 64, 16 lanes a key; else 8
 __global__ __launch_bounds__(256) void at_delta_kernel(AttendArgs a)
 {
     typedef typename AtEl<T>::x8 x8;
+    constexpr bool UNIT = __is_same(T, _Float16);
+    constexpr int LANES = WIDE ? 16 : 8, KEYS = UNIT ? AT_DELTA_KEYS * LANES / 256 : 0; // keys a thread has a chunk of
     if ((int)blockIdx.x >= a.delta_blocks) {
         at_mask_bits(a, 4 * (int64_t)(blockIdx.x - a.delta_blocks) + (threadIdx.x >> 6));
         return;
     }
-    const int64_t rows = (int64_t)a.B * a.H * a.Nq, at = (int64_t)blockIdx.x * AT_DELTA_ROWS + (threadIdx.x >> 4);
+    // fp16: a block's rows and keys are of one key head; otherwise rows of all of them.  (Rows are numbered in 30 bits.)
+    const uint32_t R = UNIT ? a.G * a.Nq : a.B * a.H * a.Nq;
+    const uint32_t part = UNIT ? blockIdx.x % a.unit_blocks : blockIdx.x, bkh = UNIT ? blockIdx.x / a.unit_blocks : 0, ub = bkh / a.Hk, ukh = bkh - ub * a.Hk;
+    const uint32_t in = part * AT_DELTA_ROWS + (threadIdx.x >> 4), list = in / a.Nq, i = in - list * a.Nq;
+    const uint32_t b = UNIT ? ub : list / a.H, head = UNIT ? ukh * a.G + list : list - b * a.H;
     const int d = (threadIdx.x & 15) * 8;
-    float sum = 0.f, top = 0.f;
-    if (at < rows && d < a.D) {
-        const int64_t bh = at / a.Nq, i = at - bh * a.Nq, head = bh % a.H, b = bh / a.H;
-        const x8 o = *reinterpret_cast<const x8*>(static_cast<const T*>(a.out_in) + ((b * a.Nq + i) * a.H + head) * a.D + d);
+    x8 v[KEYS ? KEYS : 1] = {}; // asked for first: all loads are under way together
+    if constexpr (UNIT) {
+        const int len = a.key_lengths ? min(max(a.key_lengths[ub], 0), a.Nk) : a.Nk, dv = (threadIdx.x % LANES) * 8;
+        const T* vb = static_cast<const T*>(a.v) + (int64_t)ub * a.v_sb + (int64_t)ukh * a.v_sh;
+        const uint8_t* mkey = a.mask_by_key ? a.mask + (int64_t)ub * a.m_sb + (int64_t)ukh * a.G * a.m_sh : nullptr;
+#pragma unroll
+        for (int n = 0; n < KEYS; ++n) {
+            const int key = (int)part * AT_DELTA_KEYS + n * (256 / LANES) + threadIdx.x / LANES;
+            if (key < len && dv < a.D && !(mkey && !mkey[key * a.m_sk])) v[n] = *reinterpret_cast<const x8*>(vb + key * a.v_sn + dv);
+        }
+    }
+    const uint32_t at = bkh * R + in;
+    float sum = 0.f, size = 0.f;
+    if (in < R && d < a.D) {
+        const x8 o = *reinterpret_cast<const x8*>(static_cast<const T*>(a.out_in) + (((int64_t)b * a.Nq + i) * a.H + head) * a.D + d);
         const x8 g = *reinterpret_cast<const x8*>(static_cast<const T*>(a.dout) + b * a.g_sb + head * a.g_sh + i * a.g_sn + d);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) { sum += (float)o[e] * (float)g[e]; top = fmaxf(top, fabsf((float)g[e])); }
+        for (int e = 0; e < 8; ++e) { sum += (float)o[e] * (float)g[e]; size += (float)g[e] * (float)g[e]; }
     }
-    for (int o = 8; o; o >>= 1) { sum += __shfl_xor(sum, o); top = fmaxf(top, __shfl_xor(top, o)); }
-    if (at < rows && (threadIdx.x & 15) == 0) a.delta[at] = sum;
-    __shared__ float tops[AT_DELTA_ROWS];
-    if ((threadIdx.x & 15) == 0) tops[threadIdx.x >> 4] = top;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int i = 1; i < AT_DELTA_ROWS; ++i) top = fmaxf(top, tops[i]);
-        a.amax[blockIdx.x] = top;
+    for (int o = 8; o; o >>= 1) sum += __shfl_xor(sum, o);
+    if (in < R && (threadIdx.x & 15) == 0) a.delta[at] = sum;
+    if constexpr (UNIT) {
+        for (int o = 8; o; o >>= 1) size += __shfl_xor(size, o);
+        at_u16x2 top = {in < R && a.lse[at] != -INFINITY ? at_exponent(size) : (unsigned short)0, 0};
+#pragma unroll
+        for (int n = 0; n < KEYS; ++n) {
+            float square = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) square += (float)v[n][e] * (float)v[n][e];
+            for (int o = LANES / 2; o; o >>= 1) square += __shfl_xor(square, o);
+            top.y = max(top.y, at_exponent(square));
+        }
+        __shared__ uint32_t tops[4];
+        top = at_lanes_top<8>(top);
+        if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = __builtin_bit_cast(uint32_t, top);
+        __syncthreads();
+        if (threadIdx.x == 0) a.tops[blockIdx.x] = __builtin_bit_cast(uint32_t, at_larger(at_larger(at_larger(top, tops[1]), tops[2]), tops[3]));
     }
 }
 
-// fp16 only: 2^e with 2^e max|dO| in [1, 2), over the rows of this key head.  dS = P (dP - delta) of a small gradient would fall
-// below fp16's normal range (6e-5), of a scaled loss leave it; both are linear in dO.  bf16 has fp32's range and needs none.
-template <typename T> __device__ __forceinline__ float at_grad_unit(const AttendArgs& a, int b, int kh, float* shared4) {
-    if (sizeof(T) == 2 && !__is_same(T, _Float16)) return 1.f;
-    const int64_t R = (int64_t)a.G * a.Nq, first = ((int64_t)b * a.Hk + kh) * R;
-    if (R == 0) return 1.f;
-    float top = 0.f;
-    for (int64_t n = first / AT_DELTA_ROWS + threadIdx.x; n <= (first + R - 1) / AT_DELTA_ROWS; n += 256) top = fmaxf(top, a.amax[n]);
-    for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-    if ((threadIdx.x & 63) == 0) shared4[threadIdx.x >> 6] = top;
+// The unit of this key head's dS.
+template <typename T> __device__ __forceinline__ float at_grad_unit(const AttendArgs& a, int b, int kh, uint32_t* shared4) {
+    if (!__is_same(T, _Float16) || a.Nq == 0) return 1.f;
+    const uint32_t* words = a.tops + ((int64_t)b * a.Hk + kh) * a.unit_blocks;
+    at_u16x2 top = {0, 0};
+    for (int n = threadIdx.x; n < a.unit_blocks; n += 256) top = at_larger(top, words[n]);
+    top = at_lanes_top<1>(top);
+    if ((threadIdx.x & 63) == 0) shared4[threadIdx.x >> 6] = __builtin_bit_cast(uint32_t, top);
     __syncthreads();
-    top = fmaxf(fmaxf(shared4[0], shared4[1]), fmaxf(shared4[2], shared4[3]));
-    if (!(top > 0.f) || top == INFINITY) return 1.f;
-    return __uint_as_float((254u - (__float_as_uint(top) >> 23)) << 23);
+    top = at_larger(at_larger(at_larger(at_top_word(shared4[0]), shared4[1]), shared4[2]), shared4[3]);
+    return at_unit(__builtin_amdgcn_readfirstlane(top.x), __builtin_amdgcn_readfirstlane(top.y));
 }
 
 // dQ: a wave owns 32 rows and walks the keys that they see.
@@ -585,7 +629,7 @@ template <typename T, int DP, bool MASKED, int SHAPE, bool SPLIT> __device__ __f
     const int R = a.G * a.Nq, tiles = (R + OWN - 1) / OWN;
     const AtWhere where = at_where(a, id, tiles, SPLIT ? a.row_splits : 1);
     const int tile = a.causal ? tiles - 1 - where.tile : where.tile, kh = where.kh, b = where.b;
-    const float unit = at_grad_unit<T>(a, b, kh, sh.unit4);
+    const float unit = at_grad_unit<T>(a, b, kh, sh.top4);
 
     const int len = a.key_lengths ? min(max(a.key_lengths[b], 0), a.Nk) : a.Nk;
     const int row = tile * OWN + sub * 32 + c, rowc = min(row, R - 1), g = rowc / a.Nq, i = rowc - g * a.Nq;
@@ -679,17 +723,17 @@ template <typename T, int DP, bool MASKED, int SHAPE, bool SPLIT> __device__ __f
 #pragma unroll
                 for (int db = 0; db < DP / 32; ++db) acc[db] = AtEl<T>::mfma(at_colfrag<T, DP>(tk, 32 * n + 16 * s, db, lane), ds[n][s], acc[db]);
     }
-    const float f = a.scale / unit;
+    const float f = 1.f / unit; // the unit is taken off first: scale / unit could be infinite
     const bool blind = lse == -INFINITY; // sees nothing: a gradient of zero whatever the (unread) products gave
     auto store = [&](int n, const float* o) {
         const int d = at_channel(n, h);
         if (SPLIT && a.row_splits > 1) {
-            if (d < a.D) *reinterpret_cast<at_f32x4*>(a.part_dq + (((int64_t)(where.split * a.B + b) * a.Hk + kh) * R + row) * a.D + d) = blind ? at_f32x4{0.f, 0.f, 0.f, 0.f} : at_f32x4{o[0] * f, o[1] * f, o[2] * f, o[3] * f};
+            if (d < a.D) *reinterpret_cast<at_f32x4*>(a.part_dq + (((int64_t)(where.split * a.B + b) * a.Hk + kh) * R + row) * a.D + d) = blind ? at_f32x4{0.f, 0.f, 0.f, 0.f} : at_f32x4{o[0] * f * a.scale, o[1] * f * a.scale, o[2] * f * a.scale, o[3] * f * a.scale};
             return;
         }
         x4 y;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) y[e] = blind ? (T)0.f : (T)(o[e] * f);
+        for (int e = 0; e < 4; ++e) y[e] = blind ? (T)0.f : (T)(o[e] * f * a.scale);
         if (d < a.D) *reinterpret_cast<x4*>(static_cast<T*>(a.dq) + (int64_t)b * a.dq_sb + (int64_t)head * a.dq_sh + (int64_t)i * a.dq_sn + d) = y;
     };
     float flat[DP / 2];
@@ -721,7 +765,7 @@ template <typename T, int DP, bool MASKED, int SHAPE, bool SPLIT> __device__ __f
     const int R = a.G * a.Nq, tiles = (a.Nk + OWN - 1) / OWN, off = a.Nk - a.Nq;
     const AtWhere where = at_where(a, id, tiles, SPLIT ? a.key_splits : 1);
     const int tile = where.tile, kh = where.kh, b = where.b; // causal: the first keys are seen by most rows, the long ones come first as they are
-    const float unit = at_grad_unit<T>(a, b, kh, sh.unit4);
+    const float unit = at_grad_unit<T>(a, b, kh, sh.top4);
     const int len = a.key_lengths ? min(max(a.key_lengths[b], 0), a.Nk) : a.Nk;
     const int k0 = tile * OWN, wave_k0 = k0 + sub * 32, key = wave_k0 + c;
 
@@ -880,20 +924,20 @@ template <typename T, int DP, bool MASKED, int SHAPE, bool SPLIT> __device__ __f
             if (t + STREAMS < t1) note(buf ^ 1);
         }
     }
-    const float f = a.scale / unit;
+    const float f = 1.f / unit;
     auto store = [&](int n, const float* x, const float* y) {
         const int d = at_channel(n, h);
         if (SPLIT && a.key_splits > 1) {
             const int64_t to = (((int64_t)(where.split * a.B + b) * a.Hk + kh) * a.Nk + key) * a.D + d;
             if (d < a.D) {
-                *reinterpret_cast<at_f32x4*>(a.part_dk + to) = at_f32x4{x[0] * f, x[1] * f, x[2] * f, x[3] * f};
+                *reinterpret_cast<at_f32x4*>(a.part_dk + to) = at_f32x4{x[0] * f * a.scale, x[1] * f * a.scale, x[2] * f * a.scale, x[3] * f * a.scale};
                 *reinterpret_cast<at_f32x4*>(a.part_dv + to) = at_f32x4{y[0], y[1], y[2], y[3]};
             }
             return;
         }
         x4 k4, v4;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) { k4[e] = (T)(x[e] * f); v4[e] = (T)y[e]; }
+        for (int e = 0; e < 4; ++e) { k4[e] = (T)(x[e] * f * a.scale); v4[e] = (T)y[e]; }
         if (d < a.D) {
             *reinterpret_cast<x4*>(static_cast<T*>(a.dk) + (int64_t)b * a.dk_sb + (int64_t)kh * a.dk_sh + (int64_t)key * a.dk_sn + d) = k4;
             *reinterpret_cast<x4*>(static_cast<T*>(a.dv) + (int64_t)b * a.dv_sb + (int64_t)kh * a.dv_sh + (int64_t)key * a.dv_sn + d) = v4;
@@ -1045,6 +1089,12 @@ static int at_check(int dtype, int B, int H, int Hk, int Nq, int Nk, int D, floa
     return 0;
 }
 
+// Blocks of at_delta_kernel that a key head has in fp16.
+static int at_unit_blocks(int64_t R, int64_t Nk) {
+    const int64_t rows = ceil_div(R, AT_DELTA_ROWS), keys = ceil_div(Nk, AT_DELTA_KEYS);
+    return (int)(rows > keys ? rows : keys);
+}
+
 // s: strides (batch, head, token)
 static int at_tensor(const void* p, const int64_t* s) {
     if (!p || ((uintptr_t)p & 15) || ((s[0] | s[1] | s[2]) & 7)) return ADK_EINVAL;
@@ -1091,7 +1141,8 @@ template <typename T> static int at_fwd(const AttendArgs& a, hipStream_t stream)
 
 template <typename T> static int at_bwd(const AttendArgs& a, hipStream_t stream) {
     const int64_t blocks = a.delta_blocks + (a.mask ? ceil_div(at_mask_waves(a), 4) : 0);
-    if (blocks) hipLaunchKernelGGL((at_delta_kernel<T>), dim3((unsigned)blocks), dim3(256), 0, stream, a);
+    if (blocks && a.D > 64) hipLaunchKernelGGL((at_delta_kernel<T, true>), dim3((unsigned)blocks), dim3(256), 0, stream, a);
+    else if (blocks) hipLaunchKernelGGL((at_delta_kernel<T, false>), dim3((unsigned)blocks), dim3(256), 0, stream, a);
     if (a.D <= 64) { if (a.mask) at_launch_bwd<T, 64, true>(a, stream); else at_launch_bwd<T, 64, false>(a, stream); }
     else if (a.D <= 96) { if (a.mask) at_launch_bwd<T, 96, true>(a, stream); else at_launch_bwd<T, 96, false>(a, stream); }
     else { if (a.mask) at_launch_bwd<T, 128, true>(a, stream); else at_launch_bwd<T, 128, false>(a, stream); }
@@ -1155,7 +1206,7 @@ extern "C" int64_t adk_attend_bwd_workspace_bytes(int B, int H, int Hk, int Nq, 
     const adk::AtBwdPlan p = adk::at_plan_bwd((int64_t)B * Hk, R, Nk, D, 0);
     const int rs = p.row_splits, ks = p.key_splits;
     const int64_t parts = (rs > 1 ? rs * rows * D : 0) + (ks > 1 ? 2 * ks * keys * D : 0);
-    return 4 * (parts + rows + adk::ceil_div(rows, AT_DELTA_ROWS));
+    return 4 * (parts + rows + (rows ? (int64_t)B * Hk * adk::at_unit_blocks(R, Nk) : 0));
 }
 
 extern "C" int64_t adk_attend_mask_bytes(int B, int H, int Nq, int Nk, const int64_t* strides)
@@ -1195,11 +1246,12 @@ extern "C" int adk_attend_bwd(const void* dout, const void* q, const void* k, co
         a.part_dk = a.part_dq + (a.row_splits > 1 ? a.row_splits * rows * D : 0);
         a.part_dv = a.part_dk + (a.key_splits > 1 ? a.key_splits * (int64_t)B * Hk * Nk * D : 0);
         a.delta = a.part_dv + (a.key_splits > 1 ? a.key_splits * (int64_t)B * Hk * Nk * D : 0);
-        a.amax = a.delta + rows;
-        a.delta_blocks = (int)adk::ceil_div(rows, AT_DELTA_ROWS);
+        a.tops = reinterpret_cast<uint32_t*>(a.delta + rows);
+        a.unit_blocks = adk::at_unit_blocks((int64_t)a.G * Nq, Nk);
+        a.delta_blocks = dtype == 0 ? B * Hk * a.unit_blocks : (int)adk::ceil_div(rows, AT_DELTA_ROWS);
         if (a.mask) {
             if (a.delta_blocks + adk::at_mask_waves(a) / 4 > 0x7ffffff0ll) return ADK_EUNSUPPORTED;
-            a.by_row = reinterpret_cast<uint32_t*>(a.amax + a.delta_blocks);
+            a.by_row = a.tops + (int64_t)B * Hk * a.unit_blocks;
             a.by_key = a.by_row + (adk::at_mask_set(a, B - 1, H - 1) + 1) * adk::at_words(Nk) * a.mask_rows;
             need += adk_attend_mask_bytes(B, H, Nq, Nk, strides + 9);
         }
