@@ -529,8 +529,8 @@ static __device__ __forceinline__ void at_mask_bits(const AttendArgs& a, int64_t
 //
 // fp16 holds dS = P (dP - delta) in a power of two that the launch also prepares: |dP - delta| is at most 2 |dO_i| |v_j| (2-norms; o is a mean
 // of the v), P at most 1, so the unit takes twice the largest |dO| times the largest |v| of a key head to 2^15 and nothing can leave fp16's
-// range.  An even softmax over 8192 keys then has its dS around 2^-2 of 2^15 / 8192 / sqrt(D), eleven binary places above the end of
-// fp16's normal range.  Both norms are of the key head's own rows and keys, so what a sequence gets does not depend on its neighbours in the
+// range.  An even softmax over 8192 keys then has its dS around 2^15 / 8192 / sqrt(D), about 2^-2, twelve binary places above the end of
+// fp16's normal range.  (For dQ the unit is the row's own, at_bwd_rows.)  Both norms are of the key head's own rows and keys, so what a sequence gets does not depend on its neighbours in the
 // batch; rows that see no key, keys that no query sees and rows that are not finite do not count.  bf16 has fp32's range and needs none.
 #define AT_DELTA_ROWS 16
 #define AT_DELTA_KEYS 64
@@ -604,9 +604,9 @@ __global__ __launch_bounds__(256) void at_delta_kernel(AttendArgs a)
     }
 }
 
-// The unit of this key head's dS.
-template <typename T> __device__ __forceinline__ float at_grad_unit(const AttendArgs& a, int b, int kh, uint32_t* shared4) {
-    if (!__is_same(T, _Float16) || a.Nq == 0) return 1.f;
+// The exponents of this key head.
+template <typename T> __device__ __forceinline__ at_u16x2 at_head_top(const AttendArgs& a, int b, int kh, uint32_t* shared4) {
+    if (!__is_same(T, _Float16) || a.Nq == 0) return at_u16x2{0, 0};
     const uint32_t* words = a.tops + ((int64_t)b * a.Hk + kh) * a.unit_blocks;
     at_u16x2 top = {0, 0};
     for (int n = threadIdx.x; n < a.unit_blocks; n += 256) top = at_larger(top, words[n]);
@@ -614,7 +614,16 @@ template <typename T> __device__ __forceinline__ float at_grad_unit(const Attend
     if ((threadIdx.x & 63) == 0) shared4[threadIdx.x >> 6] = __builtin_bit_cast(uint32_t, top);
     __syncthreads();
     top = at_larger(at_larger(at_larger(at_top_word(shared4[0]), shared4[1]), shared4[2]), shared4[3]);
-    return at_unit(__builtin_amdgcn_readfirstlane(top.x), __builtin_amdgcn_readfirstlane(top.y));
+    return at_top_word((uint32_t)__builtin_amdgcn_readfirstlane((int)__builtin_bit_cast(uint32_t, top)));
+}
+// The exponent of |dO|^2 of the row whose fragments the two lanes c and c + 32 hold.
+template <typename T, int DP> __device__ __forceinline__ int at_row_exponent(const typename AtEl<T>::x8* frag) {
+    float square = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < DP / 16; ++ks)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) square += (float)frag[ks][e] * (float)frag[ks][e];
+    return at_exponent(square + at_other_half(square));
 }
 
 // dQ: a wave owns 32 rows and walks the keys that they see.
@@ -629,7 +638,7 @@ template <typename T, int DP, bool MASKED, int SHAPE, bool SPLIT> __device__ __f
     const int R = a.G * a.Nq, tiles = (R + OWN - 1) / OWN;
     const AtWhere where = at_where(a, id, tiles, SPLIT ? a.row_splits : 1);
     const int tile = a.causal ? tiles - 1 - where.tile : where.tile, kh = where.kh, b = where.b;
-    const float unit = at_grad_unit<T>(a, b, kh, sh.top4);
+    const int value_top = at_head_top<T>(a, b, kh, sh.top4).y;
 
     const int len = a.key_lengths ? min(max(a.key_lengths[b], 0), a.Nk) : a.Nk;
     const int row = tile * OWN + sub * 32 + c, rowc = min(row, R - 1), g = rowc / a.Nq, i = rowc - g * a.Nq;
@@ -673,6 +682,8 @@ template <typename T, int DP, bool MASKED, int SHAPE, bool SPLIT> __device__ __f
         for (int ks = 0; ks < DP / 16; ++ks) { qf[ks] = at_global_frag<T>(qp, ks, lane, a.D); gf[ks] = at_global_frag<T>(gp, ks, lane, a.D); }
     }
     const int64_t at = ((int64_t)b * a.Hk + kh) * R + rowc;
+    // a row's dQ depends on no other row: its unit is its own (one for the key head cost a row of 1e-3 of the largest 2e-3 of its dQ at 8192 keys)
+    const float unit = __is_same(T, _Float16) ? at_unit(at_row_exponent<T, DP>(gf), value_top) : 1.f;
     const float lse = a.lse[at], neg_lse = lse == -INFINITY ? -INFINITY : -lse * 1.4426950408889634f, neg_delta = -a.delta[at] * unit;
     at_f32x16 acc[DP / 32] = {};
 
@@ -765,7 +776,8 @@ template <typename T, int DP, bool MASKED, int SHAPE, bool SPLIT> __device__ __f
     const int R = a.G * a.Nq, tiles = (a.Nk + OWN - 1) / OWN, off = a.Nk - a.Nq;
     const AtWhere where = at_where(a, id, tiles, SPLIT ? a.key_splits : 1);
     const int tile = where.tile, kh = where.kh, b = where.b; // causal: the first keys are seen by most rows, the long ones come first as they are
-    const float unit = at_grad_unit<T>(a, b, kh, sh.top4);
+    const at_u16x2 top = at_head_top<T>(a, b, kh, sh.top4);
+    const float unit = at_unit(top.x, top.y);
     const int len = a.key_lengths ? min(max(a.key_lengths[b], 0), a.Nk) : a.Nk;
     const int k0 = tile * OWN, wave_k0 = k0 + sub * 32, key = wave_k0 + c;
 

@@ -156,3 +156,13 @@ def test_a_sequence_beside_one_of_large_gradients(dev):
     both = gradients(q, k, v, do)
     alone = gradients(*(t[:1] for t in (q, k, v, do)))
     assert all(torch.equal(both[n][:1], alone[n]) for n in both)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("Nk", [1031, 8192])
+def test_a_row_of_a_huge_gradient_beside_others(Nk, dev):
+    """One row's gradient is 3e5 times the others': their dQ keeps the accuracy that it has without that row."""
+    q, k, v, do = tensors(1, 2, 1, 70, Nk, 64, dev, seed=9)
+    do *= 0.05
+    do[0, 1, 33] = (do[0, 1, 33].float() * 3e5).half()
+    check(gradients(q, k, v, do), norm_tolerances(q, k, v, do), names=("dq",), shows=4e-3)
