@@ -777,7 +777,9 @@ template <typename T, int DP, bool MASKED, int SHAPE, bool SPLIT> __device__ __f
     const AtWhere where = at_where(a, id, tiles, SPLIT ? a.key_splits : 1);
     const int tile = where.tile, kh = where.kh, b = where.b; // causal: the first keys are seen by most rows, the long ones come first as they are
     const at_u16x2 top = at_head_top<T>(a, b, kh, sh.top4);
-    const float unit = at_unit(top.x, top.y);
+    // fp16 holds P for dV times 2^14: an even softmax over 16384 keys ends fp16's normal range, and P is at most 1
+    constexpr float P_SHIFT = __is_same(T, _Float16) ? 14.f : 0.f, P_UNIT = __is_same(T, _Float16) ? 16384.f : 1.f;
+    const float unit = at_unit(top.x, top.y), unit_p = unit / P_UNIT; // P carries its own unit into dS
     const int len = a.key_lengths ? min(max(a.key_lengths[b], 0), a.Nk) : a.Nk;
     const int k0 = tile * OWN, wave_k0 = k0 + sub * 32, key = wave_k0 + c;
 
@@ -822,8 +824,8 @@ template <typename T, int DP, bool MASKED, int SHAPE, bool SPLIT> __device__ __f
         };
         auto note = [&](int buf) {
             if (brings) {
-                sh.lse[stream][buf][slot] = n_lse == -INFINITY ? -INFINITY : -n_lse * 1.4426950408889634f;
-                sh.delta[stream][buf][slot] = -n_delta * unit;
+                sh.lse[stream][buf][slot] = n_lse == -INFINITY ? -INFINITY : fmaf(-n_lse, 1.4426950408889634f, P_SHIFT);
+                sh.delta[stream][buf][slot] = -n_delta * unit_p;
             }
         };
         Tile::pad(sh.tiles[0][0][0], 2, a.D);
@@ -884,7 +886,7 @@ template <typename T, int DP, bool MASKED, int SHAPE, bool SPLIT> __device__ __f
                         const int r = 4 * r4 + e;
                         const float p = __builtin_amdgcn_exp2f(fmaf(st[n][r], a.scale_log2e, nl[e]));
                         pf[n][r >> 3][r & 7] = (T)p;
-                        df[n][r >> 3][r & 7] = (T)(p * fmaf(dp[n][r], unit, nd[e]));
+                        df[n][r >> 3][r & 7] = (T)(p * fmaf(dp[n][r], unit_p, nd[e]));
                     }
                 }
             };
@@ -943,13 +945,13 @@ template <typename T, int DP, bool MASKED, int SHAPE, bool SPLIT> __device__ __f
             const int64_t to = (((int64_t)(where.split * a.B + b) * a.Hk + kh) * a.Nk + key) * a.D + d;
             if (d < a.D) {
                 *reinterpret_cast<at_f32x4*>(a.part_dk + to) = at_f32x4{x[0] * f * a.scale, x[1] * f * a.scale, x[2] * f * a.scale, x[3] * f * a.scale};
-                *reinterpret_cast<at_f32x4*>(a.part_dv + to) = at_f32x4{y[0], y[1], y[2], y[3]};
+                *reinterpret_cast<at_f32x4*>(a.part_dv + to) = at_f32x4{y[0] / P_UNIT, y[1] / P_UNIT, y[2] / P_UNIT, y[3] / P_UNIT};
             }
             return;
         }
         x4 k4, v4;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) { k4[e] = (T)(x[e] * f * a.scale); v4[e] = (T)y[e]; }
+        for (int e = 0; e < 4; ++e) { k4[e] = (T)(x[e] * f * a.scale); v4[e] = (T)(y[e] / P_UNIT); }
         if (d < a.D) {
             *reinterpret_cast<x4*>(static_cast<T*>(a.dk) + (int64_t)b * a.dk_sb + (int64_t)kh * a.dk_sh + (int64_t)key * a.dk_sn + d) = k4;
             *reinterpret_cast<x4*>(static_cast<T*>(a.dv) + (int64_t)b * a.dv_sb + (int64_t)kh * a.dv_sh + (int64_t)key * a.dv_sn + d) = v4;

@@ -166,3 +166,12 @@ def test_a_row_of_a_huge_gradient_beside_others(Nk, dev):
     do *= 0.05
     do[0, 1, 33] = (do[0, 1, 33].float() * 3e5).half()
     check(gradients(q, k, v, do), norm_tolerances(q, k, v, do), names=("dq",), shows=4e-3)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("Nk", [40000, 300001])
+def test_probabilities_of_many_keys(Nk, dev):
+    """An even softmax over so many keys that each probability lies below fp16's normal range."""
+    q, k, v, do = tensors(1, 1, 1, 40, Nk, 64, dev, seed=8)
+    do = do * 1000
+    check(gradients(q, k, v, do), norm_tolerances(q, k, v, do), names=("dv",), shows=2e-3)
