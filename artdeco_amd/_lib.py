@@ -175,6 +175,13 @@ def launch(fn, what: str, device, *args) -> None:
         check(rc, what)
 
 
+def differentiated(*tensors) -> bool:
+    """Whether autograd follows a call on these tensors: one requires a gradient in grad mode, or a level of forward-mode differentiation is
+    open (a dual tensor requires none)."""
+    import torch
+    return torch.autograd.forward_ad._current_level >= 0 or (torch.is_grad_enabled() and any(t.requires_grad for t in tensors))
+
+
 def require_cuda(*tensors) -> None:
     for t in tensors:
         if t is not None and not t.is_cuda:

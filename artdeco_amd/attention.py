@@ -207,12 +207,13 @@ class _Attend(torch.autograd.Function):
 
 
 def attend(q, k, v, *, scale=None, causal=False, mask=None, key_lengths=None) -> torch.Tensor:
-    """attend_forward's out as part of autograd: differentiable once with respect to q, k and v.  -> [B,Nq,H*D].
+    """attend_forward's out as part of autograd: differentiable once with respect to q, k and v, in reverse mode (forward-mode
+    differentiation raises torch's error).  -> [B,Nq,H*D].
 
     A training step that is captured into a graph is captured whole, while no graph of the same leaves recorded outside it is alive
     (autograd would wait for the stream that one was recorded on, which ends the capture); attend_forward and attend_backward have no
     such tie."""
-    if not (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)):
+    if not _lib.differentiated(q, k, v):
         return attend_forward(q, k, v, scale=scale, causal=causal, mask=mask, key_lengths=key_lengths)[0]
     return _Attend.apply(q, k, v, scale, causal, mask, key_lengths)
 
@@ -249,6 +250,6 @@ def attend_packed(qkv, heads, kv_heads=None, *, scale=None, causal=False, mask=N
     kv_heads = heads if kv_heads is None else kv_heads
     if qkv.dim() != 4 or heads < 1 or kv_heads < 1 or qkv.shape[2] != heads + 2 * kv_heads:
         raise _lib.AdkError(f"attend_packed: qkv [B,N,heads + 2 kv_heads,D] is required; got {tuple(qkv.shape)} for {heads} and {kv_heads} heads")
-    if not (torch.is_grad_enabled() and qkv.requires_grad):
+    if not _lib.differentiated(qkv):
         return attend_forward(*_packed_views(qkv, heads, kv_heads), scale=scale, causal=causal, mask=mask, key_lengths=key_lengths)[0]
     return _AttendPacked.apply(qkv, heads, kv_heads, scale, causal, mask, key_lengths)

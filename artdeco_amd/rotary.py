@@ -105,10 +105,6 @@ def _turn(x, y, positions, frequencies, factor, layout, heads, transpose):
     return y
 
 
-def _recorded(x):
-    return torch.is_grad_enabled() and x.requires_grad
-
-
 class _Rotary(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, positions, frequencies, factor, layout, heads, transpose, inplace):
@@ -132,21 +128,22 @@ class _Rotary(torch.autograd.Function):
 
 def rotary(x, positions, frequencies, *, factor=1.0, layout="half", heads=None) -> torch.Tensor:
     """x [B,N,H,D] (float16, bfloat16 or float32, dense last dimension) with the first `heads` heads (all if None) turned, as a new
-    contiguous tensor; the other channels and heads are copied.  positions int64 [N], [B,N] or [B,N,axes].  Differentiable."""
-    if not _recorded(x):
+    contiguous tensor; the other channels and heads are copied.  positions int64 [N], [B,N] or [B,N,axes].  Differentiable
+    (in reverse mode; forward-mode differentiation raises torch's error, as in rotary_ and rotary_transpose)."""
+    if not _lib.differentiated(x):
         return _turn(x, None, positions, frequencies, factor, layout, heads, False)
     return _Rotary.apply(x, positions, frequencies, factor, layout, heads, False, False)
 
 
 def rotary_(x, positions, frequencies, *, factor=1.0, layout="half", heads=None) -> torch.Tensor:
     """rotary in place: what is not turned is not touched.  -> x."""
-    if _recorded(x) and x.is_leaf:
+    if torch.is_grad_enabled() and x.requires_grad and x.is_leaf:
         raise _lib.AdkError("rotary_: x is a leaf that requires a gradient: turn it out of place, with rotary")
     return _Rotary.apply(x, positions, frequencies, factor, layout, heads, False, True)
 
 
 def rotary_transpose(x, positions, frequencies, *, factor=1.0, layout="half", heads=None) -> torch.Tensor:
     """The transpose of rotary, which is the gradient's form: the same pairs turned back, times factor."""
-    if not _recorded(x):
+    if not _lib.differentiated(x):
         return _turn(x, None, positions, frequencies, factor, layout, heads, True)
     return _Rotary.apply(x, positions, frequencies, factor, layout, heads, True, False)
