@@ -123,7 +123,7 @@ template <typename T, int DP> __device__ __forceinline__ typename AtEl<T>::x8 at
 // builtin's loads before any LDS read; the waits are at_landed() before a tile is read.  The address is a
 // uniform base and a 32-bit byte offset (token strides are below 2^24 elements).
 __device__ __forceinline__ void at_lds16(uint32_t lds, const void* base, uint32_t offset) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(offset), "s"(base) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(offset), "s"(base) : "memory", "m0");
 }
 // the wave's tiles are in LDS (all but its last `later` loads), and its reads of earlier ones are done, so that what it loads next
 // may take their place
