@@ -106,6 +106,13 @@ def _trains(module, x) -> bool:
     return getattr(module, "trains", False) and torch.is_grad_enabled() and x.is_cuda
 
 
+def _plain(module, kind) -> bool:
+    """Whether calling the module does what its class says and nothing else: no subclass (an adapter, a parametrised weight), no hook."""
+    m = module
+    return type(m) is kind and "forward" not in m.__dict__ and not (m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks
+                                                                    or nn.modules.module._has_any_global_hook())
+
+
 class Mlp(nn.Module):
     kept8 = None   # "int8" / "e4m3": the hidden values are kept for the backward pass in 8 bits (to_training_dtype)
 
@@ -116,9 +123,12 @@ class Mlp(nn.Module):
         self.fc2 = nn.Linear(hidden_features or in_features, out_features or in_features)
 
     def forward(self, x):
-        if self.kept8 is not None and _trains(self, x):
-            from artdeco_amd.activation8 import mlp8
-            return mlp8(x.to(self.fc1.weight.dtype), self.fc1.weight, self.fc1.bias, self.fc2.weight, self.fc2.bias, format=self.kept8)
+        if self.kept8 is not None and _trains(self, x) and _plain(self.act, nn.GELU):
+            from artdeco_amd.activation8 import activation8, mlp8
+            x, how = x.to(self.fc1.weight.dtype), dict(kind="gelu_tanh" if self.act.approximate == "tanh" else "gelu", format=self.kept8)
+            if _plain(self.fc1, nn.Linear) and _plain(self.fc2, nn.Linear):
+                return mlp8(x, self.fc1.weight, self.fc1.bias, self.fc2.weight, self.fc2.bias, **how)
+            return self.fc2(activation8(self.fc1(x).contiguous(), **how))   # what hangs on the layers is called; fc2 keeps its input
         return self.fc2(self.act(self.fc1(x.to(self.fc1.weight.dtype))))
 
 
@@ -571,7 +581,8 @@ class AsymmetricMASt3R(nn.Module):
         """For fine-tuning: the trunk's Linear and patch-embedding weights in `dtype` (float16 or bfloat16), products accumulated in
         fp32, residual stream, LayerNorms and softmax in fp32 as to_inference_dtype(fp32_stream=True) has them, and the blocks'
         attention, rotary positions and MLPs on kernels with a gradient.  kept8 ("int8" / "e4m3"): the MLPs keep their hidden values in 8
-        bits for the backward pass.  The heads stay fp32.  training_forward() then gives results with a graph; forward() stays
+        bits for the backward pass (an fc1 or fc2 that is hooked or replaced is called as it is, and then also keeps fc2's input; an activation
+        that is, as without kept8).  The heads stay fp32.  training_forward() then gives results with a graph; forward() stays
         without."""
         if dtype not in (torch.float16, torch.bfloat16):
             raise ValueError(f"to_training_dtype: float16 or bfloat16; got {dtype}")

@@ -33,3 +33,56 @@ def test_forward_mode_differentiation_is_refused(launches):
     assert ro.rotary(x.requires_grad_(True), pos, f).requires_grad
     with torch.no_grad():
         assert not ro.rotary(x, pos, f).requires_grad
+
+
+class Adapted(torch.nn.Linear):
+    """A Linear with something beside it, as adapters have it."""
+    def __init__(self, inner):
+        super().__init__(inner.in_features, inner.out_features)
+        self.load_state_dict(inner.state_dict())
+        self.called = 0
+
+    def forward(self, x):
+        self.called += 1
+        return super().forward(x)
+
+
+@pytest.mark.parametrize("layer", ["fc1", "fc2", "act"])
+def test_an_mlp_that_keeps_8_bits_calls_what_hangs_on_its_layers(layer, launches, monkeypatch):
+    """Hooks of each kind, an adapter in a layer's place, a forward of its own; without them the layers are one operator."""
+    from artdeco_amd import mast3r_model as mm
+    monkeypatch.setattr(mm, "_trains", lambda module, x: True)
+    x = torch.randn(2, 3, 8, requires_grad=True)
+
+    def fresh():
+        mlp = mm.Mlp(8, 16)
+        mlp.kept8 = "int8"
+        return mlp, getattr(mlp, layer)
+    forwards = lambda: [n for n, _ in launches].count("adk_activation8_fwd")  # noqa: E731
+    mlp, _ = fresh()
+    assert type(mlp(x).grad_fn).__name__ == "_Mlp8Backward" and forwards() == 1
+    seen = []
+    for hang in (lambda m: m.register_forward_hook(lambda *a: seen.append(1)), lambda m: m.register_forward_pre_hook(lambda *a: seen.append(1)),
+                 lambda m: m.register_full_backward_hook(lambda *a: seen.append(1)), lambda m: m.register_full_backward_pre_hook(lambda *a: seen.append(1))):
+        mlp, m = fresh()
+        seen.clear()
+        launches.clear()
+        hang(m)
+        mlp(x).sum().backward()
+        assert seen == [1] and forwards() == (0 if layer == "act" else 1)
+    mlp, m = fresh()
+    m.forward = lambda t, f=m.forward: (seen.append(2), f(t))[1]
+    mlp(x).sum().backward()
+    assert seen[-1] == 2
+    if layer != "act":
+        mlp, m = fresh()
+        setattr(mlp, layer, Adapted(m))
+        mlp(x).sum().backward()
+        assert getattr(mlp, layer).called == 1 and getattr(mlp, layer).weight.grad is not None
+    handle = torch.nn.modules.module.register_module_forward_hook(lambda m, *a: seen.append(type(m).__name__))
+    try:
+        seen.clear()
+        fresh()[0](x)
+        assert {"Linear", "GELU"} <= set(seen)
+    finally:
+        handle.remove()
