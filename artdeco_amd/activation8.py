@@ -122,17 +122,26 @@ class _Mlp8(torch.autograd.Function):
         nx, nw1, nb1, nw2, nb2 = ctx.needs_input_grad[:5]
         g2 = grad.reshape(-1, grad.shape[-1])
         dx = dw1 = db1 = dw2 = None
-        if nx or nw1 or nb1 or nw2:
-            dh, y = activation8_backward(torch.mm(g2, w2).view(*shape[:-1], w2.shape[1]), Packed8(codes, units, shape, dtype, format), kind=kind, gated=gated, again=nw2)
-            dh = dh.view(-1, dh.shape[-1])
-            dx = torch.mm(dh, w1).view(x.shape) if nx else None
-            dw1 = torch.mm(dh.t(), x.reshape(-1, x.shape[-1])) if nw1 else None
-            db1 = dh.sum(0) if nb1 else None
-            dw2 = torch.mm(g2.t(), y.view(-1, y.shape[-1])) if nw2 else None
-        return dx, dw1, db1, dw2, g2.sum(0) if nb2 else None, None, None, None
+        with torch.autocast(grad.device.type, enabled=False):  # all of one type: the products are to stay in it
+            if nx or nw1 or nb1 or nw2:
+                dh, y = activation8_backward(torch.mm(g2, w2).view(*shape[:-1], w2.shape[1]), Packed8(codes, units, shape, dtype, format), kind=kind, gated=gated, again=nw2)
+                dh = dh.view(-1, dh.shape[-1])
+                dx = torch.mm(dh, w1).view(x.shape) if nx else None
+                dw1 = torch.mm(dh.t(), x.reshape(-1, x.shape[-1])) if nw1 else None
+                db1 = dh.sum(0) if nb1 else None
+                dw2 = torch.mm(g2.t(), y.view(-1, y.shape[-1])) if nw2 else None
+            return dx, dw1, db1, dw2, g2.sum(0) if nb2 else None, None, None, None
 
 
 def mlp8(x, w1, b1, w2, b2, *, kind="gelu", gated=False, format="int8") -> torch.Tensor:
     """act(x w1^T + b1) w2^T + b2 (gated: w1's outputs are gate and up halves), keeping x and 8 bits a hidden value for the backward pass.
-    x, weights and biases (or None) of one type.  The four products of the gradient are the library's."""
-    return _Mlp8.apply(x, w1, b1, w2, b2, kind, gated, format)
+    x, weights and biases (or None) of one type; under autocast of any, and taken in autocast's, as linear layers are.  The four products of the
+    gradient are the library's."""
+    given, device = (x, w1, b1, w2, b2), x.device.type
+    if torch.is_autocast_enabled(device):
+        dtype = torch.get_autocast_dtype(device)
+        given = tuple(t.to(dtype) if t is not None and t.dtype in _DTYPES else t for t in given)
+    if any(t is not None and t.dtype != given[0].dtype for t in given):
+        raise _lib.AdkError(f"mlp8: x, weights and biases are of one type; got {', '.join('none' if t is None else str(t.dtype) for t in given)}")
+    with torch.autocast(device, enabled=False):
+        return _Mlp8.apply(*given, kind, gated, format)

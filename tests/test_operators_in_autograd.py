@@ -86,3 +86,18 @@ def test_an_mlp_that_keeps_8_bits_calls_what_hangs_on_its_layers(layer, launches
         assert {"Linear", "GELU"} <= set(seen)
     finally:
         handle.remove()
+
+
+def test_mlp8_takes_autocasts_type_and_refuses_a_mixture(launches):
+    from artdeco_amd import _lib, activation8 as a8
+    x, w1, b1, w2, b2 = (torch.randn(s, requires_grad=True) for s in ((2, 8), (16, 8), (16,), (4, 16), (4,)))
+    with torch.autocast("cpu", dtype=torch.bfloat16):
+        out = a8.mlp8(x, w1, b1.bfloat16(), w2, b2)
+    assert out.dtype == torch.bfloat16
+    assert all(g.dtype == torch.float32 for g in torch.autograd.grad(out, (x, w1, w2, b2), torch.ones_like(out)))
+    out = a8.mlp8(x, w1, b1, w2, b2)
+    with torch.autocast("cpu", dtype=torch.bfloat16):
+        assert all(g.dtype == torch.float32 for g in torch.autograd.grad(out, (x, w1, b1, w2, b2), torch.ones_like(out)))
+    for bad in ((x.half(), w1, b1, w2, b2), (x, w1, b1, w2.double(), b2), (x, w1, b1, w2, b2.half())):
+        with pytest.raises(_lib.AdkError, match="of one type"):
+            a8.mlp8(*bad)

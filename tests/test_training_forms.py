@@ -1,0 +1,40 @@
+"""The operators for fine-tuning in the forms that training programs call them: autocast, frozen parameters, adapters, masks on packed
+projections, validation between steps.
+
+Tolerances: where two ways make the same launches on the same operands the bits are the same; otherwise as said at each test."""
+import pytest
+import torch
+
+U = {torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8, torch.float32: 2.0 ** -24}
+
+
+def mlp_leaves(dev, dtype=torch.float32, gated=False, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    W = 96 * (2 if gated else 1)
+    make = lambda *s, size=1.0: (torch.randn(*s, generator=g) * size).to(dtype).to(dev).requires_grad_(True)  # noqa: E731
+    return [make(2, 9, 32), make(W, 32, size=0.2), make(W), make(24, 96, size=0.2), make(24)], (torch.randn(2, 9, 24, generator=g)).to(dev)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_mlp8_under_autocast(dtype, dev):
+    """float32 leaves, and leaves of several types: the call and the gradients of the same operands cast by hand; backward inside the region
+    too, also for a call that was made outside it."""
+    from artdeco_amd import activation8 as a8
+    leaves, grad = mlp_leaves(dev)
+    cast = [t.detach().to(dtype).requires_grad_(True) for t in leaves]
+    out = a8.mlp8(*cast)
+    want = torch.autograd.grad(out, cast, grad.to(dtype))
+    mixed = [leaves[0].detach().to(dtype).requires_grad_(True)] + leaves[1:]
+    for operands in (leaves, mixed):
+        with torch.autocast("cuda", dtype=dtype):
+            got = a8.mlp8(*operands)
+            assert got.dtype == dtype and torch.equal(got, out)
+            inside = torch.autograd.grad(got, operands, grad.to(dtype), retain_graph=True)
+        for grads in (inside, torch.autograd.grad(got, operands, grad.to(dtype))):
+            assert all(torch.equal(a, b.to(a.dtype)) and a.dtype == t.dtype for a, b, t in zip(grads, want, operands))
+    plain = a8.mlp8(*leaves)
+    first = torch.autograd.grad(plain, leaves, grad, retain_graph=True)
+    with torch.autocast("cuda", dtype=dtype):
+        again = torch.autograd.grad(plain, leaves, grad)
+    assert all(torch.equal(a, b) for a, b in zip(first, again))
