@@ -43,9 +43,8 @@ def _names(what, kind, format):
         raise _lib.AdkError(f"{what}: format is int8 or e4m3; got {format!r}")
 
 
-def activation8_forward(x, *, kind="gelu", gated=False, format="int8"):
-    """-> (act(x), or act(gate) * up for x's halves, in x's type; x as Packed8), outside autograd.  x contiguous, float16, bfloat16 or
-    float32.  Infinities are held as the format's largest value in their block, NaN as NaN."""
+def _forward(x, kind, gated, format, keep):
+    """-> (act(x), x as Packed8 or None without `keep`)."""
     _names("activation8", kind, format)
     if x.dtype not in _DTYPES or not x.is_contiguous():
         raise _lib.AdkError(f"activation8: a contiguous float16, bfloat16 or float32 tensor is required; got {x.dtype}, strides {x.stride()}")
@@ -55,11 +54,17 @@ def activation8_forward(x, *, kind="gelu", gated=False, format="int8"):
     shape, dtype, device = x.shape, x.dtype, x.device
     blocks = -(-x.numel() // 32)
     y = torch.empty((*shape[:-1], width), dtype=dtype, device=device)
-    codes = torch.empty(32 * blocks, dtype=torch.uint8, device=device)
-    units = torch.empty(blocks, dtype=torch.uint8, device=device)
+    codes = torch.empty(32 * blocks, dtype=torch.uint8, device=device) if keep else None
+    units = torch.empty(blocks, dtype=torch.uint8, device=device) if keep else None
     _lib.launch(_lib.load().adk_activation8_fwd, "adk_activation8_fwd", device, x.data_ptr(), _DTYPES[dtype], rows, width, _KINDS[kind], gated, _FORMATS[format],
-                y.data_ptr(), codes.data_ptr(), units.data_ptr())
-    return y, Packed8(codes, units, shape, dtype, format)
+                y.data_ptr(), _lib.ptr(codes), _lib.ptr(units))
+    return y, Packed8(codes, units, shape, dtype, format) if keep else None
+
+
+def activation8_forward(x, *, kind="gelu", gated=False, format="int8"):
+    """-> (act(x), or act(gate) * up for x's halves, in x's type; x as Packed8), outside autograd.  x contiguous, float16, bfloat16 or
+    float32.  Infinities are held as the format's largest value in their block, NaN as NaN."""
+    return _forward(x, kind, gated, format, True)
 
 
 def activation8_backward(grad, packed, *, kind="gelu", gated=False, again=True):
@@ -102,7 +107,9 @@ class _Activation8(torch.autograd.Function):
 
 
 def activation8(x, *, kind="gelu", gated=False, format="int8") -> torch.Tensor:
-    """activation8_forward's result as part of autograd, which keeps x in 8 bits."""
+    """activation8_forward's result as part of autograd, which keeps x in 8 bits (nothing where no gradient is recorded)."""
+    if not _lib.differentiated(x):
+        return _forward(x, kind, gated, format, False)[0]
     return _Activation8.apply(x, kind, gated, format)
 
 
@@ -144,4 +151,6 @@ def mlp8(x, w1, b1, w2, b2, *, kind="gelu", gated=False, format="int8") -> torch
     if any(t is not None and t.dtype != given[0].dtype for t in given):
         raise _lib.AdkError(f"mlp8: x, weights and biases are of one type; got {', '.join('none' if t is None else str(t.dtype) for t in given)}")
     with torch.autocast(device, enabled=False):
+        if not _lib.differentiated(*(t for t in given if t is not None)):
+            return F.linear(_forward(F.linear(*given[:3]), kind, gated, format, False)[0], *given[3:])
         return _Mlp8.apply(*given, kind, gated, format)

@@ -103,7 +103,8 @@ template <bool E4M3> __device__ __forceinline__ void a8_decode(const A8Codes& c,
 }
 __device__ __forceinline__ float a8_unit_value(int unit) { return __uint_as_float((uint32_t)unit << 23); }
 
-// A thread's 8 consecutive values, from value i of the flat tensor on.  width: columns of the gate (0: not gated).
+// A thread's 8 consecutive values, from value i of the flat tensor on.  width: columns of the gate (0: not gated).  codes: null where nothing is
+// kept (16384 x 2 x 5461 bf16, gated: 114 us, 164 where x is kept).
 template <typename T, int KIND, bool E4M3, bool GATED>
 __global__ __launch_bounds__(256) void a8_fwd_kernel(const T* __restrict__ x, int64_t n, int64_t width, T* __restrict__ y, uint8_t* __restrict__ codes,
                                                      uint8_t* __restrict__ units)
@@ -116,15 +117,17 @@ __global__ __launch_bounds__(256) void a8_fwd_kernel(const T* __restrict__ x, in
     else
         for (int j = 0; j < 8; ++j)
             if (i + j < n) v[j] = (float)x[i + j];
-    float top = 0.f;
+    if (codes) {
+        float top = 0.f;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(v[j]) < INFINITY ? fabsf(v[j]) : 0.f);
-    top = fmaxf(top, __shfl_xor(top, 1));
-    top = fmaxf(top, __shfl_xor(top, 2));
-    if (i >= ((n + 31) & ~(int64_t)31)) return; // the codes' room ends with the last block
-    const int unit = a8_unit<E4M3>(top);
-    *reinterpret_cast<A8Codes*>(codes + i) = a8_encode<E4M3>(v, unit);
-    if ((i & 31) == 0) units[i >> 5] = (uint8_t)unit;
+        for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(v[j]) < INFINITY ? fabsf(v[j]) : 0.f);
+        top = fmaxf(top, __shfl_xor(top, 1));
+        top = fmaxf(top, __shfl_xor(top, 2));
+        if (i >= ((n + 31) & ~(int64_t)31)) return; // the codes' room ends with the last block
+        const int unit = a8_unit<E4M3>(top);
+        *reinterpret_cast<A8Codes*>(codes + i) = a8_encode<E4M3>(v, unit);
+        if ((i & 31) == 0) units[i >> 5] = (uint8_t)unit;
+    }
     if (!GATED) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = a8_value<KIND>(v[j]);
@@ -264,7 +267,7 @@ extern "C" int adk_activation8_fwd(const void* x, int dtype, int64_t rows, int64
     const int e = adk::a8_check(dtype, rows, width, kind, gated, format);
     if (e) return e;
     if (rows == 0 || width == 0) return 0;
-    if (!x || !y || !codes || !units || ((uintptr_t)codes & 7)) return ADK_EINVAL;
+    if (!x || !y || !codes != !units || ((uintptr_t)codes & 7)) return ADK_EINVAL;
     adk::A8Call c = {};
     c.x = x; c.y = y; c.codes = codes; c.units = units;
     c.n = rows * width * (gated ? 2 : 1); c.width = gated ? width : 0;

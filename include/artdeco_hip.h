@@ -345,7 +345,7 @@ int adk_rotary(const void* x, void* y, const int64_t* positions, const double* f
  * Forward: y = act(x), x [rows, width]; gated: act(x[:, :width]) * x[:, width:], x [rows, 2 width]; and x as codes, 32 consecutive
  * values of the contiguous tensor sharing the power of two 2^(units - 127).  kind 0 = gelu, 1 = gelu (tanh), 2 = silu; format 0 =
  * int8, 1 = e4m3; dtype 0 = float16, 1 = float32, 2 = bfloat16.  codes: n values rounded up to a multiple of 32 bytes, 8-byte
- * aligned; units: one byte for each 32.  Backward: dx in x's shape and, unless NULL, the activation of the held values
+ * aligned; units: one byte for each 32; both NULL in the forward where nothing is to be kept.  Backward: dx in x's shape and, unless NULL, the activation of the held values
  * (again, y's shape).  All contiguous.  No reference counterpart (croco/models/blocks.py: Mlp is the activation's place).
  */
 int adk_activation8_fwd(const void* x, int dtype, int64_t rows, int64_t width, int kind, int gated, int format, void* y, uint8_t* codes,

@@ -101,3 +101,25 @@ def test_mlp8_takes_autocasts_type_and_refuses_a_mixture(launches):
     for bad in ((x.half(), w1, b1, w2, b2), (x, w1, b1, w2.double(), b2), (x, w1, b1, w2, b2.half())):
         with pytest.raises(_lib.AdkError, match="of one type"):
             a8.mlp8(*bad)
+
+
+def test_nothing_is_kept_where_no_gradient_is_recorded(launches):
+    from artdeco_amd import activation8 as a8
+    x, w = torch.randn(4, 8), torch.randn(8, 8)
+    kept = lambda: [args[-2:] for _, args in launches][-1]  # noqa: E731  (codes, units)
+    with torch.no_grad():
+        a8.activation8(x.clone().requires_grad_(True))
+        assert kept() == (None, None)
+    a8.mlp8(x, w, None, w, None)
+    assert kept() == (None, None)
+    a8.activation8(x.clone().requires_grad_(True))
+    assert None not in kept()
+    a8.mlp8(x, w, None, w.clone().requires_grad_(True), None)
+    assert None not in kept()
+    a8.activation8_forward(x)
+    assert None not in kept()
+
+
+def test_the_activations_c_entry_keeps_both_codes_and_units_or_neither(lib):
+    P, N = 1 << 20, None
+    assert lib.adk_activation8_fwd(P, 0, 1, 1, 0, 0, 0, P, P, N, N) == -1 and lib.adk_activation8_fwd(P, 0, 1, 1, 0, 0, 0, P, N, P, N) == -1

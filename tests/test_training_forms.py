@@ -38,3 +38,20 @@ def test_mlp8_under_autocast(dtype, dev):
     with torch.autocast("cuda", dtype=dtype):
         again = torch.autograd.grad(plain, leaves, grad)
     assert all(torch.equal(a, b) for a, b in zip(first, again))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("shape,gated", [((1, 1), False), ((3, 7, 41), False), ((5, 26), True), ((257, 1000), True)], ids=str)
+def test_values_without_a_checkpoint(shape, gated, dtype, dev):
+    """The same bits as with one."""
+    from artdeco_amd import activation8 as a8
+    g = torch.Generator().manual_seed(1)
+    x = torch.randn(shape, generator=g).to(dtype).to(dev)
+    for kind in ("gelu", "gelu_tanh", "silu"):
+        want, _ = a8.activation8_forward(x, kind=kind, gated=gated)
+        assert torch.equal(a8.activation8(x, kind=kind, gated=gated), want)
+    leaves, _ = mlp_leaves(dev, dtype, gated)
+    with torch.no_grad():
+        got = a8.mlp8(*leaves, gated=gated)
+    assert torch.equal(got, a8.mlp8(*leaves, gated=gated).detach()) and not got.requires_grad
