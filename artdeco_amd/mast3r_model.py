@@ -444,11 +444,15 @@ class AsymmetricMASt3R(nn.Module):
         ckpt = {k: v for k, v in ckpt.items() if not k.startswith("prediction_head")}
         return super().load_state_dict(ckpt, **kw)
 
+    def _records(self) -> bool:
+        """Whether a pass of the model set up for training is recorded; its passes without a graph (validation) are the inference path's."""
+        return getattr(self, "_training_ops", False) and torch.is_grad_enabled()
+
     def _fused_norms(self, x) -> bool:
         """TF32-class mode on the GPU: residual add + LayerNorm + operand cast run as one HIP launch per sub-layer
         (ADK_MAST3R_FUSED_NORM=0 keeps the three torch kernels, for A/B measurements and the equivalence test)."""
         import os
-        if getattr(self, "_training_ops", False):   # that launch has no gradient
+        if self._records():   # that launch has no gradient
             return False
         C = x.shape[-1]   # what adk_add_layernorm takes (fused_norm.supported); anything else keeps the torch kernels
         return bool(getattr(self, "_fp32_stream", False) and x.is_cuda and self.patch_embed.proj.weight.dtype == torch.float16
@@ -536,8 +540,8 @@ class AsymmetricMASt3R(nn.Module):
     def _side_stream(self, t):
         """Second HIP stream for the independent halves of the decoder / the two heads (GPU only; ADK_MAST3R_STREAMS=0 disables)."""
         import os
-        if not t.is_cuda or os.environ.get("ADK_MAST3R_STREAMS", "1") == "0" or getattr(self, "_training_ops", False):
-            return None   # (training: what the graph keeps is freed in the order of one stream)
+        if not t.is_cuda or os.environ.get("ADK_MAST3R_STREAMS", "1") == "0" or self._records():
+            return None   # (a recorded pass: what the graph keeps is freed in the order of one stream)
         st = getattr(self, "_side", None)
         if st is None or st.device != t.device:
             st = self._side = torch.cuda.Stream(device=t.device)
@@ -583,7 +587,7 @@ class AsymmetricMASt3R(nn.Module):
         attention, rotary positions and MLPs on kernels with a gradient.  kept8 ("int8" / "e4m3"): the MLPs keep their hidden values in 8
         bits for the backward pass (an fc1 or fc2 that is hooked or replaced is called as it is, and then also keeps fc2's input; an activation
         that is, as without kept8).  The heads stay fp32.  training_forward() then gives results with a graph; forward() stays
-        without."""
+        without, and is what to_inference_dtype(dtype, fp32_stream=True) makes it."""
         if dtype not in (torch.float16, torch.bfloat16):
             raise ValueError(f"to_training_dtype: float16 or bfloat16; got {dtype}")
         if kept8 not in (None, "int8", "e4m3"):

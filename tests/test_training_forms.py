@@ -55,3 +55,36 @@ def test_values_without_a_checkpoint(shape, gated, dtype, dev):
     with torch.no_grad():
         got = a8.mlp8(*leaves, gated=gated)
     assert torch.equal(got, a8.mlp8(*leaves, gated=gated).detach()) and not got.requires_grad
+
+
+def small_model(dev):
+    from artdeco_amd.mast3r_model import AsymmetricMASt3R
+    torch.manual_seed(0)
+    net = AsymmetricMASt3R(img_size=(64, 64), enc_embed_dim=128, enc_depth=2, enc_num_heads=2, dec_embed_dim=64, dec_depth=4, dec_num_heads=1).to(dev)
+    g = torch.Generator().manual_seed(1)
+    return net, [{"img": (torch.rand(1, 3, 48, 64, generator=g) * 2 - 1).to(dev), "true_shape": torch.tensor([[48, 64]])} for _ in range(2)]
+
+
+@pytest.mark.gpu
+def test_validation_between_steps_is_the_inference_path(dev, monkeypatch):
+    """forward() of a model set up for training: the fused norms, the second stream and the trunk's bits of one set up for inference (the heads
+    are library convolutions, whose results differ by a step from call to call of one and the same model)."""
+    from artdeco_amd import fused_norm
+    net, views = small_model(dev)
+    tokens, heads = [], net.both_heads
+    monkeypatch.setattr(net, "both_heads", lambda dec1, dec2, *a: (tokens.append([*dec1, *dec2]), heads(dec1, dec2, *a))[1])
+    norms, add_layernorm = [], fused_norm.add_layernorm
+    monkeypatch.setattr(fused_norm, "add_layernorm", lambda *a, **kw: (norms.append(1), add_layernorm(*a, **kw))[1])
+    net.to_inference_dtype(torch.float16, fp32_stream=True)
+    net(*views)
+    count = len(norms)
+    net.to_training_dtype(torch.float16, kept8="int8")
+    norms.clear()
+    net(*views)
+    assert count > 0 and len(norms) == count and net._side_stream(views[0]["img"]) is None
+    with torch.no_grad():
+        assert net._side_stream(views[0]["img"]) is not None
+    assert len(tokens[0]) == 10 and all(torch.equal(a, b) for a, b in zip(*tokens))
+    norms.clear()
+    r1, r2 = net.training_forward(*views)
+    assert not norms and r1["pts3d"].requires_grad and r2["desc"].requires_grad
