@@ -170,10 +170,13 @@ class CrossAttention(nn.Module):
         self.rope = rope
 
     def _stacked_kv(self):
-        """[projk; projv] weight and bias, rebuilt whenever either parameter was replaced, cast or edited in place (inference only)."""
+        """[projk; projv] weight and bias, rebuilt whenever either parameter was replaced, cast or edited in place (inference only); on every
+        call while the block is set up for training, whose steps may change weights unseen (a replayed graph, an optimizer on .data)."""
         ps = (self.projk.weight, self.projk.bias, self.projv.weight, self.projv.bias)
         key = tuple((p.data_ptr(), -1 if p.is_inference() else p._version, p.dtype, p.device) for p in ps)
-        if getattr(self, "_kv_key", None) != key:
+        if getattr(self, "trains", False):
+            key = None
+        if key is None or getattr(self, "_kv_key", None) != key:
             with torch.no_grad():
                 self._kv = (torch.cat([ps[0], ps[2]], 0).contiguous(), torch.cat([ps[1], ps[3]], 0).contiguous())
             self._kv_key = key
@@ -578,6 +581,7 @@ class AsymmetricMASt3R(nn.Module):
             for m in root.modules():
                 if isinstance(m, (Attention, CrossAttention, Mlp)):
                     m.trains = on
+                    m._kv_key = None   # what was stacked before may be out of date when the training ends
                 if isinstance(m, Mlp):
                     m.kept8 = kept8
 

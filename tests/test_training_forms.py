@@ -88,3 +88,30 @@ def test_validation_between_steps_is_the_inference_path(dev, monkeypatch):
     norms.clear()
     r1, r2 = net.training_forward(*views)
     assert not norms and r1["pts3d"].requires_grad and r2["desc"].requires_grad
+
+
+@pytest.mark.gpu
+def test_validation_sees_the_weights_of_a_replayed_step(dev, monkeypatch):
+    """A captured step changes weights without touching their version counters: forward() between replays and after the training."""
+    net, views = small_model(dev)
+    net.to_training_dtype(torch.float16)
+    tokens, heads = [], net.both_heads
+    monkeypatch.setattr(net, "both_heads", lambda dec1, dec2, *a: (tokens.append([*dec1, *dec2]), heads(dec1, dec2, *a))[1])
+    net(*views)
+    weights = [blk.cross_attn.projk.weight for blk in (*net.dec_blocks, *net.dec_blocks2)]
+    graph = torch.cuda.CUDAGraph()
+    with torch.no_grad(), torch.cuda.graph(graph):
+        for w in weights:
+            w.mul_(-1.5)
+    for turn in ("between", "between", "after", "after one without validation"):
+        if turn == "after one without validation":
+            net.to_training_dtype(torch.float16)
+        graph.replay()
+        if turn != "between":
+            net.to_inference_dtype(torch.float16, fp32_stream=True)
+        net(*views)
+        with torch.no_grad():
+            for blk in (*net.dec_blocks, *net.dec_blocks2):
+                blk.cross_attn.projk.weight.mul_(1.0)      # seen by its version counter
+        net(*views)
+        assert all(torch.equal(a, b) for a, b in zip(tokens[-2], tokens[-1])) and not torch.equal(tokens[0][-1], tokens[-1][-1]), turn
