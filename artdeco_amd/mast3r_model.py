@@ -652,7 +652,10 @@ class AsymmetricMASt3R(nn.Module):
         return self._both_views(view1, view2)
 
     def training_forward(self, view1, view2):
-        """forward() under the caller's grad mode."""
+        """forward() under the caller's grad mode, of a model that to_training_dtype() has set up: on the GPU the inference path's rotation,
+        attention and norms give no gradient."""
+        if torch.is_grad_enabled() and view1["img"].is_cuda and not getattr(self, "_training_ops", False):
+            raise RuntimeError("training_forward: to_training_dtype() first; the inference path's kernels give no gradient")
         return self._both_views(view1, view2)
 
     def _both_views(self, view1, view2):

@@ -115,3 +115,15 @@ def test_validation_sees_the_weights_of_a_replayed_step(dev, monkeypatch):
                 blk.cross_attn.projk.weight.mul_(1.0)      # seen by its version counter
         net(*views)
         assert all(torch.equal(a, b) for a, b in zip(tokens[-2], tokens[-1])) and not torch.equal(tokens[0][-1], tokens[-1][-1]), turn
+
+
+@pytest.mark.gpu
+def test_a_model_set_up_for_inference_does_not_pretend_to_train(dev):
+    """Its kernels pass autograd by: the rotation would be missing from the gradients, or everything before the attention."""
+    net, views = small_model(dev)
+    for set_up in (lambda: None, lambda: net.to_inference_dtype(torch.float16, fp32_stream=True), lambda: (net.to_training_dtype(torch.float16), net.to_inference_dtype(torch.float16))):
+        set_up()
+        with pytest.raises(RuntimeError, match="to_training_dtype"):
+            net.training_forward(*views)
+        with torch.no_grad():
+            assert not net.training_forward(*views)[0]["pts3d"].requires_grad
