@@ -137,8 +137,13 @@ def rotary(x, positions, frequencies, *, factor=1.0, layout="half", heads=None) 
 
 def rotary_(x, positions, frequencies, *, factor=1.0, layout="half", heads=None) -> torch.Tensor:
     """rotary in place: what is not turned is not touched.  -> x."""
-    if torch.is_grad_enabled() and x.requires_grad and x.is_leaf:
-        raise _lib.AdkError("rotary_: x is a leaf that requires a gradient: turn it out of place, with rotary")
+    if torch.is_grad_enabled() and x.requires_grad:
+        # what torch refuses as well, but only when x has been turned
+        if x.is_leaf or (x._is_view() and x._base.is_leaf):
+            raise _lib.AdkError("rotary_: x is a leaf that requires a gradient, or a view of one: turn it out of place, with rotary")
+        if x._is_view() and torch._C._autograd._get_creation_meta(x) != torch._C._autograd.CreationMeta.DEFAULT:
+            raise _lib.AdkError("rotary_: x is a view that autograd does not follow in place (one of a split's, or made without grad mode): turn it out of "
+                                "place, with rotary")
     return _Rotary.apply(x, positions, frequencies, factor, layout, heads, False, True)
 
 

@@ -123,3 +123,22 @@ def test_nothing_is_kept_where_no_gradient_is_recorded(launches):
 def test_the_activations_c_entry_keeps_both_codes_and_units_or_neither(lib):
     P, N = 1 << 20, None
     assert lib.adk_activation8_fwd(P, 0, 1, 1, 0, 0, 0, P, P, N, N) == -1 and lib.adk_activation8_fwd(P, 0, 1, 1, 0, 0, 0, P, N, P, N) == -1
+
+
+def test_rotary_in_place_refuses_before_it_turns(launches):
+    """Views that autograd does not follow in place: the refusal leaves them as they are."""
+    from artdeco_amd import _lib, rotary as ro
+    f, _ = ro.rotary_frequencies(8)
+    pos, leaf = torch.arange(4), torch.randn(1, 4, 16, requires_grad=True)
+    whole = (leaf * 1).view(1, 4, 2, 8)
+    with torch.no_grad():
+        unrecorded = (leaf * 1).requires_grad_(True).view(1, 4, 2, 8)
+    for x in (leaf.view(1, 4, 2, 8), whole.split(1, 2)[0], whole.chunk(2, 2)[1], unrecorded):
+        with pytest.raises(_lib.AdkError, match="out of place|out of"):
+            ro.rotary_(x, pos, f)
+    assert not launches
+    for x in (whole, whole[:, :, :1], leaf.detach().view(1, 4, 2, 8), leaf.detach().view(1, 4, 2, 8).split(1, 2)[0]):
+        ro.rotary_(x, pos, f)
+    with torch.no_grad():
+        ro.rotary_(leaf.view(1, 4, 2, 8), pos, f)
+    assert len(launches) == 5
