@@ -68,7 +68,7 @@ def _prepare(what, q, k, v, scale, mask, key_lengths):
                  and not (qs[0] | qs[1] | qs[2] | ks[0] | ks[1] | ks[2] | vs[0] | vs[1] | vs[2]) & 7 and not (q.data_ptr() | k.data_ptr() | v.data_ptr()) & 15)
     except ValueError:
         plain = False
-    if not plain:
+    if not plain or (qs[2] | ks[2] | vs[2]) >> 24:  # (a single token far from the next is no matter)
         _refuse(what, q, k, v)
         B, H, Nq, D = q.shape
         Nk = k.shape[2]

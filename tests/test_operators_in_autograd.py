@@ -142,3 +142,16 @@ def test_rotary_in_place_refuses_before_it_turns(launches):
     with torch.no_grad():
         ro.rotary_(leaf.view(1, 4, 2, 8), pos, f)
     assert len(launches) == 5
+
+
+def test_a_single_token_has_no_token_stride(monkeypatch):
+    """One position of a sequence-major cache of a large batch: its token stride is past the kernels' 2^24 elements and used by nothing."""
+    import ctypes
+    from artdeco_amd import _lib, attention as att
+    strides = []
+    monkeypatch.setattr(_lib, "require_cuda", lambda *tensors: None)
+    monkeypatch.setattr(_lib, "launch", lambda fn, what, device, *args: strides.append(list((ctypes.c_int64 * 13).from_address(args[14]))))
+    far = torch.empty(2 * 4 * 64, dtype=torch.float16).as_strided((2, 4, 1, 64), (256, 64, 1 << 24, 1))
+    att.attend_forward(far, far, far)
+    att.attend_forward(torch.empty(2, 4, 1, 64, dtype=torch.float16), far, far)
+    assert [s[2::3][:3] for s in strides] == [[0, 0, 0]] * 2
