@@ -73,6 +73,8 @@ def _prepare(what, q, k, v, scale, mask, key_lengths):
         B, H, Nq, D = q.shape
         Nk = k.shape[2]
         qs, ks, vs = _strides(q), _strides(k), _strides(v)
+    if (B | H | Nq | Nk) >> 31:
+        raise _lib.AdkError(f"{what}: batch, heads and tokens are counted in 31 bits; got q {tuple(q.shape)}, k {tuple(k.shape)}")
     if scale is None:
         scale = D ** -0.5
     elif not 0.0 < scale < 1e37:

@@ -57,6 +57,8 @@ def _turn(x, y, positions, frequencies, factor, layout, heads, transpose):
         raise _lib.AdkError(f"rotary: x [B,N,H,D] is required; got {tuple(x.shape)}") from None
     dtype, device = x.dtype, x.device
     xb, xn, xh, xd = x.stride()
+    if (B | N | H | D) >> 31:
+        raise _lib.AdkError(f"rotary: batch, tokens, heads and channels are counted in 31 bits; got {tuple(shape)}")
     if dtype not in _DTYPES:
         raise _lib.AdkError(f"rotary: float16, bfloat16 and float32 are supported; got {dtype}")
     if xd != 1 and D > 1:

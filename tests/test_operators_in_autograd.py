@@ -155,3 +155,18 @@ def test_a_single_token_has_no_token_stride(monkeypatch):
     att.attend_forward(far, far, far)
     att.attend_forward(torch.empty(2, 4, 1, 64, dtype=torch.float16), far, far)
     assert [s[2::3][:3] for s in strides] == [[0, 0, 0]] * 2
+
+
+@pytest.mark.parametrize("n", [2 ** 31, 2 ** 32 + 1])
+def test_sizes_past_31_bits_are_refused(n, launches):
+    """They would reach the library cut to 32 bits: 2^32 + 1 tokens as one."""
+    from artdeco_amd import _lib, attention as att, rotary as ro
+    one = torch.zeros(1, 1, 1, 8, dtype=torch.float16)
+    f, _ = ro.rotary_frequencies(2)
+    for q, k in ((one.expand(1, 1, n, 8), one), (one, one.expand(1, 1, n, 8)), (one.expand(n, 1, 1, 8), one.expand(n, 1, 1, 8)), (one.expand(1, n, 1, 8), one)):
+        with pytest.raises(_lib.AdkError, match="31 bits"):
+            att.attend_forward(q, k, k)
+    for shape in ((1, n, 1, 2), (n, 1, 1, 2), (1, 1, n, 2)):
+        with pytest.raises(_lib.AdkError, match="31 bits"):
+            ro.rotary(one[..., :2].expand(shape), torch.zeros(1, dtype=torch.int64).expand(shape[1]), f)
+    assert not launches
