@@ -230,7 +230,7 @@ struct A8Call {
 template <typename T, int KIND, bool E4M3, bool GATED> static int a8_launch(const A8Call& c, bool forward, hipStream_t stream) {
     const int64_t chunks = forward ? ceil_div(c.n, 32) * 4 : GATED ? c.n / (2 * c.width) * ceil_div(c.width, 8) : ceil_div(c.n, 8);
     const int64_t blocks = ceil_div(chunks, 256);
-    if (blocks > 0x7fffffff) return ADK_EUNSUPPORTED;
+    if (blocks > 0xffffff) return ADK_EUNSUPPORTED; // a launch has fewer than 2^32 threads
     if (forward)
         hipLaunchKernelGGL((a8_fwd_kernel<T, KIND, E4M3, GATED>), dim3((unsigned)blocks), dim3(256), 0, stream, static_cast<const T*>(c.x), c.n, c.width,
                            static_cast<T*>(c.y), c.codes, c.units);

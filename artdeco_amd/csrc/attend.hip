@@ -1263,8 +1263,8 @@ extern "C" int adk_attend_bwd(const void* dout, const void* q, const void* k, co
         a.tops = reinterpret_cast<uint32_t*>(a.delta + rows);
         a.unit_blocks = adk::at_unit_blocks((int64_t)a.G * Nq, Nk);
         a.delta_blocks = dtype == 0 ? B * Hk * a.unit_blocks : (int)adk::ceil_div(rows, AT_DELTA_ROWS);
+        if (a.delta_blocks + (a.mask ? adk::ceil_div(adk::at_mask_waves(a), 4) : 0) > 0xffffff) return ADK_EUNSUPPORTED; // a launch has fewer than 2^32 threads
         if (a.mask) {
-            if (a.delta_blocks + adk::at_mask_waves(a) / 4 > 0x7ffffff0ll) return ADK_EUNSUPPORTED;
             a.by_row = a.tops + (int64_t)B * Hk * a.unit_blocks;
             a.by_key = a.by_row + (adk::at_mask_set(a, B - 1, H - 1) + 1) * adk::at_words(Nk) * a.mask_rows;
             need += adk_attend_mask_bytes(B, H, Nq, Nk, strides + 9);

@@ -127,7 +127,7 @@ template <typename T, int W> static int rotary_launch(RotaryArgs& a, int half, h
     if (per_token <= 0) return 0;
     if (per_token > 0x7fffffff) return ADK_EUNSUPPORTED;
     const int64_t blocks = per_token <= 256 ? ceil_div(a.tokens, 256 / per_token) : a.tokens * ceil_div(per_token, 256);
-    if (blocks > 0x7fffffff) return ADK_EUNSUPPORTED;
+    if (blocks > 0xffffff) return ADK_EUNSUPPORTED; // a launch has fewer than 2^32 threads
     if (half) hipLaunchKernelGGL((rotary_kernel<T, W, true>), dim3((unsigned)blocks), dim3(256), 0, stream, a);
     else hipLaunchKernelGGL((rotary_kernel<T, W, false>), dim3((unsigned)blocks), dim3(256), 0, stream, a);
     ADK_RETURN_LAST_ERROR();

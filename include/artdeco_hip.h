@@ -317,7 +317,8 @@ int adk_attention_fwd_f16(const void* q, const void* k, const void* v, void* out
  * lies behind is never read, its dk and dv are 0.  mask or NULL: one byte a pair, 1 shows and 0 hides it, no other value (a
  * stride of 0 broadcasts).  A query without a visible key: out 0, lse -inf, no gradient.  scale > 0.  No atomics: the same bits on every run.
  * ws: *_workspace_bytes() bytes (may be 0), in the backward with a mask adk_attend_mask_bytes() more (of the mask's four
- * strides), 16-byte aligned, contents free after the call.
+ * strides), 16-byte aligned, contents free after the call.  ADK_EUNSUPPORTED
+ * where a launch would take 2^24 workgroups: from about 2^28 rows on.
  */
 int64_t adk_attend_fwd_workspace_bytes(int B, int H, int Hk, int Nq, int Nk, int D);
 int adk_attend_fwd(const void* q, const void* k, const void* v, void* out, float* lse, const int32_t* key_lengths, const uint8_t* mask,
@@ -345,7 +346,8 @@ int adk_rotary(const void* x, void* y, const int64_t* positions, const double* f
  * Forward: y = act(x), x [rows, width]; gated: act(x[:, :width]) * x[:, width:], x [rows, 2 width]; and x as codes, 32 consecutive
  * values of the contiguous tensor sharing the power of two 2^(units - 127).  kind 0 = gelu, 1 = gelu (tanh), 2 = silu; format 0 =
  * int8, 1 = e4m3; dtype 0 = float16, 1 = float32, 2 = bfloat16.  codes: n values rounded up to a multiple of 32 bytes, 8-byte
- * aligned; units: one byte for each 32; both NULL in the forward where nothing is to be kept.  Backward: dx in x's shape and, unless NULL, the activation of the held values
+ * aligned; units: one byte for each 32; both NULL in the forward where nothing is to be kept.  Fewer than 2^35
+ * values (ADK_EUNSUPPORTED).  Backward: dx in x's shape and, unless NULL, the activation of the held values
  * (again, y's shape).  All contiguous.  No reference counterpart (croco/models/blocks.py: Mlp is the activation's place).
  */
 int adk_activation8_fwd(const void* x, int dtype, int64_t rows, int64_t width, int kind, int gated, int format, void* y, uint8_t* codes,

@@ -170,3 +170,16 @@ def test_sizes_past_31_bits_are_refused(n, launches):
         with pytest.raises(_lib.AdkError, match="31 bits"):
             ro.rotary(one[..., :2].expand(shape), torch.zeros(1, dtype=torch.int64).expand(shape[1]), f)
     assert not launches
+
+
+def test_c_entries_refuse_launches_that_the_grid_does_not_hold(lib):
+    """2^24 workgroups of 256 threads are 2^32 threads: refused before a launch (of several, the first would be missing)."""
+    import ctypes
+    P, N = 1 << 20, None
+    assert lib.adk_activation8_fwd(P, 0, 1 << 20, 1 << 16, 0, 0, 0, P, P, P, N) == -3
+    assert lib.adk_activation8_bwd(P, P, P, 0, 1 << 20, 1 << 16, 0, 0, 0, P, N, N) == -3
+    odd = (ctypes.c_int64 * 9)(256 << 26, 257, 257, 256 << 26, 257, 257, 0, 1, 0)
+    assert lib.adk_rotary(P, P, P, P, 0, 1, 1 << 26, 1, 256, 1, 128, 1, 1, 0, 1.0, odd, N) == -3
+    strides = (ctypes.c_int64 * 25)(*[8] * 9, 0, 0, 1, 0, *[8] * 12)
+    for dtype, mask, rows in ((0, N, 1 << 28), (2, N, 1 << 28), (2, P, (1 << 28) - 64)):
+        assert lib.adk_attend_bwd(P, P, P, P, P, P, N, mask, dtype, 1, 1, 1, rows, 1, 8, strides, 1.0, 0, P, P, P, P, 1 << 60, N) == -3, (dtype, mask, rows)
