@@ -189,11 +189,14 @@ struct AtMask32 {
             }
         }
     }
-    __device__ __forceinline__ uint32_t bits() const { // bytes of 0 or 1: sums of powers of two
+    // 128 for a byte that is not 0: a boolean tensor may be a view of any bytes, of 0 and 255 say (2 % of a masked call: 517 x 1031 x 12/4 heads,
+    // D 80, 42.9 -> 43.9 us)
+    static __device__ __forceinline__ uint32_t shown(uint32_t x) { return (((x & 0x7f7f7f7fu) + 0x7f7f7f7fu) | x) & 0x80808080u; }
+    __device__ __forceinline__ uint32_t bits() const { // sums of powers of two, times 128
         typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
-        const uint32_t lo = __builtin_amdgcn_udot4(x[1], 0x80402010u, __builtin_amdgcn_udot4(x[0], 0x08040201u, 0u, false), false);
-        const uint32_t hi = __builtin_amdgcn_udot4(x[3], 0x80402010u, __builtin_amdgcn_udot4(x[2], 0x08040201u, 0u, false), false);
-        const uint32_t mine = lo | hi << 8;
+        const uint32_t lo = __builtin_amdgcn_udot4(shown(x[1]), 0x80402010u, __builtin_amdgcn_udot4(shown(x[0]), 0x08040201u, 0u, false), false);
+        const uint32_t hi = __builtin_amdgcn_udot4(shown(x[3]), 0x80402010u, __builtin_amdgcn_udot4(shown(x[2]), 0x08040201u, 0u, false), false);
+        const uint32_t mine = lo >> 7 | hi << 1;
         const u32x2 both = __builtin_amdgcn_permlane32_swap(mine, mine, false, false); // lane c's and lane c + 32's
         return both.x | both.y << 16;
     }

@@ -314,11 +314,11 @@ int adk_attention_fwd_f16(const void* q, const void* k, const void* v, void* out
  * dout, dq, dk, dv: 13 and 25 numbers.  The tensors' strides are multiples of 8, their last dimension dense, their pointers
  * 16-byte aligned (out 8-byte in the forward).
  * causal: query i sees keys j <= i + Nk - Nq.  key_lengths [B] int32 or NULL: sequence b has keys below key_lengths[b]; what
- * lies behind is never read, its dk and dv are 0.  mask or NULL: one byte a pair, 1 shows and 0 hides it, no other value (a
+ * lies behind is never read, its dk and dv are 0.  mask or NULL: one byte a pair, 0 hides it, any other value shows it (a
  * stride of 0 broadcasts).  A query without a visible key: out 0, lse -inf, no gradient.  scale > 0.  No atomics: the same bits on every run.
  * ws: *_workspace_bytes() bytes (may be 0), in the backward with a mask adk_attend_mask_bytes() more (of the mask's four
- * strides), 16-byte aligned, contents free after the call.  ADK_EUNSUPPORTED
- * where a launch would take 2^24 workgroups: from about 2^28 rows on.
+ * strides), 16-byte aligned, contents free after the call.  ADK_EUNSUPPORTED where a launch would take 2^24
+ * workgroups: from about 2^28 rows on.
  */
 int64_t adk_attend_fwd_workspace_bytes(int B, int H, int Hk, int Nq, int Nk, int D);
 int adk_attend_fwd(const void* q, const void* k, const void* v, void* out, float* lse, const int32_t* key_lengths, const uint8_t* mask,

@@ -127,3 +127,24 @@ def test_a_model_set_up_for_inference_does_not_pretend_to_train(dev):
             net.training_forward(*views)
         with torch.no_grad():
             assert not net.training_forward(*views)[0]["pts3d"].requires_grad
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("size", [(2, 4, 2, 77, 150, 64), (1, 24, 24, 300, 1133, 96), (8, 8, 2, 1, 700, 128)], ids=str)
+def test_masks_of_any_bytes(size, dev):
+    """A boolean view of bytes other than 0 and 1 shows what the same mask of 0 and 1 shows, side by side in memory and apart."""
+    from artdeco_amd import attention as att
+    B, H, Hk, Nq, Nk, D = size
+    g = torch.Generator().manual_seed(3)
+    q, do = (torch.randn(B, H, Nq, D, generator=g).bfloat16().to(dev) for _ in range(2))
+    k, v = (torch.randn(B, Hk, Nk, D, generator=g).bfloat16().to(dev) for _ in range(2))
+    flat = do.transpose(1, 2).reshape(B, Nq, H * D)
+    values = torch.tensor([0, 255, 2, 0, 128, 1, 0, 254], dtype=torch.uint8)
+    for shape in ((B, 1, Nq, Nk), (B, 1, 1, Nk), (1, 1, Nk, Nq)):
+        raw = values[torch.randint(0, 8, shape, generator=g)].to(dev)
+        raw = raw.transpose(2, 3) if shape[2] == Nk else raw
+        results = []
+        for mask in (raw != 0, raw.view(torch.bool)):
+            out, lse = att.attend_forward(q, k, v, mask=mask)
+            results.append((out, lse, *att.attend_backward(flat, q, k, v, out, lse, mask=mask)))
+        assert all(torch.equal(a, b) for a, b in zip(*results)), shape
