@@ -596,6 +596,11 @@ class AsymmetricMASt3R(nn.Module):
             raise ValueError(f"to_training_dtype: float16 or bfloat16; got {dtype}")
         if kept8 not in (None, "int8", "e4m3"):
             raise ValueError(f"to_training_dtype: kept8 is None, int8 or e4m3; got {kept8!r}")
+        for m in self.modules():   # whatever an earlier to_inference_dtype() narrowed: norms and heads
+            if isinstance(m, nn.LayerNorm):
+                m.float()
+        self.downstream_head1.float()
+        self.downstream_head2.float()
         self.to_inference_dtype(dtype, fp32_stream=True)
         self._set_training_ops(True, kept8)
         return self

@@ -148,3 +148,17 @@ def test_masks_of_any_bytes(size, dev):
             out, lse = att.attend_forward(q, k, v, mask=mask)
             results.append((out, lse, *att.attend_backward(flat, q, k, v, out, lse, mask=mask)))
         assert all(torch.equal(a, b) for a, b in zip(*results)), shape
+
+
+@pytest.mark.parametrize("first", [dict(dtype=torch.bfloat16), dict(dtype=torch.float16, fp32_stream=True, heads=True)], ids=["trunk", "heads"])
+def test_training_after_a_narrower_inference(first):
+    """Norms and heads are fp32 again, whatever to_inference_dtype() had narrowed."""
+    from artdeco_amd.mast3r_model import AsymmetricMASt3R
+    net = AsymmetricMASt3R(img_size=(32, 32), enc_embed_dim=64, enc_depth=1, enc_num_heads=1, dec_embed_dim=64, dec_depth=4, dec_num_heads=1)
+    net.to_inference_dtype(**first)
+    net.to_training_dtype(torch.bfloat16)
+    for name, p in net.named_parameters():
+        trunk = name.startswith(("enc_blocks", "dec_blocks", "patch_embed", "decoder_embed")) and "norm" not in name
+        assert p.dtype == (torch.bfloat16 if trunk else torch.float32), name
+    view = {"img": torch.rand(1, 3, 32, 32)}
+    assert net.training_forward(view, view)[0]["pts3d"].requires_grad
