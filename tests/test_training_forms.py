@@ -162,3 +162,50 @@ def test_training_after_a_narrower_inference(first):
         assert p.dtype == (torch.bfloat16 if trunk else torch.float32), name
     view = {"img": torch.rand(1, 3, 32, 32)}
     assert net.training_forward(view, view)[0]["pts3d"].requires_grad
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("gated", [False, True])
+def test_mlp8_of_some_gradients(gated, dtype, dev):
+    """Frozen parameters and inputs, every combination of two kinds: the gradients that are asked for are those of the full call; without biases,
+    those of biases of zero."""
+    from artdeco_amd import activation8 as a8
+    leaves, grad = mlp_leaves(dev, dtype, gated)
+    grad = grad.to(dtype)
+    full = torch.autograd.grad(a8.mlp8(*leaves, kind="silu", gated=gated), leaves, grad)
+    for asked in ([0], [1], [2], [3], [4], [0, 3], [1, 2], [3, 4], [0, 1, 2], [1, 2, 3, 4]):
+        some = [t.detach().requires_grad_(i in asked) for i, t in enumerate(leaves)]
+        got = torch.autograd.grad(a8.mlp8(*some, kind="silu", gated=gated), [some[i] for i in asked], grad)
+        assert all(torch.equal(g, full[i]) for g, i in zip(got, asked)), asked
+    x, w1, b1, w2, b2 = leaves
+    zeros = [torch.zeros_like(b1).requires_grad_(True), torch.zeros_like(b2).requires_grad_(True)]
+    bare, filled = a8.mlp8(x, w1, None, w2, None, gated=gated), a8.mlp8(x, w1, zeros[0], w2, zeros[1], gated=gated)
+    assert torch.equal(bare, filled)
+    for a, b in zip(torch.autograd.grad(bare, (x, w1, w2), grad), torch.autograd.grad(filled, (x, w1, w2), grad)):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("heads,kv_heads,D", [(6, 2, 64), (4, 1, 40), (3, 3, 128)])
+def test_attend_packed_with_masks_and_lengths(heads, kv_heads, D, dtype, dev):
+    """One projection's heads, fewer of keys than of queries: the bits of attend_forward and attend_backward on its three views, whatever hides."""
+    from artdeco_amd import attention as att
+    B, N = 3, 77
+    g = torch.Generator().manual_seed(6)
+    qkv = torch.randn(B, N, heads + 2 * kv_heads, D, generator=g).to(dtype).to(dev).requires_grad_(True)
+    do = torch.randn(B, N, heads * D, generator=g).to(dtype).to(dev)
+    lengths = torch.tensor([N, 0, 31], dtype=torch.int32, device=dev)
+    free = (torch.rand(B, heads, N, N, generator=g) < 0.6).to(dev)
+    wide = torch.zeros(B, 1, N, 2 * N, dtype=torch.bool, device=dev)
+    wide[..., ::2] = free[:, :1]
+    for mask in (None, free, free[:, :1], free[:1, :1, :1], wide[..., ::2]):
+        for how in (dict(mask=mask), dict(mask=mask, key_lengths=lengths), dict(mask=mask, key_lengths=lengths, causal=True, scale=0.3)):
+            out = att.attend_packed(qkv, heads, kv_heads, **how)
+            got, = torch.autograd.grad(out, qkv, do)
+            t = qkv.detach().transpose(1, 2)
+            q, k, v = t[:, :heads], t[:, heads:heads + kv_heads], t[:, heads + kv_heads:]
+            o, lse = att.attend_forward(q, k, v, **how)
+            want = torch.cat([s.transpose(1, 2) for s in att.attend_backward(do, q, k, v, o, lse, **how)], 2)
+            assert torch.equal(out, o) and torch.equal(got, want), how.keys()
