@@ -2,8 +2,9 @@
 
 A float16 MLP layer keeps fc1's output for the activation's gradient and the activation's output for fc2's weight gradient: 4 bytes a
 hidden value.  Here the forward pass leaves one code a value, 32 consecutive values sharing a power of two (33/32 byte a value), and the
-backward pass takes both from it.  int8 holds a value to 1/254 .. 1/127 of its block's largest, e4m3 to 1/16 of itself; forward
-results are exact, gradients are those of the held values."""
+backward pass takes both from it.  int8 holds a value to 1/254 .. 1/127 of its block's largest, e4m3 to 1/16 of itself, at best to 2^-18
+of its block's largest (smaller ones are held as 0).  Forward results are those of the values as they are, worked out in 32 bits and rounded
+once; gradients are those of the held values."""
 from __future__ import annotations
 
 import math
@@ -63,7 +64,7 @@ def _forward(x, kind, gated, format, keep):
 
 def activation8_forward(x, *, kind="gelu", gated=False, format="int8"):
     """-> (act(x), or act(gate) * up for x's halves, in x's type; x as Packed8), outside autograd.  x contiguous, float16, bfloat16 or
-    float32.  Infinities are held as the format's largest value in their block, NaN as NaN."""
+    float32, fewer than 2^35 values.  Infinities are held as the format's largest value in their block, NaN as NaN."""
     return _forward(x, kind, gated, format, True)
 
 

@@ -6,7 +6,7 @@
 //              gives act(z) (times z_up) again, which the weight gradient of the layer behind reads: y need not be kept either
 //
 // The unit is a power of two so that x / 2^e is exact and the code is the format's one rounding to nearest even: int8 holds x to
-// 2^(e-1), e4m3 to 2^-4 of itself.  An infinity is held as the format's largest value, a NaN as 0x7f (e4m3) or -128 (int8); they
+// 2^(e-1), e4m3 to 2^-4 of itself and at best to 2^(e-10), its smallest steps (below that, 2^-18 of the block's largest, 0).  An infinity is held as the format's largest value, a NaN as 0x7f (e4m3) or -128 (int8); they
 // do not count for the unit.
 //
 // Bound by memory: forward 2 accesses and 33/32 byte a value, backward 33/32 byte and 2 to 3 accesses.  A thread takes 8 values;
