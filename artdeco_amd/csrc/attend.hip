@@ -534,11 +534,11 @@ static __device__ __forceinline__ void at_mask_bits(const AttendArgs& a, int64_t
 // fp16 holds dS = P (dP - delta) in a power of two that the launch also prepares: |dP - delta| is at most 2 |dO_i| |v_j| (2-norms; o is a mean
 // of the v), P at most 1, so the unit takes twice the largest |dO| times the largest |v| of a key head to 2^15 and nothing can leave fp16's
 // range.  An even softmax over 8192 keys then has its dS around 2^15 / 8192 / sqrt(D), about 2^-2, twelve binary places above the end of
-// fp16's normal range.  (For dQ the unit is the row's own, at_bwd_rows.)  Both norms are of the key head's own rows and keys, so what a sequence gets does not depend on its neighbours in the
-// batch; rows that see no key, keys behind the length or hidden by a mask over keys, and what is not finite do not count.  (What a free mask
-// hides from every query does: values there of more than some thousand times the others' size cost those bits.)  bf16 has fp32's range
-// and needs none.  The pass over V: 8 x 768 x 16 heads, D 64, 9.7 -> 13.0 us, 38 MB where it had been 25; where V is most
-// of what there is, one query for each of 64 x 8 heads of 512 keys, the whole backward pass 57 -> 63 us.
+// fp16's normal range.  (For dQ the unit is the row's own, at_bwd_rows.)  Both norms are of the key head's own rows and keys, so what a sequence
+// gets does not depend on its neighbours in the batch; rows that see no key, keys behind the length or hidden by a mask over keys, and
+// what is not finite do not count.  (What a free mask hides from every query does: values there of more than some thousand times the
+// others' size cost those bits.)  bf16 has fp32's range and needs none.  The pass over V: 8 x 768 x 16 heads, D 64, 9.7 -> 13.0 us, 38 MB
+// where it had been 25; where V is most of what there is, one query for each of 64 x 8 heads of 512 keys, the whole backward pass 57 -> 63 us.
 #define AT_DELTA_ROWS 16
 #define AT_DELTA_KEYS 64
 typedef unsigned short at_u16x2 __attribute__((ext_vector_type(2))); // exponents (biased) of the largest |dO|^2 and |v|^2
@@ -689,7 +689,8 @@ template <typename T, int DP, bool MASKED, int SHAPE, bool SPLIT> __device__ __f
         for (int ks = 0; ks < DP / 16; ++ks) { qf[ks] = at_global_frag<T>(qp, ks, lane, a.D); gf[ks] = at_global_frag<T>(gp, ks, lane, a.D); }
     }
     const int64_t at = ((int64_t)b * a.Hk + kh) * R + rowc;
-    // a row's dQ depends on no other row: its unit is its own (one for the key head cost a row of 1e-3 of the largest 2e-3 of its dQ at 8192 keys)
+    // a row's dQ depends on no other row: its unit is its own (one for the key head cost the rows beside one 3e5 times as large 3 % of their
+    // dQ at 8192 keys)
     const float unit = __is_same(T, _Float16) ? at_unit(at_row_exponent<T, DP>(gf), value_top) : 1.f;
     const float lse = a.lse[at], neg_lse = lse == -INFINITY ? -INFINITY : -lse * 1.4426950408889634f, neg_delta = -a.delta[at] * unit;
     at_f32x16 acc[DP / 32] = {};

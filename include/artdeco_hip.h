@@ -315,7 +315,8 @@ int adk_attention_fwd_f16(const void* q, const void* k, const void* v, void* out
  * 16-byte aligned (out 8-byte in the forward).
  * causal: query i sees keys j <= i + Nk - Nq.  key_lengths [B] int32 or NULL: sequence b has keys below key_lengths[b]; what
  * lies behind is never read, its dk and dv are 0.  mask or NULL: one byte a pair, 0 hides it, any other value shows it (a
- * stride of 0 broadcasts).  A query without a visible key: out 0, lse -inf, no gradient.  scale > 0.  No atomics: the same bits on every run.
+ * stride of 0 broadcasts).  A query without a visible key: out 0, lse -inf, no gradient (of a
+ * finite dout).  scale > 0.  No atomics: the same bits on every run.
  * ws: *_workspace_bytes() bytes (may be 0), in the backward with a mask adk_attend_mask_bytes() more (of the mask's four
  * strides), 16-byte aligned, contents free after the call.  ADK_EUNSUPPORTED where a launch would take 2^24
  * workgroups: from about 2^28 rows on.
